@@ -1,4 +1,5 @@
-"""ctypes binding of libspecmoe_mi355x.so (the C ABI in include/specmoe_mi355x.h).
+"""ctypes binding of libspecmoe_mi355x.so (the C ABI in include/specmoe_mi355x.h and
+include/specmoe_mi355x_products.h).
 
 The library is built in-tree by ``ae_amd.build``. Loading fails loudly when it is missing:
 there is no fallback implementation of any entry point.
@@ -97,6 +98,29 @@ SIGNATURES = [
     ("smx_stream_read", ctypes.c_int, [_c_void_p, _sz, _sz, _c_void_p, _c_void_p]),
 ]
 
+# The same for include/specmoe_mi355x_products.h.
+_product = [_c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i64]  # x, stride, dtype, rows, K, weight, stride
+PRODUCT_SIGNATURES = [
+    ("smx_linear_workspace_size", _sz, [_i64, _i64, _i64, _i64, _i32, _i32]),
+    ("smx_linear", ctypes.c_int,
+     _product + [_i64, _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _sz,
+                 _c_void_p]),
+    ("smx_grouped_linear", ctypes.c_int,
+     _product + [_i64, _i64, _i64, _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                 _i32, _c_void_p, _i64, _c_void_p, _c_void_p, _sz, _c_void_p]),
+    ("smx_linear_grad_workspace_size", _sz, [_i64, _i64, _i64, _i64, _i32, _i32]),
+    ("smx_linear_grad", ctypes.c_int,
+     [_c_void_p, _i64, _c_void_p] + _product + [_i64, _i32, _c_void_p, _c_void_p, _c_void_p,
+                                                _c_void_p, _sz, _c_void_p]),
+    ("smx_grouped_linear_grad", ctypes.c_int,
+     [_c_void_p, _i64, _c_void_p] + _product + [_i64, _i64, _i64, _i32, _c_void_p, _i64, _c_void_p,
+                                                _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz,
+                                                _c_void_p]),
+]
+
+# enum smx_activation
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
+
 _lock = threading.Lock()
 _lib = None
 
@@ -127,7 +151,7 @@ def lib() -> ctypes.CDLL:
             # see torch's device context.
             import torch  # noqa: F401
             handle = ctypes.CDLL(LIB_PATH)
-            for name, restype, argtypes in SIGNATURES:
+            for name, restype, argtypes in SIGNATURES + PRODUCT_SIGNATURES:
                 fn = getattr(handle, name)
                 fn.restype = restype
                 fn.argtypes = argtypes

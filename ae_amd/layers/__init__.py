@@ -7,6 +7,7 @@ from .fused_moe_kernel import (fp32_gemm_outputs_fp16, fused_down_max_tokens, fu
                                set_routing_in_gateup,
                                set_tiled_min_tokens, stack_fused_moe, stack_fused_moe_shared,
                                tiled_min_tokens)
+from .linear import fused_linear, grouped_linear
 from .layernorm import RMSNorm, add_rmsnorm_gate
 from .mixtral_moe import MixtralMoE
 from .moe_layer import PostAttentionMoE, moe_layer_forward
@@ -18,7 +19,7 @@ __all__ = [
     "fused_moe_shared_forward", "moe_align_block_size", "stack_fused_moe",
     "stack_fused_moe_shared", "MixtralMoE",
     "SharedExpertMoE", "Qwen2MoeSparseMoeBlock", "DeepseekV2MoE", "fused_topk", "grouped_topk",
-    "select_experts",
+    "select_experts", "fused_linear", "grouped_linear",
     "RMSNorm", "add_rmsnorm_gate", "PostAttentionMoE", "moe_layer_forward",
     "set_tiled_min_tokens", "tiled_min_tokens", "set_fused_down_max_tokens",
     "fused_down_max_tokens", "set_fp32_gemm_outputs_fp16", "fp32_gemm_outputs_fp16",
