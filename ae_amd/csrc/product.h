@@ -272,42 +272,52 @@ __device__ __forceinline__ void store4(char* base, int64_t at, int left, bool ve
   }
 }
 
-// Output columns col .. col + 3 of one row: product + bias -> z, activation, residual, one rounding.
+// The bias of a column group of four (gated: of gate and up columns), and the residual of a row's.
 template <int DT>
-__device__ __forceinline__ void finish4(const ProductArgs& a, const ProductItem& it, int64_t row, int col, f32x4 v) {
-  const int left = a.out_cols - col;
+__device__ __forceinline__ f32x4 bias4(const ProductArgs& a, const ProductItem& it, int col, int left) {
+  if (a.bias == nullptr || left <= 0) return f32x4{0.f, 0.f, 0.f, 0.f};
+  return load4<DT>(a.bias, it.w * a.bias_ld + col, left, a.vec);
+}
+template <int DT>
+__device__ __forceinline__ f32x4 res4(const ProductArgs& a, int64_t row, int col, int left) {
+  if (a.res == nullptr || left <= 0) return f32x4{0.f, 0.f, 0.f, 0.f};
+  return load4<DT>(a.res, row * a.res_ld + col, left, a.vec);
+}
+
+// Output columns col .. col + 3 of one row: product + bias -> z, activation, residual, one rounding. `left` of them
+// exist.
+template <int DT>
+__device__ __forceinline__ void finish4(const ProductArgs& a, const ProductItem& it, int64_t row, int col, int left,
+                                        f32x4 v, const f32x4& bias, const f32x4& res) {
   if (left <= 0) return;
-  const bool vec = a.vec;
-  if (a.bias != nullptr) v += load4<DT>(a.bias, it.w * a.bias_ld + col, left, vec);
-  if (a.z != nullptr) store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, vec, v);
+  if (a.bias != nullptr) v += bias;
+  if (a.z != nullptr) store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, a.vec, v);
   if (a.act != kActNone) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = activate(a.act, v[e]);
   }
-  if (a.res != nullptr) v += load4<DT>(a.res, row * a.res_ld + col, left, vec);
-  store4<DT>(a.out, it.g * a.out_group + row * a.out_ld + col, left, vec, v);
+  if (a.res != nullptr) v += res;
+  store4<DT>(a.out, it.g * a.out_group + row * a.out_ld + col, left, a.vec, v);
 }
 
 // The same of a gated product: gate and up columns of outputs col .. col + 3.
 template <int DT>
-__device__ __forceinline__ void finish4_gated(const ProductArgs& a, const ProductItem& it, int64_t row, int col,
-                                              f32x4 gate, f32x4 up) {
-  const int left = a.out_cols - col;
+__device__ __forceinline__ void finish4_gated(const ProductArgs& a, int64_t row, int col, int left, f32x4 gate, f32x4 up,
+                                              const f32x4& gate_bias, const f32x4& up_bias, const f32x4& res) {
   if (left <= 0) return;
-  const bool vec = a.vec;
   if (a.bias != nullptr) {
-    gate += load4<DT>(a.bias, it.w * a.bias_ld + col, left, vec);
-    up += load4<DT>(a.bias, it.w * a.bias_ld + a.out_cols + col, left, vec);
+    gate += gate_bias;
+    up += up_bias;
   }
   if (a.z != nullptr) {
-    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, vec, gate);
-    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + a.out_cols + col, left, vec, up);
+    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, a.vec, gate);
+    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + a.out_cols + col, left, a.vec, up);
   }
   f32x4 v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = activate(kActSilu, gate[e]) * up[e];
-  if (a.res != nullptr) v += load4<DT>(a.res, row * a.res_ld + col, left, vec);
-  store4<DT>(a.out, row * a.out_ld + col, left, vec, v);
+  if (a.res != nullptr) v += res;
+  store4<DT>(a.out, row * a.out_ld + col, left, a.vec, v);
 }
 
 // Rows of no group (before the first, behind the last, of a group without weights): the residual's row, or zeros.
@@ -336,9 +346,14 @@ __device__ __forceinline__ void fill_rows(const ProductArgs& a, int fb) {
 // Launchers. Sizes and alignments that a kernel assumes are checked by the plan (products.hip) that chooses it.
 struct TileShape {
   int bm, bn;   // output rows and columns of a workgroup (product columns: gated outputs take two)
-  bool staged;  // operands go through registers: any alignment. Otherwise straight into LDS
+  bool staged;  // operands go through registers: any alignment. Otherwise straight into LDS (whole 16-byte slots)
 };
 hipError_t launch_product_tile(int dtype, bool p_strided, bool q_strided, bool depth_groups, const TileShape& t,
                                const ProductArgs& a, hipStream_t s);
+
+
+// 256 x 256 tiles, 16-bit types, sizes and pitches in whole 16-byte slots.
+hipError_t launch_product_wide(int dtype, bool p_strided, bool q_strided, bool depth_groups, const ProductArgs& a,
+                               hipStream_t s);
 
 }  // namespace smx

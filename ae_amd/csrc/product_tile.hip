@@ -50,10 +50,11 @@ struct Stage {
       // Transposing read of 8 bytes per lane: the 16 lanes of a group address four rows of 16
       // elements (lane r: row r / 4, elements 4 (r % 4) ..); lane r receives element r of each.
       u32x2 h[2];
+      const int k = 8 * g + (r >> 2);
+      const char* base = reinterpret_cast<const char*>(st) + (k * kRowSlots + perm(k, (row >> 3) + ((r & 3) >> 1))) * 16 + 8 * (r & 1);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int k = 32 * u + 8 * g + 4 * j + (r >> 2);
-        const char* at = reinterpret_cast<const char*>(st + k * kRowSlots + perm(k, (row >> 3) + ((r & 3) >> 1))) + 8 * (r & 1);
+        const char* at = base + (32 * u + 4 * j) * kRowSlots * 16;
         h[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) i16x4*)(at)));
       }
@@ -123,40 +124,52 @@ struct Waves {
   static_assert(kNI >= 2 && kNI % 2 == 0 && kNJ >= 1, "column tiles in pairs");
 };
 
-// Row of P that column q of a tile stands for, relative to the tile's first. Gated: 16 gate columns, then the
-// matching 16 up columns (out_cols further), and so on.
-__device__ __forceinline__ int64_t p_row(const ProductArgs& a, int q) {
-  return a.gated ? ((q >> 5) << 4) + (q & 15) + ((q >> 4) & 1) * static_cast<int64_t>(a.out_cols) : q;
-}
-
-// Epilogue of a wave's accumulators; c0: first product column of the tile (gated: twice its first output column).
-template <int DT, int NI, int NJ>
-__device__ __forceinline__ void finish_tile(const ProductArgs& a, const ProductItem& it, int c0, int wrow, int wcol,
-                                            const f32x4 (&acc)[NI][NJ]) {
+// Epilogue of a wave's accumulators: through its part of LDS, CJ row tiles at a time, as rows of 4 NI 16-byte slots
+// (slot s of row r at s ^ r, modulo the row: no bank conflicts), from which a lane takes four columns (gated: the gate
+// and up columns of four outputs) of some rows. The bias then stays in registers, stores cover whole row pieces, and
+// the activation's code stands once.
+// c0: first product column of the tile (gated: 16 gate columns, the matching 16 up columns, and so on: twice the
+// first output column). wrow, wcol: the wave's place in the tile.
+template <int DT, int NI, int NJ, int CJ>
+__device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductItem& it, int c0, int wrow, int wcol,
+                                            u32x4* lds, const f32x4 (&acc)[NI][NJ]) {
+  constexpr int kS = 4 * NI;  // slots of a row
+  static_assert(NJ % CJ == 0, "whole chunks");
+  f32x4* st = reinterpret_cast<f32x4*>(lds);
   const int lane = lane_id();
+  // lanes side by side along a row: one per output column quad
+  const int quads = a.gated ? kS / 2 : kS;
+  const int c = lane & (quads - 1), rr = lane / quads, rows = kWave / quads;
+  const int s0 = a.gated ? (c >> 2) * 8 + (c & 3) : c;
+  const int col = a.gated ? (c0 + wcol) / 2 + 4 * c : c0 + wcol + 4 * c;
+  const int left = a.out_cols - col;
+  const bool part = a.splits > 1;
+  const f32x4 bias0 = part ? f32x4{} : bias4<DT>(a, it, col, left);
+  const f32x4 bias1 = part || !a.gated ? f32x4{} : bias4<DT>(a, it, a.out_cols + col, left);
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int r = wrow + j * 16 + (lane & 15);
-    if (r >= it.m) continue;
-    const int64_t row = it.row + r;
-    if (a.splits > 1) {
-      float* dst = a.part + (static_cast<int64_t>(it.split) * a.rows + row) * a.cols;
+  for (int j0 = 0; j0 < NJ; j0 += CJ) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int q = wcol + i * 16 + 4 * (lane >> 4);
-        const int col = (a.gated ? c0 / 2 : c0) + static_cast<int>(p_row(a, q));
-        const int end = a.gated && !((q >> 4) & 1) ? a.out_cols : a.cols;
-        if (col < end) store4<kF32>(reinterpret_cast<char*>(dst), col, end - col, a.cols % 4 == 0 && a.out_cols % 4 == 0, acc[i][j]);
+    for (int j = 0; j < CJ; ++j)
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        st[(j * 16 + (lane & 15)) * kS + ((4 * i + (lane >> 4)) ^ (lane & (kS - 1) & 15))] = acc[i][j0 + j];
+#pragma unroll 2
+    for (int y = rr; y < CJ * 16; y += rows) {
+      const int r = wrow + j0 * 16 + y;
+      const f32x4 v = st[y * kS + (s0 ^ (y & (kS - 1) & 15))];
+      const f32x4 u = a.gated ? st[y * kS + ((s0 + 4) ^ (y & (kS - 1) & 15))] : f32x4{};
+      if (r >= it.m) continue;
+      const int64_t row = static_cast<int64_t>(it.row) + r;
+      if (part) {
+        const int64_t at = (static_cast<int64_t>(it.split) * a.rows + row) * a.cols + col;
+        const bool vec = a.cols % 4 == 0 && a.out_cols % 4 == 0;
+        if (left > 0) store4<kF32>(reinterpret_cast<char*>(a.part), at, left, vec, v);
+        if (left > 0 && a.gated) store4<kF32>(reinterpret_cast<char*>(a.part), at + a.out_cols, left, vec, u);
+      } else if (a.gated) {
+        finish4_gated<DT>(a, row, col, left, v, u, bias0, bias1, res4<DT>(a, row, col, left));
+      } else {
+        finish4<DT>(a, it, row, col, left, v, bias0, res4<DT>(a, row, col, left));
       }
-    } else if (a.gated) {
-      if constexpr (NI % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < NI; i += 2)
-          finish4_gated<DT>(a, it, row, (c0 + wcol) / 2 + i * 8 + 4 * (lane >> 4), acc[i][j], acc[i + 1][j]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) finish4<DT>(a, it, row, c0 + wcol + i * 16 + 4 * (lane >> 4), acc[i][j]);
     }
   }
 }
@@ -238,7 +251,152 @@ __global__ __launch_bounds__(kPThreads) void product_staged_kernel(ProductArgs a
         for (int j = 0; j < W::kNJ; ++j) acc[i][j] = Elem<DT>::mfma(fp[i], fq[j], acc[i][j]);
     }
   }
-  finish_tile<DT>(a, it, c0, wrow, wcol, acc);
+  __syncthreads();
+  u32x4* mine = (wave < 2 ? sp : sq) + (wave & 1) * (GP::kSlots / 2);
+  static_assert(GP::kSlots == GQ::kSlots, "a square tile");
+  constexpr int kChunk = GP::kSlots / 2 / (W::kNI * 64);
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
+}
+
+// Copies of one operand's steps straight into LDS: copy j of wave w fills stage slots 64 (4 j + w) .. in lane order.
+template <int DT, int R, bool ST>
+struct TileCopy {
+  using G = Stage<DT, R, ST>;
+  const char* base;
+  int64_t step_bytes;
+  uint32_t off[G::kLoads];
+  int k[G::kLoads];  // the lane's first contraction element within a step
+  // at(y): byte offset of the operand's row y (contiguous); last: byte offset of its last whole slot (strided)
+  template <typename At>
+  __device__ __forceinline__ void init(int wave, int64_t pitch, At&& at, int last) {
+    step_bytes = ST ? G::kDepth * pitch : kPStep;
+#pragma unroll
+    for (int j = 0; j < G::kLoads; ++j) {
+      const int p = 64 * (kPWaves * j + wave) + lane_id();
+      const int y = p / G::kRowSlots, s = G::perm(y, p % G::kRowSlots);
+      k[j] = ST ? y : s * G::kEps;
+      off[j] = ST ? static_cast<uint32_t>(y * pitch) + min(s * 16, last) : at(y) + s * 16;
+    }
+  }
+  // Elements of the step from contraction index `left` on are left out (zeros); left <= 0: nothing is read.
+  __device__ __forceinline__ void copy(u32x4* st, int wave, int step, int left) const {
+    const auto r = make_rsrc(base + step * step_bytes, left > 0 ? kPOutside : 0u);
+#pragma unroll
+    for (int j = 0; j < G::kLoads; ++j) {
+      const uint32_t o = k[j] < left ? off[j] : kPOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(st + (j * kPWaves + wave) * kWave), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+__device__ __forceinline__ void bare_barrier() {  // without a memory fence, which would wait for the copies
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The same tile with the operands copied straight into LDS, two stages: while one step is multiplied the next one's
+// copies are under way, and the other workgroups of the CU cover the waits.
+template <int DT, int BM, int BN, bool PS, bool QS, bool DG>
+__global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArgs a) {
+  using GP = Stage<DT, BN, PS>;
+  using GQ = Stage<DT, BM, QS>;
+  using W = Waves<BM, BN>;
+  constexpr int64_t kEs = GP::kEs;
+  const int b = static_cast<int>(blockIdx.x);
+  if (b >= a.item_blocks) {
+    fill_rows<DT>(a, b - a.item_blocks);
+    return;
+  }
+  ProductItem it;
+  const int col_tiles = (a.gated ? (a.out_cols + BN / 2 - 1) / (BN / 2) : (a.cols + BN - 1) / BN);
+  if (!(DG ? find_depth_item(a, b, BM, col_tiles, it) : find_row_item(a, b, BM, col_tiles, it))) return;
+  __shared__ u32x4 p0[GP::kSlots], p1[GP::kSlots], q0[GQ::kSlots], q1[GQ::kSlots];
+
+  const int c0 = it.ct * BN;
+  const int cfirst = a.gated ? c0 / 2 : c0;
+  const int wave = wave_id();
+  const int64_t p_pitch = a.p_ld * kEs, q_pitch = a.q_ld * kEs;
+  TileCopy<DT, BN, PS> cp;
+  TileCopy<DT, BM, QS> cq;
+  cp.base = a.p + (DG ? int64_t{0} : it.w * a.p_group * kEs) + (PS ? it.k0 * p_pitch + cfirst * kEs : cfirst * p_pitch);
+  cq.base = a.q + (QS ? it.k0 * q_pitch + it.row * kEs : it.row * q_pitch);
+  const int plast = a.out_cols - 1 - cfirst;  // columns past the last: the last one again (not stored)
+  cp.init(wave, p_pitch, [&](int q) -> uint32_t {
+    const int64_t row = a.gated ? min(((q >> 5) << 4) + (q & 15), plast) + ((q >> 4) & 1) * static_cast<int64_t>(a.out_cols)
+                                : static_cast<int64_t>(min(q, plast));
+    return static_cast<uint32_t>(row * p_pitch);
+  }, static_cast<int>((a.cols - cfirst) * kEs) - 16);
+  cq.init(wave, q_pitch, [&](int q) -> uint32_t { return static_cast<uint32_t>(min(q, it.m - 1) * q_pitch); },
+          static_cast<int>((a.rows - it.row) * kEs) - 16);
+
+  const int steps = (it.depth + GP::kDepth - 1) / GP::kDepth;
+  const int s0 = it.split * a.split_steps;
+  const int s1 = a.splits > 1 ? min(steps, s0 + a.split_steps) : steps;
+  const int wrow = (wave / W::kColWaves) * W::kNJ * 16, wcol = (wave % W::kColWaves) * W::kNI * 16;
+  f32x4 acc[W::kNI][W::kNJ];
+#pragma unroll
+  for (int i = 0; i < W::kNI; ++i)
+#pragma unroll
+    for (int j = 0; j < W::kNJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int kCopies = GP::kLoads + GQ::kLoads;
+  auto copy = [&](u32x4* sp, u32x4* sq, int s) {
+    const int left = s < s1 ? it.depth - s * GP::kDepth : 0;
+    cp.copy(sp, wave, s, left);
+    cq.copy(sq, wave, s, left);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](u32x4* sp, u32x4* sq, int s) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kCopies));  // this step's copies have landed, the next one's may be under way
+    bare_barrier();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      u32x4 fp[W::kNI], fq[W::kNJ];
+#pragma unroll
+      for (int i = 0; i < W::kNI; ++i) fp[i] = GP::frag(sp, wcol + i * 16, u);
+#pragma unroll
+      for (int j = 0; j < W::kNJ; ++j) fq[j] = GQ::frag(sq, wrow + j * 16, u);
+#pragma unroll
+      for (int i = 0; i < W::kNI; ++i)
+#pragma unroll
+        for (int j = 0; j < W::kNJ; ++j) acc[i][j] = Elem<DT>::mfma(fp[i], fq[j], acc[i][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    bare_barrier();  // every wave has read the stage (its fragments are in registers: the MFMAs are issued)
+    copy(sp, sq, s + 2);
+  };
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  __builtin_amdgcn_sched_barrier(0);
+  copy(p0, q0, s0);
+  copy(p1, q1, s0 + 1);
+  for (int s = s0; s < s1; s += 2) {
+    step(p0, q0, s);
+    step(p1, q1, s + 1);  // past the end: zeros (a branch here costs waits for all copies)
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // copies past the end write zeros into the stages
+  __syncthreads();
+  u32x4* mine = wave == 0 ? p0 : wave == 1 ? p1 : wave == 2 ? q0 : q1;
+  constexpr int kMine = GP::kSlots < GQ::kSlots ? GP::kSlots : GQ::kSlots;
+  constexpr int kChunk = kMine / (W::kNI * 64);
+  static_assert(kChunk >= 1, "a row tile of the wave fits its LDS");
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
+}
+
+template <int DT, int BM, int BN>
+static hipError_t copied_launch(bool ps, bool qs, bool dg, const ProductArgs& a, hipStream_t s) {
+  const unsigned blocks = static_cast<unsigned>(a.item_blocks + a.fill_blocks);
+  // whole 16-byte slots: the contraction of a contiguous operand, the columns (rows) of a strided one
+  constexpr int n = 16 / dtype_bytes(DT);
+  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0) return hipErrorInvalidValue;
+  if ((!ps || !qs) && a.depth % n != 0) return hipErrorInvalidValue;
+  if ((ps && a.cols % n != 0) || (qs && a.rows % n != 0)) return hipErrorInvalidValue;
+  if (!ps && !qs && !dg) product_copied_kernel<DT, BM, BN, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
+  else if (ps && !qs && !dg) product_copied_kernel<DT, BM, BN, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
+  else if constexpr (BM == BN) {
+    if (ps && qs && dg) product_copied_kernel<DT, BM, BN, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
+    else return hipErrorInvalidValue;
+  } else return hipErrorInvalidValue;
+  return hipGetLastError();
 }
 
 template <int DT, int BM, int BN>
@@ -253,6 +411,9 @@ static hipError_t staged_launch(bool ps, bool qs, bool dg, const ProductArgs& a,
 
 template <int DT>
 static hipError_t tile_launch(bool ps, bool qs, bool dg, const TileShape& t, const ProductArgs& a, hipStream_t s) {
+  if (!t.staged && t.bm == 128 && t.bn == 128) return copied_launch<DT, 128, 128>(ps, qs, dg, a, s);
+  if (!t.staged && t.bm == 64 && t.bn == 128) return copied_launch<DT, 64, 128>(ps, qs, dg, a, s);
+  if (!t.staged && t.bm == 32 && t.bn == 128) return copied_launch<DT, 32, 128>(ps, qs, dg, a, s);
   if (t.staged && t.bm == 64 && t.bn == 64) return staged_launch<DT, 64, 64>(ps, qs, dg, a, s);
   if (t.staged && t.bm == 128 && t.bn == 128) return staged_launch<DT, 128, 128>(ps, qs, dg, a, s);
   return hipErrorInvalidValue;

@@ -3,6 +3,7 @@
 #include "../../include/specmoe_mi355x.h"
 #include "../../include/specmoe_mi355x_products.h"
 #include <algorithm>
+#include <cmath>
 
 #include "product.h"
 
@@ -144,8 +145,9 @@ __global__ __launch_bounds__(kPThreads) void join_kernel(ProductArgs a, int spli
     v += load4<kF32>(part, at, left, vec);
     if (a.gated) u += load4<kF32>(part, at + a.out_cols, left, vec);
   }
-  if (a.gated) finish4_gated<DT>(a, it, row, col, v, u);
-  else finish4<DT>(a, it, row, col, v);
+  const f32x4 bias = bias4<DT>(a, it, col, left), res = res4<DT>(a, row, col, left);
+  if (a.gated) finish4_gated<DT>(a, row, col, left, v, u, bias, bias4<DT>(a, it, a.out_cols + col, left), res);
+  else finish4<DT>(a, it, row, col, left, v, bias, res);
 }
 
 namespace {
@@ -167,8 +169,57 @@ struct ProductPlan {
   int64_t part_bytes = 0;
 };
 
-ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64_t depth, int64_t groups, bool gated) {
+// Tiles of the copied kernels with the time of one contraction step (us, 128 bytes of it) when 1, 2, .. workgroups run
+// on a CU, as many as fit (bf16, 4096 x 4096 weight, 1 to 8192 rows).
+struct TileCost {
+  int bm, bn, fit;
+  float step[4];
+};
+constexpr TileCost kTileCosts[] = {
+    {256, 256, 1, {1.6f, 0.f, 0.f, 0.f}},
+    {128, 128, 2, {0.70f, 1.06f, 0.f, 0.f}},
+    {64, 128, 3, {0.46f, 0.66f, 0.97f, 0.f}},
+    {32, 128, 4, {0.38f, 0.50f, 0.75f, 0.96f}},
+};
+constexpr int kCUs = 256;
+
+// slots: both operands consist of whole 16-byte slots (see launch_product_*).
+ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64_t depth, int64_t groups, bool gated,
+                         bool slots) {
   ProductPlan p;
+  if (!slots || rows == 0) return p;
+  const bool depth_groups = kind == kWeightGrad;
+  const double mean_depth = depth_groups ? static_cast<double>(depth) / groups : static_cast<double>(depth);
+  const double steps = std::max(1.0, mean_depth / (kPStep / dtype_bytes(dtype)));
+  double best = 0;
+  for (const TileCost& t : kTileCosts) {
+    if (t.bm == 256 && dtype == kF32) continue;
+    if (kind == kWeightGrad && t.bm < 128) continue;
+    // row tiles: of every group with rows, half a tile more than its rows fill
+    double row_tiles = static_cast<double>(cdiv(rows, t.bm));
+    if (!depth_groups && groups > 1) {
+      const double active = static_cast<double>(std::min(groups, rows));
+      row_tiles = std::max(active, static_cast<double>(rows) / t.bm + active / 2);
+    }
+    const double tiles = row_tiles * static_cast<double>(cdiv(cols, t.bn)) * (depth_groups ? groups : 1);
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (t.bm == 256 || (depth_groups && groups > 1) || splits * 4 > steps)) break;
+      double per_cu = std::ceil(tiles * splits / kCUs), time = 0;
+      const double len = steps / splits + 6;  // and the ends of a tile
+      time += std::floor(per_cu / t.fit) * t.step[t.fit - 1] * len;
+      const int rest = static_cast<int>(per_cu) % t.fit;
+      if (rest > 0) time += t.step[rest - 1] * len;
+      if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch, partial sums out and in
+      if (best == 0 || time < best) {
+        best = time;
+        p.tile = TileShape{t.bm, t.bn, false};
+        const int64_t all = cdiv(depth, kPStep / dtype_bytes(dtype));
+        p.split_steps = static_cast<int>(cdiv(all, splits));
+        p.splits = splits == 1 ? 1 : static_cast<int>(cdiv(all, p.split_steps));
+        p.part_bytes = p.splits > 1 ? p.splits * rows * cols * 4 : 0;
+      }
+    }
+  }
   return p;
 }
 
@@ -189,7 +240,9 @@ int run_product(Kind kind, int dtype, const ProductPlan& plan, ProductArgs& a, b
   a.split_steps = plan.split_steps;
   a.item_blocks = static_cast<int>(items);
   a.fill_blocks = plan.splits > 1 ? 0 : fills;
-  hipError_t err = launch_product_tile(dtype, kind != kForward, kind == kWeightGrad, depth_groups, plan.tile, a, s);
+  hipError_t err = plan.tile.bm == 256
+                       ? launch_product_wide(dtype, kind != kForward, kind == kWeightGrad, depth_groups, a, s)
+                       : launch_product_tile(dtype, kind != kForward, kind == kWeightGrad, depth_groups, plan.tile, a, s);
   if (err != hipSuccess || plan.splits == 1) return static_cast<int>(err);
   const int splits = a.splits;
   a.splits = 1;
@@ -232,10 +285,15 @@ struct GradLayout {
   int64_t dz = 0, dz_ld = 0, sums = 0, part = 0, total = 0;
 };
 
-GradLayout grad_layout(const Sizes& z) {
+// Whole 16-byte slots: the base and the pitch, and the length of whatever lies side by side.
+bool whole_slots(const void* base, int64_t pitch, int64_t length, int64_t es) {
+  return aligned(base, 16) && pitch * es % 16 == 0 && length * es % 16 == 0;
+}
+
+GradLayout grad_layout(const Sizes& z, bool dx_slots, bool dw_slots) {
   GradLayout l;
-  l.dx = plan_product(kInputGrad, z.dtype, z.rows, z.K, z.Nw, z.G, false);
-  l.dw = plan_product(kWeightGrad, z.dtype, z.Nw, z.K, z.rows, z.G, false);
+  l.dx = plan_product(kInputGrad, z.dtype, z.rows, z.K, z.Nw, z.G, false, dx_slots);
+  l.dw = plan_product(kWeightGrad, z.dtype, z.Nw, z.K, z.rows, z.G, false, dw_slots);
   l.dz_ld = cdiv(z.Nw, 16 / z.es) * (16 / z.es);
   int64_t at = 0;
   if (z.act != SMX_ACT_NONE) at += align256(z.rows * l.dz_ld * z.es);
@@ -287,7 +345,9 @@ int forward(const Sizes& z, const void* x, int64_t x_stride, const void* weight,
   if (!aligned(x, z.es) || !aligned(weight, z.es) || !aligned(y, z.es) || !aligned(bias, z.es) ||
       !aligned(residual, z.es) || !aligned(preact, 4))
     return SMX_ERR_MISALIGNED;
-  const ProductPlan plan = plan_product(kForward, z.dtype, z.rows, z.Nw, z.K, z.G, z.Nw != z.N);
+  const bool slots = whole_slots(x, x_stride, z.K, z.es) && whole_slots(weight, weight_stride, z.K, z.es) &&
+                     g.stride * z.es % 16 == 0;
+  const ProductPlan plan = plan_product(kForward, z.dtype, z.rows, z.Nw, z.K, z.G, z.Nw != z.N, slots);
   if (plan.part_bytes > 0) {
     if (!workspace || workspace_bytes < static_cast<size_t>(plan.part_bytes)) return SMX_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return SMX_ERR_MISALIGNED;
@@ -327,7 +387,12 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
   if (rc == SMX_OK) rc = check_pitch(dy_stride, z.N, z.es);
   if (rc != SMX_OK) return rc;
   if (g.slots && (grad_weight || grad_bias)) return SMX_ERR_INVALID_ARG;
-  const GradLayout l = grad_layout(z);
+  // dz is dy itself, or rows of whole slots in the workspace
+  const bool own_dz = z.act != SMX_ACT_NONE;
+  const bool dz_slots = z.Nw * z.es % 16 == 0 && (own_dz || whole_slots(dy, dy_stride, z.N, z.es));
+  const bool dx_slots = dz_slots && whole_slots(weight, weight_stride, z.K, z.es) && g.stride * z.es % 16 == 0;
+  const bool dw_slots = dz_slots && whole_slots(x, x_stride, z.K, z.es);
+  const GradLayout l = grad_layout(z, dx_slots, dw_slots);
   if (l.dz_ld * z.es > kPMaxPitch || z.K * z.es > kPMaxPitch) return SMX_ERR_UNSUPPORTED;
   if (z.rows > 0) {
     if (!dy || (grad_weight && !x) || (grad_x && !weight) || (z.act != SMX_ACT_NONE && !preact)) return SMX_ERR_INVALID_ARG;
@@ -431,7 +496,9 @@ extern "C" {
 size_t smx_linear_workspace_size(int64_t rows, int64_t K, int64_t N, int64_t G, int activation, int dtype) {
   Sizes z;
   if (check_sizes(rows, K, N, G, activation, dtype, z) != SMX_OK) return 0;
-  return static_cast<size_t>(plan_product(kForward, dtype, rows, z.Nw, K, z.G, z.Nw != N).part_bytes);
+  // whatever the alignment
+  return static_cast<size_t>(std::max(plan_product(kForward, dtype, rows, z.Nw, K, z.G, z.Nw != N, true).part_bytes,
+                                      plan_product(kForward, dtype, rows, z.Nw, K, z.G, z.Nw != N, false).part_bytes));
 }
 
 int smx_linear(const void* x, int64_t x_stride, int dtype, int64_t rows, int64_t K, const void* weight,
@@ -460,7 +527,7 @@ int smx_grouped_linear(const void* x, int64_t x_stride, int dtype, int64_t rows,
 size_t smx_linear_grad_workspace_size(int64_t rows, int64_t K, int64_t N, int64_t G, int activation, int dtype) {
   Sizes z;
   if (check_sizes(rows, K, N, G, activation, dtype, z) != SMX_OK) return 0;
-  return static_cast<size_t>(grad_layout(z).total);
+  return static_cast<size_t>(std::max(grad_layout(z, true, true).total, grad_layout(z, false, false).total));
 }
 
 int smx_linear_grad(const void* dy, int64_t dy_stride, const float* preact, const void* x, int64_t x_stride, int dtype,
