@@ -20,7 +20,7 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_NAME = "libspecmoe_mi355x.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["routing.hip", "experts.hip", "layer1.hip", "tiles.hip", "wide.hip", "capi.hip", "transfer.hip",
-           "stream_probe.hip", "products.hip", "product_tile.hip", "product_wide.hip"]
+           "stream_probe.hip", "products.hip", "product_tile.hip", "product_wide.hip", "product_rows.hip"]
 ARCH = "gfx950"
 
 # Packed-fp32 VALU forms are disabled for every HIP translation unit (the host pass warns

@@ -16,6 +16,8 @@
 // 16 x 16 tile.
 #pragma once
 
+#include <type_traits>
+
 #include "expert_items.h"
 
 namespace smx {
@@ -63,6 +65,9 @@ struct ProductArgs {
 // Groups
 // ---------------------------------------------------------------------------------------
 
+// The maps as constant memory (no kernel writes them): where the group is the same for the wave, a scalar load.
+typedef const __attribute__((address_space(4))) int64_t* ConstMap;
+
 // Row bounds of group g, inside [0, total] and in order whatever the caller's bounds hold.
 __device__ __forceinline__ void group_bounds(const ProductArgs& a, int g, int total, int& lo, int& n) {
   if (a.offsets == nullptr) {
@@ -70,7 +75,8 @@ __device__ __forceinline__ void group_bounds(const ProductArgs& a, int g, int to
     n = total;
     return;
   }
-  const int64_t b0 = a.offsets[g], b1 = a.offsets[g + 1];
+  const ConstMap offsets = (ConstMap)(a.offsets);
+  const int64_t b0 = offsets[g], b1 = offsets[g + 1];
   const int64_t c0 = min(max(b0, int64_t{0}), static_cast<int64_t>(total));
   const int64_t c1 = min(max(b1, c0), static_cast<int64_t>(total));
   lo = static_cast<int>(c0);
@@ -80,7 +86,7 @@ __device__ __forceinline__ void group_bounds(const ProductArgs& a, int g, int to
 // The group's P, or -1: a slot outside the pool holds no weights, and its rows are of no group.
 __device__ __forceinline__ int64_t group_weight(const ProductArgs& a, int g) {
   if (a.slots == nullptr) return g;
-  const int64_t s = a.slots[g];
+  const int64_t s = ((ConstMap)(a.slots))[g];
   return s >= 0 && s < a.weights ? s : -1;
 }
 
@@ -134,13 +140,14 @@ __device__ __forceinline__ bool find_row_item(const ProductArgs& a, int b, int b
     return true;
   }
   const int lane = lane_id();
-  int rt = 0, lo = 0, n = 0, incl = 0;
+  int rt = 0, lo = 0, n = 0, incl = 0, w = 0;
   auto scan = [&](int base) {
     const int g = base + lane;
     lo = n = 0;
     if (g < a.groups) {
+      w = static_cast<int>(group_weight(a, g));  // (the host checks that there are fewer than 2^31)
       group_bounds(a, g, a.rows, lo, n);
-      if (a.slots != nullptr && group_weight(a, g) < 0) n = 0;
+      if (w < 0) n = 0;
     }
     incl = wave_incl_scan((n + bm - 1) / bm);
   };
@@ -162,8 +169,8 @@ __device__ __forceinline__ bool find_row_item(const ProductArgs& a, int b, int b
       it.g = base + l;
       it.row = __builtin_amdgcn_readlane(lo, l) + (r - first) * bm;
       it.m = min(bm, __builtin_amdgcn_readlane(n, l) - (r - first) * bm);
-      it.w = uniform64(group_weight(a, it.g));
-      return it.w >= 0;
+      it.w = __builtin_amdgcn_readlane(w, l);
+      return true;
     }
     before += here;
   }
@@ -192,40 +199,132 @@ __device__ __forceinline__ bool find_depth_item(const ProductArgs& a, int b, int
 // Epilogue
 // ---------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float sigmoid_f32(float z) { return 1.0f / (1.0f + expf(-z)); }
-// Normal distribution function by the complementary error function: relative accuracy in the left tail.
-__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(z * -0.70710678f); }
-// gelu's tanh form is z * sigmoid(2 u), u = sqrt(2 / pi) (z + 0.044715 z^3).
-__device__ __forceinline__ float gelu_tanh_2u(float z) { return 1.59576912f * fmaf(0.044715f * z * z, z, z); }
+// fp32 results: the library's exponential and complementary error function and IEEE quotients (an ulp or two).
+// 16-bit results (step 2^-8 or 2^-11): the hardware's exponential and reciprocal, and the normal distribution function in
+// the tail as exp(-z^2 / 2) times a polynomial in t = 1 / (1 + 0.36 |z|), fitted here to the least relative error
+// over |z| <= 14 (1.2e-6 in fp32, the tail's own relative accuracy kept): 5 to 17 operations instead of 25 to 60 per
+// value, which one wave per SIMD does not hide (256 x 256 tiles, 8192 x 4096 -> 14336: gelu_tanh cost 206 us
+// of 1062, gelu 280 of 1136).
+constexpr float kLog2e = 1.44269504f;
+constexpr float kTanh0 = 1.59576912f, kTanh1 = 0.0713548163f;  // gelu's tanh form: z * sigmoid(z (kTanh0 + kTanh1 z^2))
 
+template <bool EXACT>
+__device__ __forceinline__ float sigmoid_f32(float z) {
+  if constexpr (EXACT) return 1.0f / (1.0f + expf(-z));
+  else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -kLog2e));
+}
+// exp(-z^2 / 2).
+template <bool EXACT>
+__device__ __forceinline__ float bell_f32(float z) {
+  if constexpr (EXACT) return expf(-0.5f * z * z);
+  else return __builtin_amdgcn_exp2f(z * z * (-0.5f * kLog2e));
+}
+// Normal distribution function of -|z|, bell = exp(-z^2 / 2).
+template <bool EXACT>
+__device__ __forceinline__ float normal_tail(float z, float bell) {
+  if constexpr (EXACT) {
+    return 0.5f * erfcf(fabsf(z) * 0.70710678f);
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.36f, fabsf(z), 1.0f));
+    float p = 0.0470067784f;
+    p = fmaf(p, t, -0.179588974f);
+    p = fmaf(p, t, 0.180709541f);
+    p = fmaf(p, t, 0.0267180651f);
+    p = fmaf(p, t, 0.139659077f);
+    p = fmaf(p, t, 0.141782865f);
+    p = fmaf(p, t, 0.143712372f);
+    return p * t * bell;
+  }
+}
+template <bool EXACT>
+__device__ __forceinline__ float normal_cdf(float z, float bell) {
+  const float c = normal_tail<EXACT>(z, bell);
+  return z > 0.0f ? 1.0f - c : c;
+}
+
+template <bool EXACT>
 __device__ __forceinline__ float activate(int act, float z) {
   switch (act) {
     case kActRelu: return z < 0.0f ? 0.0f : z;
-    case kActGelu: return z * normal_cdf(z);
-    case kActGeluTanh: return z * sigmoid_f32(gelu_tanh_2u(z));
-    case kActSilu: return z * sigmoid_f32(z);
+    case kActGelu: return z * normal_cdf<EXACT>(z, bell_f32<EXACT>(z));
+    case kActGeluTanh: return z * sigmoid_f32<EXACT>(z * fmaf(kTanh1 * z, z, kTanh0));
+    case kActSilu: return z * sigmoid_f32<EXACT>(z);
     default: return z;
   }
 }
 
+// The activation of N groups of four (one branch for all of them: the operations of different values overlap).
+template <bool EXACT, int N>
+__device__ __forceinline__ void activate_all(int act, f32x4 (&v)[N]) {
+  auto each = [&](auto code) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[n][e] = activate<EXACT>(decltype(code)::value, v[n][e]);
+  };
+  switch (act) {
+    case kActRelu: each(std::integral_constant<int, kActRelu>{}); break;
+    case kActGelu: each(std::integral_constant<int, kActGelu>{}); break;
+    case kActGeluTanh: each(std::integral_constant<int, kActGeluTanh>{}); break;
+    case kActSilu: each(std::integral_constant<int, kActSilu>{}); break;
+    default: break;
+  }
+}
+
 // d act / dz. The slope terms vanish faster than any power of z grows: 0 where they underflow, also at infinity.
+template <bool EXACT>
 __device__ __forceinline__ float activate_grad(int act, float z) {
   switch (act) {
     case kActRelu: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
     case kActGelu: {
-      const float e = expf(-0.5f * z * z);
-      return e == 0.0f ? normal_cdf(z) : fmaf(z, 0.398942280f * e, normal_cdf(z));
+      const float e = bell_f32<EXACT>(z), c = normal_cdf<EXACT>(z, e);
+      return e == 0.0f ? c : fmaf(z, 0.398942280f * e, c);
     }
     case kActGeluTanh: {
-      const float s = sigmoid_f32(gelu_tanh_2u(z)), t = s * (1.0f - s);
-      return t == 0.0f ? s : fmaf(z * t, 1.59576912f * fmaf(3.0f * 0.044715f * z, z, 1.0f), s);
+      const float s = sigmoid_f32<EXACT>(z * fmaf(kTanh1 * z, z, kTanh0)), t = s * (1.0f - s);
+      return t == 0.0f ? s : fmaf(z * t, fmaf(3.0f * kTanh1 * z, z, kTanh0), s);
     }
     case kActSilu: {
-      const float s = sigmoid_f32(z), t = s * (1.0f - s);
+      const float s = sigmoid_f32<EXACT>(z), t = s * (1.0f - s);
       return t == 0.0f ? s : fmaf(z, t, s);
     }
     default: return 1.0f;
   }
+}
+
+// d *= d act / dz of N groups of four.
+template <bool EXACT, int N>
+__device__ __forceinline__ void activate_grad_all(int act, const f32x4 (&z)[N], f32x4 (&d)[N]) {
+  auto each = [&](auto code) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[n][e] *= activate_grad<EXACT>(decltype(code)::value, z[n][e]);
+  };
+  switch (act) {
+    case kActRelu: each(std::integral_constant<int, kActRelu>{}); break;
+    case kActGelu: each(std::integral_constant<int, kActGelu>{}); break;
+    case kActGeluTanh: each(std::integral_constant<int, kActGeluTanh>{}); break;
+    case kActSilu: each(std::integral_constant<int, kActSilu>{}); break;
+    default: break;
+  }
+}
+
+// A 16-byte slot of T's of an operand in memory, of any alignment: `have` of its elements exist, the others are 0.
+template <int DT>
+__device__ __forceinline__ u32x4 load_slot(const typename Elem<DT>::S* at, int have) {
+  using S = typename Elem<DT>::S;
+  constexpr int kEps = 16 / sizeof(S);
+  u32x4 r = {0, 0, 0, 0};
+  if (have >= kEps) {
+    __builtin_memcpy(&r, at, 16);
+  } else if (have > 0) {
+    S e[kEps];
+#pragma unroll
+    for (int i = 0; i < kEps; ++i) e[i] = i < have ? at[i] : S{};
+    __builtin_memcpy(&r, e, 16);
+  }
+  return r;
 }
 
 // Four consecutive elements of an array of T (DT), those from column `n` on left alone.
@@ -258,12 +357,10 @@ __device__ __forceinline__ void store4(char* base, int64_t at, int left, bool ve
     if constexpr (DT == kF32) {
       *reinterpret_cast<f32x4*>(s) = v;
     } else {
-      u32x2 b;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[h] = static_cast<uint32_t>(Elem<DT>::from_f32(v[2 * h])) |
-               static_cast<uint32_t>(Elem<DT>::from_f32(v[2 * h + 1])) << 16;
-      *reinterpret_cast<u32x2*>(s) = b;
+      typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+      if constexpr (DT == kBF16) *reinterpret_cast<u32x2*>(s) = __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
+      else *reinterpret_cast<u32x2*>(s) = __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4));
     }
   } else {
 #pragma unroll
@@ -284,40 +381,70 @@ __device__ __forceinline__ f32x4 res4(const ProductArgs& a, int64_t row, int col
   return load4<DT>(a.res, row * a.res_ld + col, left, a.vec);
 }
 
-// Output columns col .. col + 3 of one row: product + bias -> z, activation, residual, one rounding. `left` of them
-// exist.
-template <int DT>
-__device__ __forceinline__ void finish4(const ProductArgs& a, const ProductItem& it, int64_t row, int col, int left,
-                                        f32x4 v, const f32x4& bias, const f32x4& res) {
+// N rows' output columns col .. col + 3 (of row[n]; `left` of the columns exist, where in[n]): product + bias -> z,
+// activation, residual, one rounding.
+template <int DT, int N>
+__device__ __forceinline__ void finish_rows(const ProductArgs& a, const ProductItem& it, const int64_t (&row)[N],
+                                            const bool (&in)[N], int col, int left, f32x4 (&v)[N], const f32x4& bias,
+                                            const f32x4 (&res)[N]) {
   if (left <= 0) return;
-  if (a.bias != nullptr) v += bias;
-  if (a.z != nullptr) store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, a.vec, v);
-  if (a.act != kActNone) {
+  if (a.bias != nullptr) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = activate(a.act, v[e]);
+    for (int n = 0; n < N; ++n) v[n] += bias;
   }
-  if (a.res != nullptr) v += res;
-  store4<DT>(a.out, it.g * a.out_group + row * a.out_ld + col, left, a.vec, v);
+  if (a.z != nullptr) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (in[n]) store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, v[n]);
+  }
+  activate_all<DT == kF32>(a.act, v);
+  if (a.res != nullptr) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += res[n];
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (in[n]) store4<DT>(a.out, it.g * a.out_group + row[n] * a.out_ld + col, left, a.vec, v[n]);
 }
 
 // The same of a gated product: gate and up columns of outputs col .. col + 3.
-template <int DT>
-__device__ __forceinline__ void finish4_gated(const ProductArgs& a, int64_t row, int col, int left, f32x4 gate, f32x4 up,
-                                              const f32x4& gate_bias, const f32x4& up_bias, const f32x4& res) {
+template <int DT, int N>
+__device__ __forceinline__ void finish_rows_gated(const ProductArgs& a, const int64_t (&row)[N], const bool (&in)[N],
+                                                  int col, int left, f32x4 (&gate)[N], f32x4 (&up)[N],
+                                                  const f32x4& gate_bias, const f32x4& up_bias, const f32x4 (&res)[N]) {
   if (left <= 0) return;
   if (a.bias != nullptr) {
-    gate += gate_bias;
-    up += up_bias;
+#pragma unroll
+    for (int n = 0; n < N; ++n) gate[n] += gate_bias, up[n] += up_bias;
   }
   if (a.z != nullptr) {
-    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + col, left, a.vec, gate);
-    store4<kF32>(reinterpret_cast<char*>(a.z), row * a.z_ld + a.out_cols + col, left, a.vec, up);
-  }
-  f32x4 v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = activate(kActSilu, gate[e]) * up[e];
-  if (a.res != nullptr) v += res;
-  store4<DT>(a.out, row * a.out_ld + col, left, a.vec, v);
+    for (int n = 0; n < N; ++n) {
+      if (!in[n]) continue;
+      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, gate[n]);
+      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + a.out_cols + col, left, a.vec, up[n]);
+    }
+  }
+  activate_all<DT == kF32>(kActSilu, gate);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    gate[n] *= up[n];
+    if (a.res != nullptr) gate[n] += res[n];
+    if (in[n]) store4<DT>(a.out, row[n] * a.out_ld + col, left, a.vec, gate[n]);
+  }
+}
+
+// One row of either kind.
+template <int DT>
+__device__ __forceinline__ void finish4(const ProductArgs& a, const ProductItem& it, int64_t row, int col, int left,
+                                        const f32x4& v, const f32x4& up, const f32x4& bias, const f32x4& up_bias,
+                                        const f32x4& res) {
+  const int64_t rows[1] = {row};
+  const bool in[1] = {true};
+  const f32x4 r[1] = {res};
+  f32x4 x[1] = {v}, u[1] = {up};
+  if (a.gated) finish_rows_gated<DT, 1>(a, rows, in, col, left, x, u, bias, up_bias, r);
+  else finish_rows<DT, 1>(a, it, rows, in, col, left, x, bias, r);
 }
 
 // Rows of no group (before the first, behind the last, of a group without weights): the residual's row, or zeros.
@@ -345,15 +472,18 @@ __device__ __forceinline__ void fill_rows(const ProductArgs& a, int fb) {
 
 // Launchers. Sizes and alignments that a kernel assumes are checked by the plan (products.hip) that chooses it.
 struct TileShape {
-  int bm, bn;   // output rows and columns of a workgroup (product columns: gated outputs take two)
-  bool staged;  // operands go through registers: any alignment. Otherwise straight into LDS (whole 16-byte slots)
+  int bm, bn;  // output rows and columns of a workgroup (product columns: gated outputs take two)
+  // The kernel: operands through registers (any alignment) or straight into LDS (whole 16-byte slots)
+  enum Form { kStaged, kCopied, kWide, kRows, kRowsStaged, kShallow } form;
 };
+// kStaged: 64 x 64. kCopied: 128 x 128, and not grouped along the contraction 64 x 128, 32 x 128.
+// kShallow: 128 x 128, grouped along the contraction.
 hipError_t launch_product_tile(int dtype, bool p_strided, bool q_strided, bool depth_groups, const TileShape& t,
                                const ProductArgs& a, hipStream_t s);
-
-
-// 256 x 256 tiles, 16-bit types, sizes and pitches in whole 16-byte slots.
+// kWide: 16-bit types, 256 x 256.
 hipError_t launch_product_wide(int dtype, bool p_strided, bool q_strided, bool depth_groups, const ProductArgs& a,
                                hipStream_t s);
+// Forward, no splits. kRows: 16 x 16 (not gated), 16 x 32, 32 x 32, 64 x 64. kRowsStaged: 16 x 32, 32 x 32.
+hipError_t launch_product_rows(int dtype, const TileShape& t, const ProductArgs& a, hipStream_t s);
 
 }  // namespace smx

@@ -74,20 +74,6 @@ struct StagedLoad {
   int depth;       // contraction length
   u32x4 v[G::kLoads];
 
-  // Element `e` of a slot lies at `at[e]`; the first `have` of the kEps exist.
-  static __device__ __forceinline__ u32x4 load_slot(const S* at, int have) {
-    u32x4 r = {0, 0, 0, 0};
-    if (have >= G::kEps) {
-      __builtin_memcpy(&r, at, 16);
-    } else if (have > 0) {
-      S e[G::kEps];
-#pragma unroll
-      for (int i = 0; i < G::kEps; ++i) e[i] = i < have ? at[i] : S{};
-      __builtin_memcpy(&r, e, 16);
-    }
-    return r;
-  }
-
   template <typename RowAt>
   __device__ __forceinline__ void load(int k0, RowAt&& row_at) {
 #pragma unroll
@@ -96,10 +82,10 @@ struct StagedLoad {
       const int y = i / G::kRowSlots, s = i % G::kRowSlots;
       if constexpr (!ST) {
         const int k = k0 + s * G::kEps;
-        v[j] = y < n ? load_slot(base + row_at(y) * ld + k, depth - k) : u32x4{0, 0, 0, 0};
+        v[j] = y < n ? load_slot<DT>(base + row_at(y) * ld + k, depth - k) : u32x4{0, 0, 0, 0};
       } else {
         const int k = k0 + y;
-        v[j] = k < depth ? load_slot(base + k * ld + s * G::kEps, n - s * G::kEps) : u32x4{0, 0, 0, 0};
+        v[j] = k < depth ? load_slot<DT>(base + k * ld + s * G::kEps, n - s * G::kEps) : u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -130,7 +116,8 @@ struct Waves {
 // the activation's code stands once.
 // c0: first product column of the tile (gated: 16 gate columns, the matching 16 up columns, and so on: twice the
 // first output column). wrow, wcol: the wave's place in the tile.
-template <int DT, int NI, int NJ, int CJ>
+// PLAIN: whole sums of a weight gradient, which are only rounded and stored.
+template <int DT, int NI, int NJ, int CJ, bool PLAIN>
 __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductItem& it, int c0, int wrow, int wcol,
                                             u32x4* lds, const f32x4 (&acc)[NI][NJ]) {
   constexpr int kS = 4 * NI;  // slots of a row
@@ -143,6 +130,26 @@ __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductI
   const int s0 = a.gated ? (c >> 2) * 8 + (c & 3) : c;
   const int col = a.gated ? (c0 + wcol) / 2 + 4 * c : c0 + wcol + 4 * c;
   const int left = a.out_cols - col;
+  if constexpr (PLAIN) {
+    const int lc = lane % kS, lr = lane / kS;
+    const int pcol = c0 + wcol + 4 * lc, pleft = a.cols - pcol;
+#pragma unroll
+    for (int j0 = 0; j0 < NJ; j0 += CJ) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          st[(j * 16 + (lane & 15)) * kS + ((4 * i + (lane >> 4)) ^ (lane & (kS - 1) & 15))] = acc[i][j0 + j];
+#pragma unroll 4
+      for (int y = lr; y < CJ * 16; y += kWave / kS) {
+        const f32x4 v = st[y * kS + (lc ^ (y & (kS - 1) & 15))];
+        const int r = wrow + j0 * 16 + y;
+        if (r < it.m && pleft > 0)
+          store4<DT>(a.out, it.g * a.out_group + (static_cast<int64_t>(it.row) + r) * a.out_ld + pcol, pleft, a.vec, v);
+      }
+    }
+    return;
+  }
   const bool part = a.splits > 1;
   const f32x4 bias0 = part ? f32x4{} : bias4<DT>(a, it, col, left);
   const f32x4 bias1 = part || !a.gated ? f32x4{} : bias4<DT>(a, it, a.out_cols + col, left);
@@ -153,22 +160,34 @@ __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductI
 #pragma unroll
       for (int i = 0; i < NI; ++i)
         st[(j * 16 + (lane & 15)) * kS + ((4 * i + (lane >> 4)) ^ (lane & (kS - 1) & 15))] = acc[i][j0 + j];
-#pragma unroll 2
-    for (int y = rr; y < CJ * 16; y += rows) {
-      const int r = wrow + j0 * 16 + y;
-      const f32x4 v = st[y * kS + (s0 ^ (y & (kS - 1) & 15))];
-      const f32x4 u = a.gated ? st[y * kS + ((s0 + 4) ^ (y & (kS - 1) & 15))] : f32x4{};
-      if (r >= it.m) continue;
-      const int64_t row = static_cast<int64_t>(it.row) + r;
+    constexpr int kBatch = 4;  // rows of a lane that are finished together
+    for (int y0 = rr; y0 < CJ * 16; y0 += kBatch * rows) {
+      int64_t row[kBatch];
+      bool in[kBatch];
+      f32x4 v[kBatch], u[kBatch], res[kBatch];
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int y = y0 + n * rows, r = wrow + j0 * 16 + y;
+        in[n] = y < CJ * 16 && r < it.m && left > 0;
+        row[n] = static_cast<int64_t>(it.row) + r;
+        const int yy = y < CJ * 16 ? y : 0;
+        v[n] = st[yy * kS + (s0 ^ (yy & (kS - 1) & 15))];
+        u[n] = a.gated ? st[yy * kS + ((s0 + 4) ^ (yy & (kS - 1) & 15))] : f32x4{};
+        res[n] = res4<DT>(a, row[n], col, in[n] && !part ? left : 0);
+      }
       if (part) {
-        const int64_t at = (static_cast<int64_t>(it.split) * a.rows + row) * a.cols + col;
         const bool vec = a.cols % 4 == 0 && a.out_cols % 4 == 0;
-        if (left > 0) store4<kF32>(reinterpret_cast<char*>(a.part), at, left, vec, v);
-        if (left > 0 && a.gated) store4<kF32>(reinterpret_cast<char*>(a.part), at + a.out_cols, left, vec, u);
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          if (!in[n]) continue;
+          const int64_t at = (static_cast<int64_t>(it.split) * a.rows + row[n]) * a.cols + col;
+          store4<kF32>(reinterpret_cast<char*>(a.part), at, left, vec, v[n]);
+          if (a.gated) store4<kF32>(reinterpret_cast<char*>(a.part), at + a.out_cols, left, vec, u[n]);
+        }
       } else if (a.gated) {
-        finish4_gated<DT>(a, row, col, left, v, u, bias0, bias1, res4<DT>(a, row, col, left));
+        finish_rows_gated<DT>(a, row, in, col, left, v, u, bias0, bias1, res);
       } else {
-        finish4<DT>(a, it, row, col, left, v, bias0, res4<DT>(a, row, col, left));
+        finish_rows<DT>(a, it, row, in, col, left, v, bias0, res);
       }
     }
   }
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(kPThreads) void product_staged_kernel(ProductArgs a
   u32x4* mine = (wave < 2 ? sp : sq) + (wave & 1) * (GP::kSlots / 2);
   static_assert(GP::kSlots == GQ::kSlots, "a square tile");
   constexpr int kChunk = GP::kSlots / 2 / (W::kNI * 64);
-  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ, false>(a, it, c0, wrow, wcol, mine, acc);
 }
 
 // Copies of one operand's steps straight into LDS: copy j of wave w fills stage slots 64 (4 j + w) .. in lane order.
@@ -295,10 +314,12 @@ __device__ __forceinline__ void bare_barrier() {  // without a memory fence, whi
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The same tile with the operands copied straight into LDS, two stages: while one step is multiplied the next one's
-// copies are under way, and the other workgroups of the CU cover the waits.
-template <int DT, int BM, int BN, bool PS, bool QS, bool DG>
-__global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArgs a) {
+// The same tile with the operands copied straight into LDS. NS = 2 stages: while one step is multiplied the next one's
+// copies are under way, and the other workgroup of the CU covers the waits. One stage, for contractions of a few steps
+// (the weight gradient of groups of few rows): a workgroup is then one chain of latencies, bounds, copies, stores, and
+// four on a CU instead of two overlap them.
+template <int DT, int BM, int BN, int NS, bool PS, bool QS, bool DG>
+__global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_kernel(ProductArgs a) {
   using GP = Stage<DT, BN, PS>;
   using GQ = Stage<DT, BM, QS>;
   using W = Waves<BM, BN>;
@@ -311,7 +332,7 @@ __global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArg
   ProductItem it;
   const int col_tiles = (a.gated ? (a.out_cols + BN / 2 - 1) / (BN / 2) : (a.cols + BN - 1) / BN);
   if (!(DG ? find_depth_item(a, b, BM, col_tiles, it) : find_row_item(a, b, BM, col_tiles, it))) return;
-  __shared__ u32x4 p0[GP::kSlots], p1[GP::kSlots], q0[GQ::kSlots], q1[GQ::kSlots];
+  __shared__ u32x4 p0[GP::kSlots], q0[GQ::kSlots], p1[NS > 1 ? GP::kSlots : 1], q1[NS > 1 ? GQ::kSlots : 1];
 
   const int c0 = it.ct * BN;
   const int cfirst = a.gated ? c0 / 2 : c0;
@@ -346,8 +367,11 @@ __global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArg
     cq.copy(sq, wave, s, left);
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto step = [&](u32x4* sp, u32x4* sq, int s) {
-    __builtin_amdgcn_s_waitcnt(vmcnt_imm(kCopies));  // this step's copies have landed, the next one's may be under way
+  // one step, with the copies of the step NS later behind it; or one of the last NS, without them
+  auto step = [&](u32x4* sp, u32x4* sq, int s, auto more) {
+    // this step's copies have landed, the next one's may be under way
+    if constexpr (decltype(more)::value) __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * kCopies));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     bare_barrier();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -362,40 +386,62 @@ __global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArg
         for (int j = 0; j < W::kNJ; ++j) acc[i][j] = Elem<DT>::mfma(fp[i], fq[j], acc[i][j]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    bare_barrier();  // every wave has read the stage (its fragments are in registers: the MFMAs are issued)
-    copy(sp, sq, s + 2);
+    if constexpr (decltype(more)::value) {
+      bare_barrier();  // every wave has read the stage (its fragments are in registers: the MFMAs are issued)
+      copy(sp, sq, s + NS);
+    }
   };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   __builtin_amdgcn_sched_barrier(0);
-  copy(p0, q0, s0);
-  copy(p1, q1, s0 + 1);
-  for (int s = s0; s < s1; s += 2) {
-    step(p0, q0, s);
-    step(p1, q1, s + 1);  // past the end: zeros (a branch here costs waits for all copies)
+  const std::true_type more{};
+  const std::false_type last{};
+  if (s0 < s1) {
+    copy(p0, q0, s0);
+    if constexpr (NS == 1) {
+      for (int s = s0; s + 1 < s1; ++s) step(p0, q0, s, more);
+      step(p0, q0, s1 - 1, last);
+    } else {
+      copy(p1, q1, s0 + 1);
+      int s = s0;
+      for (; s + 2 < s1; s += 2) {
+        step(p0, q0, s, more);
+        step(p1, q1, s + 1, more);
+      }
+      // (a step past the end multiplies zeros: a branch inside the loop costs waits for all copies)
+      step(p0, q0, s, last);
+      step(p1, q1, s + 1, last);
+    }
   }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // copies past the end write zeros into the stages
   __syncthreads();
-  u32x4* mine = wave == 0 ? p0 : wave == 1 ? p1 : wave == 2 ? q0 : q1;
-  constexpr int kMine = GP::kSlots < GQ::kSlots ? GP::kSlots : GQ::kSlots;
-  constexpr int kChunk = kMine / (W::kNI * 64);
+  // the wave's part of LDS
+  u32x4* mine;
+  constexpr int kSmall = GP::kSlots < GQ::kSlots ? GP::kSlots : GQ::kSlots;
+  if constexpr (NS == 1) mine = (wave < 2 ? p0 : q0) + (wave & 1) * (kSmall / 2);
+  else mine = wave == 0 ? p0 : wave == 1 ? p1 : wave == 2 ? q0 : q1;
+  constexpr int kChunk = (NS == 1 ? kSmall / 2 : kSmall) / (W::kNI * 64);
   static_assert(kChunk >= 1, "a row tile of the wave fits its LDS");
-  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ, NS == 1>(a, it, c0, wrow, wcol, mine, acc);
 }
 
-template <int DT, int BM, int BN>
+template <int DT, int BM, int BN, int NS>
 static hipError_t copied_launch(bool ps, bool qs, bool dg, const ProductArgs& a, hipStream_t s) {
   const unsigned blocks = static_cast<unsigned>(a.item_blocks + a.fill_blocks);
   // whole 16-byte slots: the contraction of a contiguous operand, the columns (rows) of a strided one
   constexpr int n = 16 / dtype_bytes(DT);
-  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0) return hipErrorInvalidValue;
+  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0 || (NS == 1 && a.splits != 1)) return hipErrorInvalidValue;
   if ((!ps || !qs) && a.depth % n != 0) return hipErrorInvalidValue;
   if ((ps && a.cols % n != 0) || (qs && a.rows % n != 0)) return hipErrorInvalidValue;
-  if (!ps && !qs && !dg) product_copied_kernel<DT, BM, BN, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
-  else if (ps && !qs && !dg) product_copied_kernel<DT, BM, BN, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
-  else if constexpr (BM == BN) {
-    if (ps && qs && dg) product_copied_kernel<DT, BM, BN, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
-    else return hipErrorInvalidValue;
-  } else return hipErrorInvalidValue;
+  if (dg) {
+    if constexpr (BM == BN) {
+      if (!ps || !qs) return hipErrorInvalidValue;
+      product_copied_kernel<DT, BM, BN, NS, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
+    } else return hipErrorInvalidValue;
+  } else {
+    if constexpr (NS == 1) return hipErrorInvalidValue;
+    else if (qs) return hipErrorInvalidValue;
+    else if (ps) product_copied_kernel<DT, BM, BN, NS, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
+    else product_copied_kernel<DT, BM, BN, NS, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
+  }
   return hipGetLastError();
 }
 
@@ -411,11 +457,12 @@ static hipError_t staged_launch(bool ps, bool qs, bool dg, const ProductArgs& a,
 
 template <int DT>
 static hipError_t tile_launch(bool ps, bool qs, bool dg, const TileShape& t, const ProductArgs& a, hipStream_t s) {
-  if (!t.staged && t.bm == 128 && t.bn == 128) return copied_launch<DT, 128, 128>(ps, qs, dg, a, s);
-  if (!t.staged && t.bm == 64 && t.bn == 128) return copied_launch<DT, 64, 128>(ps, qs, dg, a, s);
-  if (!t.staged && t.bm == 32 && t.bn == 128) return copied_launch<DT, 32, 128>(ps, qs, dg, a, s);
-  if (t.staged && t.bm == 64 && t.bn == 64) return staged_launch<DT, 64, 64>(ps, qs, dg, a, s);
-  if (t.staged && t.bm == 128 && t.bn == 128) return staged_launch<DT, 128, 128>(ps, qs, dg, a, s);
+  if (t.form == TileShape::kStaged && t.bm == 64 && t.bn == 64) return staged_launch<DT, 64, 64>(ps, qs, dg, a, s);
+  if (t.form == TileShape::kShallow && t.bm == 128 && t.bn == 128) return copied_launch<DT, 128, 128, 1>(ps, qs, dg, a, s);
+  if (t.form != TileShape::kCopied || t.bn != 128) return hipErrorInvalidValue;
+  if (t.bm == 128) return copied_launch<DT, 128, 128, 2>(ps, qs, dg, a, s);
+  if (t.bm == 64) return copied_launch<DT, 64, 128, 2>(ps, qs, dg, a, s);
+  if (t.bm == 32) return copied_launch<DT, 32, 128, 2>(ps, qs, dg, a, s);
   return hipErrorInvalidValue;
 }
 

@@ -9,8 +9,9 @@
 
 namespace smx {
 
-constexpr int kGradRows = 64;   // rows of a workgroup of the activation gradient
-constexpr int kGradCols = 256;  // its output columns: 64 lanes of 4, the 4 waves take rows in turn
+constexpr int kGradRows = 16;   // rows of a workgroup of the activation gradient, four per wave: all loaded at once
+constexpr int kSumWaves = 16;   // waves of a workgroup of the bias gradient
+constexpr int kGradCols = 256;  // its output columns: 64 lanes of 4
 constexpr int kJoinRows = 4;    // rows of a workgroup that joins splits, one per wave
 
 // dz = dy * act'(z), rounded into dz (unless null), and its fp32 column sums over the workgroup's rows.
@@ -38,33 +39,38 @@ __global__ __launch_bounds__(kPThreads) void act_grad_kernel(ActGradArgs a) {
   const bool vec = a.p.vec;
   f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   if (left > 0) {
-    for (int r = wave; r < it.m; r += kPWaves) {
-      const int64_t row = it.row + r;
-      const f32x4 dy = load4<DT>(a.dy, row * a.dy_ld + col, left, vec);
-      if (a.p.gated) {
-        const char* z = reinterpret_cast<const char*>(a.z);
-        const f32x4 g = load4<kF32>(z, row * a.z_ld + col, left, vec);
-        const f32x4 u = load4<kF32>(z, row * a.z_ld + a.p.out_cols + col, left, vec);
-        f32x4 dg, du;
+    constexpr int kN = kGradRows / kPWaves;
+    f32x4 d[kN], z[kN], u[kN];
+    bool in[kN];
+    int64_t row[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      in[n] = wave + n * kPWaves < it.m;
+      row[n] = static_cast<int64_t>(it.row) + wave + n * kPWaves;
+      d[n] = in[n] ? load4<DT>(a.dy, row[n] * a.dy_ld + col, left, vec) : f32x4{};
+      const char* zp = reinterpret_cast<const char*>(a.z);
+      z[n] = in[n] && a.z != nullptr ? load4<kF32>(zp, row[n] * a.z_ld + col, left, vec) : f32x4{};
+      u[n] = in[n] && a.p.gated ? load4<kF32>(zp, row[n] * a.z_ld + a.p.out_cols + col, left, vec) : f32x4{};
+    }
+    if (a.p.gated) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        f32x4 du;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          dg[e] = dy[e] * u[e] * activate_grad(kActSilu, g[e]);
-          du[e] = dy[e] * activate(kActSilu, g[e]);
+          du[e] = d[n][e] * activate<DT == kF32>(kActSilu, z[n][e]);
+          d[n][e] *= u[n][e] * activate_grad<DT == kF32>(kActSilu, z[n][e]);
         }
-        store4<DT>(a.dz, row * a.dz_ld + col, left, vec, dg);
-        store4<DT>(a.dz, row * a.dz_ld + a.p.out_cols + col, left, vec, du);
-        sum[0] += dg;
-        sum[1] += du;
-      } else {
-        f32x4 d = dy;
-        if (a.z != nullptr) {
-          const f32x4 z = load4<kF32>(reinterpret_cast<const char*>(a.z), row * a.z_ld + col, left, vec);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) d[e] *= activate_grad(a.p.act, z[e]);
-        }
-        if (a.dz != nullptr) store4<DT>(a.dz, row * a.dz_ld + col, left, vec, d);
-        sum[0] += d;
+        if (in[n]) store4<DT>(a.dz, row[n] * a.dz_ld + a.p.out_cols + col, left, vec, du);
+        if (in[n]) sum[1] += du;
       }
+    } else if (a.z != nullptr) {
+      activate_grad_all<DT == kF32>(a.p.act, z, d);
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      if (in[n] && a.dz != nullptr) store4<DT>(a.dz, row[n] * a.dz_ld + col, left, vec, d[n]);
+      if (in[n]) sum[0] += d[n];
     }
   }
   if (a.sums == nullptr) return;
@@ -94,7 +100,7 @@ __global__ __launch_bounds__(kPThreads) void act_grad_kernel(ActGradArgs a) {
 
 // Bias gradient: the group's row tiles' sums, added in order.
 template <int DT>
-__global__ __launch_bounds__(kPThreads) void bias_grad_kernel(ProductArgs p, const float* sums, int max_tiles, char* grad) {
+__global__ __launch_bounds__(kSumWaves* kWave) void bias_grad_kernel(ProductArgs p, const float* sums, int max_tiles, char* grad) {
   using S = typename Elem<DT>::S;
   const int cb = (p.cols + kWave - 1) / kWave;
   const int g = static_cast<int>(blockIdx.x) / cb;
@@ -110,14 +116,16 @@ __global__ __launch_bounds__(kPThreads) void bias_grad_kernel(ProductArgs p, con
   }
   first -= count;
   count = min(count, max_tiles - first);
-  __shared__ float lds[kPWaves][kWave];
+  __shared__ float lds[kSumWaves][kWave];
   float v = 0.0f;
-  if (col < p.cols)
-    for (int t = wave; t < count; t += kPWaves) v += sums[static_cast<int64_t>(first + t) * p.cols + col];
+  if (col < p.cols) {
+#pragma unroll 4
+    for (int t = wave; t < count; t += kSumWaves) v += sums[static_cast<int64_t>(first + t) * p.cols + col];
+  }
   lds[wave][lane] = v;
   __syncthreads();
   if (wave > 0 || col >= p.cols) return;
-  for (int w = 1; w < kPWaves; ++w) v += lds[w][lane];
+  for (int w = 1; w < kSumWaves; ++w) v += lds[w][lane];
   reinterpret_cast<S*>(grad)[static_cast<int64_t>(g) * p.cols + col] = Elem<DT>::from_f32(v);
 }
 
@@ -146,8 +154,7 @@ __global__ __launch_bounds__(kPThreads) void join_kernel(ProductArgs a, int spli
     if (a.gated) u += load4<kF32>(part, at + a.out_cols, left, vec);
   }
   const f32x4 bias = bias4<DT>(a, it, col, left), res = res4<DT>(a, row, col, left);
-  if (a.gated) finish4_gated<DT>(a, row, col, left, v, u, bias, bias4<DT>(a, it, a.out_cols + col, left), res);
-  else finish4<DT>(a, it, row, col, left, v, bias, res);
+  finish4<DT>(a, it, row, col, left, v, u, bias, a.gated ? bias4<DT>(a, it, a.out_cols + col, left) : f32x4{}, res);
 }
 
 namespace {
@@ -164,22 +171,33 @@ enum Kind { kForward, kInputGrad, kWeightGrad };
 
 // How a product runs.
 struct ProductPlan {
-  TileShape tile{64, 64, true};
+  TileShape tile{64, 64, TileShape::kStaged};
   int splits = 1, split_steps = 0;
   int64_t part_bytes = 0;
 };
 
-// Tiles of the copied kernels with the time of one contraction step (us, 128 bytes of it) when 1, 2, .. workgroups run
-// on a CU, as many as fit (bf16, 4096 x 4096 weight, 1 to 8192 rows).
+// The tiles, with the time of a call in us that n workgroups per CU take: 2.5 + end * n + steps * (first + each * n), a
+// step being 128 bytes of the contraction. Fitted to measured calls (bf16: 1 to 8192 rows, 4096 and 696 -> 4096 and
+// 1200, weight gradients of 1 to 100 groups of 3 to 800 rows, unaligned 1 to 3000 rows of 1999 -> 1333); the fit is
+// within about 20 % of what was measured, and where two tiles come closer than that either will do. Both sides of some
+// choices (us): 32 rows, 4096 -> 4096, 16 x 32 rows 11.4, 32 x 128 copied 33; 128 rows 28 and 64 x 64 rows 23; 512 rows
+// 64 x 64 rows 38.5, 64 x 128 copied 36; 2048 rows 128 x 128 73, wide 97; 4096 rows 129 and 117.
 struct TileCost {
-  int bm, bn, fit;
-  float step[4];
+  TileShape t;
+  float end, first, each;
+  float each32;    // fp32 (of the same bytes: half the elements, at a 16th of the matrix rate); 0: not for fp32
+  float depth_end; // end of a product grouped along its contraction; 0: not for them
 };
+using Tile = TileShape;
 constexpr TileCost kTileCosts[] = {
-    {256, 256, 1, {1.6f, 0.f, 0.f, 0.f}},
-    {128, 128, 2, {0.70f, 1.06f, 0.f, 0.f}},
-    {64, 128, 3, {0.46f, 0.66f, 0.97f, 0.f}},
-    {32, 128, 4, {0.38f, 0.50f, 0.75f, 0.96f}},
+    {{16, 16, Tile::kRows}, 0.3f, 0.085f, 0.052f, 0.06f, 0.f},  {{16, 32, Tile::kRows}, 0.5f, 0.06f, 0.08f, 0.10f, 0.f},
+    {{32, 32, Tile::kRows}, 0.5f, 0.065f, 0.096f, 0.17f, 0.f},  {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
+    {{32, 128, Tile::kCopied}, 0.7f, 0.20f, 0.22f, 0.52f, 0.f}, {{64, 128, Tile::kCopied}, 1.0f, 0.20f, 0.30f, 1.0f, 0.f},
+    {{128, 128, Tile::kCopied}, 3.5f, 0.20f, 0.43f, 1.95f, 4.5f}, {{128, 128, Tile::kShallow}, 1.8f, 0.3f, 0.75f, 2.3f, 1.8f},
+    {{256, 256, Tile::kWide}, 10.f, 0.0f, 1.57f, 0.f, 16.f},
+    // any alignment
+    {{16, 32, Tile::kRowsStaged}, 0.5f, 0.10f, 0.12f, 0.13f, 0.f}, {{32, 32, Tile::kRowsStaged}, 0.5f, 0.10f, 0.20f, 0.20f, 0.f},
+    {{64, 64, Tile::kStaged}, 1.5f, 0.18f, 0.33f, 0.9f, 1.5f},
 };
 constexpr int kCUs = 256;
 
@@ -187,14 +205,20 @@ constexpr int kCUs = 256;
 ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64_t depth, int64_t groups, bool gated,
                          bool slots) {
   ProductPlan p;
-  if (!slots || rows == 0) return p;
+  if (rows == 0) return p;
   const bool depth_groups = kind == kWeightGrad;
-  const double mean_depth = depth_groups ? static_cast<double>(depth) / groups : static_cast<double>(depth);
-  const double steps = std::max(1.0, mean_depth / (kPStep / dtype_bytes(dtype)));
+  const int64_t all = cdiv(depth, kPStep / dtype_bytes(dtype));
+  const double mean = depth_groups ? static_cast<double>(depth) / groups : static_cast<double>(depth);
+  const double steps = std::max(1.0, mean / (kPStep / dtype_bytes(dtype)));
   double best = 0;
-  for (const TileCost& t : kTileCosts) {
-    if (t.bm == 256 && dtype == kF32) continue;
-    if (kind == kWeightGrad && t.bm < 128) continue;
+  for (const TileCost& c : kTileCosts) {
+    const TileShape& t = c.t;
+    const bool by_rows = t.form == Tile::kRows || t.form == Tile::kRowsStaged;
+    if ((t.form == Tile::kStaged || t.form == Tile::kRowsStaged) == slots) continue;
+    if (by_rows && (kind != kForward || (gated && t.bn < 32))) continue;
+    if (t.form == Tile::kShallow && !depth_groups) continue;
+    const float end = depth_groups ? c.depth_end : c.end, each = dtype == kF32 ? c.each32 : c.each;
+    if (end == 0 || each == 0) continue;
     // row tiles: of every group with rows, half a tile more than its rows fill
     double row_tiles = static_cast<double>(cdiv(rows, t.bm));
     if (!depth_groups && groups > 1) {
@@ -202,22 +226,19 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
       row_tiles = std::max(active, static_cast<double>(rows) / t.bm + active / 2);
     }
     const double tiles = row_tiles * static_cast<double>(cdiv(cols, t.bn)) * (depth_groups ? groups : 1);
-    for (int splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (t.bm == 256 || (depth_groups && groups > 1) || splits * 4 > steps)) break;
-      double per_cu = std::ceil(tiles * splits / kCUs), time = 0;
-      const double len = steps / splits + 6;  // and the ends of a tile
-      time += std::floor(per_cu / t.fit) * t.step[t.fit - 1] * len;
-      const int rest = static_cast<int>(per_cu) % t.fit;
-      if (rest > 0) time += t.step[rest - 1] * len;
-      if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch, partial sums out and in
-      if (best == 0 || time < best) {
-        best = time;
-        p.tile = TileShape{t.bm, t.bn, false};
-        const int64_t all = cdiv(depth, kPStep / dtype_bytes(dtype));
-        p.split_steps = static_cast<int>(cdiv(all, splits));
-        p.splits = splits == 1 ? 1 : static_cast<int>(cdiv(all, p.split_steps));
-        p.part_bytes = p.splits > 1 ? p.splits * rows * cols * 4 : 0;
-      }
+    // (splits: not of rows tiles, whose waves split the contraction already, and of groups along it only of a single one)
+    const bool may_split = !by_rows && t.form != Tile::kShallow && !(depth_groups && groups > 1);
+    for (int splits = 1; splits <= 16 && (splits == 1 || (may_split && splits * 4 <= steps)); splits *= 2) {
+      double n = std::max(1.0, tiles * splits / kCUs);
+      if (!by_rows) n = std::ceil(n);
+      double time = 2.5 + end * n + steps / splits * (c.first + each * n);
+      if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch; partial sums out and in
+      if (best != 0 && time >= best) continue;
+      best = time;
+      p.tile = t;
+      p.split_steps = static_cast<int>(cdiv(cdiv(all, splits), 2) * 2);  // in pairs
+      p.splits = splits == 1 ? 1 : static_cast<int>(cdiv(all, p.split_steps));
+      p.part_bytes = p.splits > 1 ? p.splits * rows * cols * 4 : 0;
     }
   }
   return p;
@@ -240,9 +261,16 @@ int run_product(Kind kind, int dtype, const ProductPlan& plan, ProductArgs& a, b
   a.split_steps = plan.split_steps;
   a.item_blocks = static_cast<int>(items);
   a.fill_blocks = plan.splits > 1 ? 0 : fills;
-  hipError_t err = plan.tile.bm == 256
-                       ? launch_product_wide(dtype, kind != kForward, kind == kWeightGrad, depth_groups, a, s)
-                       : launch_product_tile(dtype, kind != kForward, kind == kWeightGrad, depth_groups, plan.tile, a, s);
+  const bool ps = kind != kForward, qs = kind == kWeightGrad;
+  hipError_t err;
+  switch (plan.tile.form) {
+    case TileShape::kRows:
+    case TileShape::kRowsStaged:
+      err = launch_product_rows(dtype, plan.tile, a, s);
+      break;
+    case TileShape::kWide: err = launch_product_wide(dtype, ps, qs, depth_groups, a, s); break;
+    default: err = launch_product_tile(dtype, ps, qs, depth_groups, plan.tile, a, s);
+  }
   if (err != hipSuccess || plan.splits == 1) return static_cast<int>(err);
   const int splits = a.splits;
   a.splits = 1;
@@ -314,6 +342,7 @@ struct Groups {
 int check_groups(const Sizes& z, const Groups& g) {
   if (!z.grouped) return SMX_OK;
   if (!g.offsets || g.weights <= 0 || g.stride < 0) return SMX_ERR_INVALID_ARG;
+  if (g.weights > kMaxSize) return SMX_ERR_UNSUPPORTED;
   if (!g.slots && g.weights != z.G) return SMX_ERR_INVALID_ARG;
   if (!aligned(g.offsets, 8) || !aligned(g.slots, 8)) return SMX_ERR_MISALIGNED;
   return SMX_OK;
@@ -444,9 +473,9 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
     const float* sums = reinterpret_cast<const float*>(ws + l.sums);
     char* out = static_cast<char*>(grad_bias);
     switch (z.dtype) {
-      case kF32: bias_grad_kernel<kF32><<<n, kPThreads, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
-      case kF16: bias_grad_kernel<kF16><<<n, kPThreads, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
-      default: bias_grad_kernel<kBF16><<<n, kPThreads, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
+      case kF32: bias_grad_kernel<kF32><<<n, kSumWaves * kWave, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
+      case kF16: bias_grad_kernel<kF16><<<n, kSumWaves * kWave, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
+      default: bias_grad_kernel<kBF16><<<n, kSumWaves * kWave, 0, s>>>(ag.p, sums, ag.max_tiles, out); break;
     }
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return static_cast<int>(err);

@@ -14,199 +14,233 @@ accumulation would join the capture from another stream): drop its outputs first
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._torch import dtype_code, require_gpu, workspace
+from ._torch import dtype_code, workspace
+
+
+_ACTIVATIONS = _lib.ACTIVATIONS
+_SWIGLU = _ACTIVATIONS["swiglu"]
+_raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index: the hipStream_t itself
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """t as a matrix of rows with adjacent elements, and their distance (a copy where needed)."""
     n = t.shape[-1]
+    if t.is_contiguous():
+        return t, n
     m = t if t.dim() == 2 else t.reshape(-1, n)
     if (m.stride(1) != 1 and n != 1) or (m.stride(0) < n and m.shape[0] > 1):
         m = m.contiguous()
     return m, (m.stride(0) if m.shape[0] > 1 else n)
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=4096)
+def _workspace_size(query: str, *sizes: int) -> int:
+    return getattr(_lib.lib(), query)(*sizes)
 
 
-def _on(device: torch.device):
-    """The device as the current one (kernels are launched on the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _workspace(query: str, device: torch.device, *sizes: int) -> tuple[Optional[torch.Tensor], Optional[int], int]:
+    """Scratch of a call from torch's caching allocator: the tensor, its address and its bytes."""
+    n = _workspace_size(query, *sizes)
+    if n == 0:
+        return None, None, 0
+    ws = workspace(n, device)
+    return ws, ws.data_ptr(), n
 
 
 def _weight_strides(weight: torch.Tensor) -> tuple[int, int]:
-    """Distances of a weight's rows and of the group's weights."""
+    """Distances of a weight's rows and of the groups' weights."""
+    if weight.is_contiguous():
+        k = weight.shape[-1]
+        return k, (weight.shape[-2] * k if weight.dim() == 3 else 0)
     nw, k = weight.shape[-2:]
     row = weight.stride(-2) if nw > 1 else k
+    if (k > 1 and weight.stride(-1) != 1) or row < k:
+        raise ValueError(f"weight rows must be apart, with adjacent elements: strides {weight.stride()}")
     group = 0
     if weight.dim() == 3:
         group = weight.stride(0) if weight.shape[0] > 1 else nw * row
     return row, group
 
 
-class _Call:
-    """Checked arguments of a product."""
+def _check(x, weight, bias, activation, residual, offsets, slots, out):
+    """The call's sizes: (dtype code, activation code, K, N, weight rows, groups, y's shape), and the
+    weight's strides."""
+    try:
+        act = _ACTIVATIONS[activation]
+    except KeyError:
+        raise ValueError(f"unknown activation {activation!r}; expected one of "
+                         f"{[a for a in _ACTIVATIONS if a]} or None") from None
+    dtype = dtype_code(x.dtype)
+    grouped = offsets is not None
+    xshape, wshape = x.shape, weight.shape
+    if len(xshape) < 1 or (grouped and len(xshape) != 2):
+        raise ValueError(f"x must be [{'rows' if grouped else '...'}, K], got {tuple(xshape)}")
+    if len(wshape) != (3 if grouped else 2):
+        raise ValueError(f"weight must be [{'G, ' if grouped else ''}Nw, K], got {tuple(wshape)}")
+    k, nw = xshape[-1], wshape[-2]
+    if k != wshape[-1]:
+        raise ValueError(f"x has {k} columns, weight {wshape[-1]}")
+    if nw == 0 or k == 0:
+        raise ValueError(f"empty weight {tuple(wshape)}")
+    n = nw
+    if act == _SWIGLU:
+        if nw % 2:
+            raise ValueError(f"swiglu takes gate and up rows: {nw} weight rows are odd")
+        n = nw // 2
+    shape = (*xshape[:-1], n)
+    strides = _weight_strides(weight)
+    device = x.device
+    for name, t, want in (("weight", weight, None), ("bias", bias, wshape[:-1]), ("residual", residual, shape),
+                          ("out", out, shape)):
+        if t is None:
+            continue
+        if want is not None and t.shape != want:
+            raise ValueError(f"{name} must be {tuple(want)}, got {tuple(t.shape)}")
+        if t.dtype != x.dtype:
+            raise TypeError(f"dtype mismatch: x is {x.dtype}, {name} {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"x is on {device}, {name} on {t.device}")
+    if not x.is_cuda:
+        raise ValueError(f"expected a GPU tensor, got one on {device}")
+    groups = 0
+    if grouped:
+        for name, t in (("group_offsets", offsets), ("weight_slots", slots)):
+            if t is None:
+                continue
+            if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise TypeError(f"{name} must be a contiguous int64 vector")
+            if t.device != device:
+                raise ValueError(f"expected a GPU tensor, {name} is on {t.device}, x on {device}")
+        groups = offsets.shape[0] - 1
+        if groups < 1:
+            raise ValueError("group_offsets must hold at least two bounds")
+        if slots is None and wshape[0] != groups:
+            raise ValueError(f"{groups} groups, {wshape[0]} weights")
+        if slots is not None and slots.shape[0] != groups:
+            raise ValueError(f"{groups} groups, {slots.shape[0]} slots")
+        if wshape[0] == 0:
+            raise ValueError("no weights")
+    return (dtype, act, k, n, nw, groups, shape), strides
 
-    def __init__(self, x, weight, bias, activation, residual, offsets, slots, out):
-        grouped = offsets is not None
-        if activation not in _lib.ACTIVATIONS:
-            raise ValueError(f"unknown activation {activation!r}; expected one of "
-                             f"{[a for a in _lib.ACTIVATIONS if a]} or None")
-        self.act = _lib.ACTIVATIONS[activation]
-        self.dtype = dtype_code(x.dtype)
-        if x.dim() < 1 or (grouped and x.dim() != 2):
-            raise ValueError(f"x must be [{'rows' if grouped else '...'}, K], got {tuple(x.shape)}")
-        if weight.dim() != (3 if grouped else 2):
-            raise ValueError(f"weight must be [{'G, ' if grouped else ''}Nw, K], got {tuple(weight.shape)}")
-        nw, k = weight.shape[-2:]
-        if k != x.shape[-1]:
-            raise ValueError(f"x has {x.shape[-1]} columns, weight {k}")
-        if nw == 0 or k == 0:
-            raise ValueError(f"empty weight {tuple(weight.shape)}")
-        if self.act == _lib.ACTIVATIONS["swiglu"]:
-            if nw % 2:
-                raise ValueError(f"swiglu takes gate and up rows: {nw} weight rows are odd")
-            self.n = nw // 2
-        else:
-            self.n = nw
-        row, group = _weight_strides(weight)
-        if (k > 1 and weight.stride(-1) != 1) or row < k:
-            raise ValueError(f"weight rows must be apart, with adjacent elements: strides {weight.stride()}")
-        shape = (*x.shape[:-1], self.n)
-        for name, t, want in (("bias", bias, tuple(weight.shape[:-1])), ("residual", residual, shape),
-                              ("out", out, shape)):
-            if t is not None and tuple(t.shape) != want:
-                raise ValueError(f"{name} must be {want}, got {tuple(t.shape)}")
-        require_gpu(x, weight, bias, residual, offsets, slots, out)
-        for t in (weight, bias, residual, out):
-            if t is not None and t.dtype != x.dtype:
-                raise TypeError(f"dtype mismatch: x is {x.dtype}, got {t.dtype}")
-        for t in (weight, bias, residual, offsets, slots, out):
-            if t is not None and t.device != x.device:
-                raise ValueError(f"x is on {x.device}, got a tensor on {t.device}")
-        self.groups = 0
-        if grouped:
-            if offsets.dtype != torch.int64 or offsets.dim() != 1 or not offsets.is_contiguous():
-                raise TypeError("group_offsets must be a contiguous int64 vector")
-            self.groups = offsets.numel() - 1
-            if self.groups < 1:
-                raise ValueError("group_offsets must hold at least two bounds")
-            if slots is None and weight.shape[0] != self.groups:
-                raise ValueError(f"{self.groups} groups, {weight.shape[0]} weights")
-            if slots is not None:
-                if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
-                    raise TypeError("weight_slots must be a contiguous int64 vector")
-                if slots.numel() != self.groups:
-                    raise ValueError(f"{self.groups} groups, {slots.numel()} slots")
-                if weight.shape[0] == 0:
-                    raise ValueError("no weights")
-        self.nw, self.k, self.shape = nw, k, shape
-        self.wargs = (weight.data_ptr(), row)
-        self.gargs = (group, weight.shape[0]) if grouped else ()
-        self.offsets, self.slots = offsets, slots
 
-    def workspace(self, query: str, rows: int, device: torch.device):
-        n = getattr(_lib.lib(), query)(rows, self.k, self.n, self.groups, self.act, self.dtype)
-        return (workspace(n, device) if n else None), n
+def _forward(sizes, strides, x, weight, bias, residual, offsets, slots, out, keep: bool):
+    """y, and the fp32 pre-activations where the gradient needs them (kept in 32 bits: their rounding would
+    weigh as much in the gradients as that of the gradients themselves)."""
+    dtype, act, k, n, nw, groups, shape = sizes
+    device = x.device
+    if device.index != torch.cuda.current_device():  # kernels are launched on the current device
+        with torch.cuda.device(device):
+            return _forward(sizes, strides, x, weight, bias, residual, offsets, slots, out, keep)
+    row, group = strides
+    xm, xs = _rows(x)
+    rows = xm.numel() // k
+    if out is None:
+        y = torch.empty(shape, dtype=x.dtype, device=device)
+        ys = n
+    else:
+        y = out
+        ys = out.stride(0) if out.dim() == 2 and rows > 1 else n
+    rm = rs = z = None
+    if residual is not None:
+        rm, rs = _rows(residual)
+    if keep and act:
+        z = torch.empty((rows, nw), dtype=torch.float32, device=device)
+    ws, wp, nbytes = _workspace("smx_linear_workspace_size", device, rows, k, n, groups, act, dtype)
+    head = (xm.data_ptr(), xs, dtype, rows, k, weight.data_ptr(), row)
+    tail = (y.data_ptr(), ys, None if z is None else z.data_ptr(), wp, nbytes, _raw_stream(device.index))
+    bm = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    bp = None if bm is None else bm.data_ptr()
+    rp = None if rm is None else rm.data_ptr()
+    if groups:
+        code = _lib.lib().smx_grouped_linear(
+            *head, group, weight.shape[0], n, bp, act, rp, rs or 0, offsets.data_ptr(), groups,
+            None if slots is None else slots.data_ptr(), out is None, *tail)
+    else:
+        code = _lib.lib().smx_linear(*head, n, bp, act, rp, rs or 0, *tail)
+    if code:
+        _lib.check("smx_grouped_linear" if groups else "smx_linear", code)
+    return y, z
 
-    def forward(self, x, bias, residual, out, keep: bool):
-        """y, and the fp32 pre-activations where the gradient needs them (kept in 32 bits: their rounding would
-        weigh as much in the gradients as that of the gradients themselves)."""
-        with _on(x.device):
-            xm, xs = _rows(x)
-            rows = xm.shape[0]
-            fresh = out is None
-            y = torch.empty(self.shape, dtype=x.dtype, device=x.device) if fresh else out
-            ym = y if y.dim() == 2 else y.view(-1, self.n)
-            ys = ym.stride(0) if rows > 1 else self.n
-            rm, rs = (None, 0) if residual is None else _rows(residual)
-            z = None
-            if keep and self.act:
-                z = torch.empty((rows, self.nw), dtype=torch.float32, device=x.device)
-            ws, nbytes = self.workspace("smx_linear_workspace_size", rows, x.device)
-            stream = torch.cuda.current_stream(x.device).cuda_stream
-            head = (xm.data_ptr(), xs, self.dtype, rows, self.k, *self.wargs)
-            tail = (ym.data_ptr(), ys, _ptr(z), _ptr(ws), nbytes, stream)
-            if self.groups:
-                _lib.call("smx_grouped_linear", *head, *self.gargs, self.n, _ptr(bias), self.act, _ptr(rm), rs,
-                          self.offsets.data_ptr(), self.groups, _ptr(self.slots), int(fresh), *tail)
-            else:
-                _lib.call("smx_linear", *head, self.n, _ptr(bias), self.act, _ptr(rm), rs, *tail)
-        return y, z
 
-    def backward(self, dy, saved, need_x: bool, need_w: bool, need_b: bool):
-        x, weight, z, offsets, slots = saved  # as autograd hands them back: perhaps not at their old addresses
-        row, group = _weight_strides(weight)
-        with _on(x.device):
-            dm, ds = _rows(dy)
-            xm, xs = _rows(x)
-            rows = xm.shape[0]
-            lead = (self.groups,) if self.groups else ()
-            new = dict(dtype=x.dtype, device=x.device)
-            dx = torch.empty(x.shape, **new) if need_x else None
-            dw = torch.empty((*lead, self.nw, self.k), **new) if need_w else None
-            db = torch.empty((*lead, self.nw), **new) if need_b else None
-            ws, nbytes = self.workspace("smx_linear_grad_workspace_size", rows, x.device)
-            stream = torch.cuda.current_stream(x.device).cuda_stream
-            head = (dm.data_ptr(), ds, _ptr(z), xm.data_ptr(), xs, self.dtype, rows, self.k,
-                    weight.data_ptr(), row)
-            tail = (_ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream)
-            if self.groups:
-                _lib.call("smx_grouped_linear_grad", *head, group, weight.shape[0], self.n, self.act,
-                          offsets.data_ptr(), self.groups, _ptr(slots), *tail)
-            else:
-                _lib.call("smx_linear_grad", *head, self.n, self.act, *tail)
-        return dx, dw, db
+def _backward(sizes, dy, saved, need_x: bool, need_w: bool, need_b: bool):
+    dtype, act, k, n, nw, groups, _ = sizes
+    x, weight, z, offsets, slots = saved  # as autograd hands them back: perhaps not at their old addresses
+    device = x.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _backward(sizes, dy, saved, need_x, need_w, need_b)
+    row, group = _weight_strides(weight)
+    dm, ds = _rows(dy)
+    xm, xs = _rows(x)
+    rows = xm.numel() // k
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if need_x else None
+    dw = torch.empty((groups, nw, k) if groups else (nw, k), dtype=x.dtype, device=device) if need_w else None
+    db = torch.empty((groups, nw) if groups else (nw,), dtype=x.dtype, device=device) if need_b else None
+    ws, wp, nbytes = _workspace("smx_linear_grad_workspace_size", device, rows, k, n, groups, act, dtype)
+    head = (dm.data_ptr(), ds, None if z is None else z.data_ptr(), xm.data_ptr(), xs, dtype, rows, k,
+            weight.data_ptr(), row)
+    tail = (*(None if t is None else t.data_ptr() for t in (dx, dw, db)), wp, nbytes, _raw_stream(device.index))
+    if groups:
+        code = _lib.lib().smx_grouped_linear_grad(
+            *head, group, weight.shape[0], n, act, offsets.data_ptr(), groups,
+            None if slots is None else slots.data_ptr(), *tail)
+    else:
+        code = _lib.lib().smx_linear_grad(*head, n, act, *tail)
+    if code:
+        _lib.check("smx_grouped_linear_grad" if groups else "smx_linear_grad", code)
+    return dx, dw, db
 
 
 class _Product(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, call):
-        needs = ctx.needs_input_grad
-        y, z = call.forward(x, bias, residual, None, any(needs[:3]))
-        ctx.save_for_backward(x, weight, z, call.offsets, call.slots)
-        call.offsets = call.slots = None
-        ctx.call = call
+    def forward(ctx, x, weight, bias, residual, offsets, slots, sizes, strides):
+        y, z = _forward(sizes, strides, x, weight, bias, residual, offsets, slots, None,
+                        any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, z, offsets, slots)
+        ctx.sizes = sizes
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        grads = (None, None, None)
-        if need_x or need_w or need_b:
-            grads = ctx.call.backward(dy, ctx.saved_tensors, need_x, need_w, need_b)
-        return (*grads, dy if need_r else None, None)
+        # (the refusal to differentiate twice costs more than the rest of this function: only where a graph of
+        # the backward pass is recorded)
+        return _gradients_once(ctx, dy) if torch.is_grad_enabled() else _gradients(ctx, dy)
+
+
+def _gradients(ctx, dy):
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    grads = (None, None, None)
+    if need_x or need_w or need_b:
+        grads = _backward(ctx.sizes, dy, ctx.saved_tensors, need_x, need_w, need_b)
+    return (*grads, dy if need_r else None, None, None, None, None)
+
+
+_gradients_once = once_differentiable(_gradients)
 
 
 def _run(x, weight, bias, activation, residual, offsets, slots, out):
-    call = _Call(x, weight, bias, activation, residual, offsets, slots, out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    sizes, strides = _check(x, weight, bias, activation, residual, offsets, slots, out)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         if out is not None:
             raise ValueError("out= takes no part in differentiation: call without it, or under torch.no_grad()")
         if slots is not None and (weight.requires_grad or (bias is not None and bias.requires_grad)):
             raise ValueError("weights reached through weight_slots have no gradient: several groups may share a "
                              "slot. Pass them detached, or index the weights first")
-        return _Product.apply(x, weight, bias, residual, call)
-    if out is not None and (out.stride(-1) != 1 and out.shape[-1] > 1 or not _viewable(out)):
-        raise ValueError(f"out rows must be apart, with adjacent elements: strides {out.stride()}")
-    return call.forward(x, bias, residual, out, False)[0]
-
-
-def _viewable(out: torch.Tensor) -> bool:
-    if out.dim() == 2:
-        return out.shape[0] <= 1 or out.stride(0) >= out.shape[1]
-    return out.is_contiguous()
+        return _Product.apply(x, weight, bias, residual, offsets, slots, sizes, strides)
+    if out is not None and not out.is_contiguous():
+        if out.dim() != 2 or (out.shape[1] > 1 and out.stride(1) != 1) or (
+                out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+            raise ValueError(f"out rows must be apart, with adjacent elements: strides {out.stride()}")
+    return _forward(sizes, strides, x, weight, bias, residual, offsets, slots, out, False)[0]
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
