@@ -36,7 +36,9 @@ struct ProductArgs {
   const char* q;
   int64_t p_ld, q_ld;       // elements
   int64_t p_group;          // elements from one group's P (forward, dx) to the next
-  int rows, cols;           // of the product; grouped along the rows: of all groups
+  int rows, cols;           // of the product; grouped along the rows: of all groups. A strided P may be padded: cols
+                            // counts its columns, out_cols those of the result
+  int q_cols;               // columns of a strided Q, at least rows
   int depth;                // contraction length; grouped along it: of all groups
   const int64_t* offsets;   // [groups + 1] row bounds, or null: one group of everything
   const int64_t* slots;     // [groups] index of the group's P (and bias), or null
@@ -88,6 +90,20 @@ __device__ __forceinline__ int64_t group_weight(const ProductArgs& a, int g) {
   if (a.slots == nullptr) return g;
   const int64_t s = ((ConstMap)(a.slots))[g];
   return s >= 0 && s < a.weights ? s : -1;
+}
+
+// fp32 sums run in chains of kFold steps (256 products), whose results are added up: a single chain of thousands of
+// products would lose a bit or two more than blocked sums do.
+constexpr int kFold = 8;
+template <int NI, int NJ>
+__device__ __forceinline__ void fold(f32x4 (&total)[NI][NJ], f32x4 (&acc)[NI][NJ]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      total[i][j] += acc[i][j];
+      acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 }
 
 // A workgroup's tile of the output.

@@ -121,11 +121,14 @@ __global__ __launch_bounds__(kPThreads) void product_rows_kernel(ProductArgs a) 
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  f32x4 acc[NP][NJ];
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[NP][NJ] = {}, total[NP][NJ] = {};
+  int chain = 0;  // steps since the last fold
+  auto folds = [&](int n) {
+    if (DT == kF32 && (chain += n) >= kFold) {
+      fold(total, acc);
+      chain = 0;
+    }
+  };
   // one step from `st`; the copies of the step NS later follow into it
   auto step = [&](u32x4* st, int c) {
     __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * T::kCopies));
@@ -158,10 +161,14 @@ __global__ __launch_bounds__(kPThreads) void product_rows_kernel(ProductArgs a) 
     step(s1, c + kPWaves);
     if constexpr (NS > 2) step(s2, c + 2 * kPWaves);
     if constexpr (NS > 3) step(s3, c + 3 * kPWaves);
+    folds(NS);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // copies past the end write zeros into the stages
+  if constexpr (DT == kF32) {
+    fold(total, acc);
+    fold(acc, total);
+  }
   __syncthreads();
-
   rows_finish<DT, NP, NJ, T::kSlots>(a, it, c0, wave, s0, s1, acc);
 }
 
@@ -208,11 +215,14 @@ __global__ __launch_bounds__(kPThreads) void product_rows_staged_kernel(ProductA
 #pragma unroll
     for (int n = 0; n < T::kCopies; ++n) v.v[n] = load_slot<DT>(at[n] + static_cast<int64_t>(c) * kDepth, have);
   };
-  f32x4 acc[NP][NJ];
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[NP][NJ] = {}, total[NP][NJ] = {};
+  int chain = 0;  // steps since the last fold
+  auto folds = [&](int n) {
+    if (DT == kF32 && (chain += n) >= kFold) {
+      fold(total, acc);
+      chain = 0;
+    }
+  };
   auto step = [&](const Step& v, u32x4* st) {
     u32x4* mine = st + wave * T::kSlots;
 #pragma unroll
@@ -240,6 +250,11 @@ __global__ __launch_bounds__(kPThreads) void product_rows_staged_kernel(ProductA
     load(v0, c + 2 * kPWaves);
     step(v1, s1);
     load(v1, c + 3 * kPWaves);
+    folds(2);
+  }
+  if constexpr (DT == kF32) {
+    fold(total, acc);
+    fold(acc, total);
   }
   __syncthreads();
   rows_finish<DT, NP, NJ, T::kSlots>(a, it, c0, wave, s0, s1, acc);

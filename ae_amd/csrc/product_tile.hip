@@ -132,7 +132,7 @@ __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductI
   const int left = a.out_cols - col;
   if constexpr (PLAIN) {
     const int lc = lane % kS, lr = lane / kS;
-    const int pcol = c0 + wcol + 4 * lc, pleft = a.cols - pcol;
+    const int pcol = c0 + wcol + 4 * lc, pleft = a.out_cols - pcol;
 #pragma unroll
     for (int j0 = 0; j0 < NJ; j0 += CJ) {
 #pragma unroll
@@ -239,11 +239,7 @@ __global__ __launch_bounds__(kPThreads) void product_staged_kernel(ProductArgs a
   const int s1 = a.splits > 1 ? min(steps, s0 + a.split_steps) : steps;
   const int wave = wave_id();
   const int wrow = (wave / W::kColWaves) * W::kNJ * 16, wcol = (wave % W::kColWaves) * W::kNI * 16;
-  f32x4 acc[W::kNI][W::kNJ];
-#pragma unroll
-  for (int i = 0; i < W::kNI; ++i)
-#pragma unroll
-    for (int j = 0; j < W::kNJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[W::kNI][W::kNJ] = {}, total[W::kNI][W::kNJ] = {};
   if (s0 < s1) {
     lp.load(s0 * GP::kDepth, p_at);
     lq.load(s0 * GP::kDepth, q_at);
@@ -269,6 +265,11 @@ __global__ __launch_bounds__(kPThreads) void product_staged_kernel(ProductArgs a
 #pragma unroll
         for (int j = 0; j < W::kNJ; ++j) acc[i][j] = Elem<DT>::mfma(fp[i], fq[j], acc[i][j]);
     }
+    if (DT == kF32 && (s - s0) % kFold == kFold - 1) fold(total, acc);
+  }
+  if constexpr (DT == kF32) {
+    fold(total, acc);
+    fold(acc, total);
   }
   __syncthreads();
   u32x4* mine = (wave < 2 ? sp : sq) + (wave & 1) * (GP::kSlots / 2);
@@ -349,17 +350,13 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
     return static_cast<uint32_t>(row * p_pitch);
   }, static_cast<int>((a.cols - cfirst) * kEs) - 16);
   cq.init(wave, q_pitch, [&](int q) -> uint32_t { return static_cast<uint32_t>(min(q, it.m - 1) * q_pitch); },
-          static_cast<int>((a.rows - it.row) * kEs) - 16);
+          static_cast<int>((a.q_cols - it.row) * kEs) - 16);
 
   const int steps = (it.depth + GP::kDepth - 1) / GP::kDepth;
   const int s0 = it.split * a.split_steps;
   const int s1 = a.splits > 1 ? min(steps, s0 + a.split_steps) : steps;
   const int wrow = (wave / W::kColWaves) * W::kNJ * 16, wcol = (wave % W::kColWaves) * W::kNI * 16;
-  f32x4 acc[W::kNI][W::kNJ];
-#pragma unroll
-  for (int i = 0; i < W::kNI; ++i)
-#pragma unroll
-    for (int j = 0; j < W::kNJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[W::kNI][W::kNJ] = {}, total[W::kNI][W::kNJ] = {};
   constexpr int kCopies = GP::kLoads + GQ::kLoads;
   auto copy = [&](u32x4* sp, u32x4* sq, int s) {
     const int left = s < s1 ? it.depth - s * GP::kDepth : 0;
@@ -406,11 +403,16 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
       for (; s + 2 < s1; s += 2) {
         step(p0, q0, s, more);
         step(p1, q1, s + 1, more);
+        if (DT == kF32 && (s - s0) % kFold == kFold - 2) fold(total, acc);
       }
       // (a step past the end multiplies zeros: a branch inside the loop costs waits for all copies)
       step(p0, q0, s, last);
       step(p1, q1, s + 1, last);
     }
+  }
+  if constexpr (DT == kF32 && NS > 1) {  // (one stage: for short chains)
+    fold(total, acc);
+    fold(acc, total);
   }
   __syncthreads();
   // the wave's part of LDS
@@ -429,8 +431,9 @@ static hipError_t copied_launch(bool ps, bool qs, bool dg, const ProductArgs& a,
   // whole 16-byte slots: the contraction of a contiguous operand, the columns (rows) of a strided one
   constexpr int n = 16 / dtype_bytes(DT);
   if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0 || (NS == 1 && a.splits != 1)) return hipErrorInvalidValue;
-  if ((!ps || !qs) && a.depth % n != 0) return hipErrorInvalidValue;
-  if ((ps && a.cols % n != 0) || (qs && a.rows % n != 0)) return hipErrorInvalidValue;
+  // (beside a strided P a contiguous Q may end inside a slot, with zeros up to the slot's end)
+  if (!ps && a.depth % n != 0) return hipErrorInvalidValue;
+  if ((ps && a.cols % n != 0) || (qs && (a.q_cols % n != 0 || a.q_cols < a.rows))) return hipErrorInvalidValue;
   if (dg) {
     if constexpr (BM == BN) {
       if (!ps || !qs) return hipErrorInvalidValue;

@@ -414,7 +414,7 @@ __global__ __launch_bounds__(kPThreads, BM * BN > 128 * 128 ? 1 : 2) void produc
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
       const int slot = (lane % C::kRowSlots) ^ strided_perm(w.q.k + C::kCopyRows * o);
-      w.q.off[o] = static_cast<uint32_t>(w.q.k * q_pitch) + min(slot * 8, a.rows - 8 - it.row) * 2;
+      w.q.off[o] = static_cast<uint32_t>(w.q.k * q_pitch) + min(slot * 8, a.q_cols - 8 - it.row) * 2;
     }
   } else {
     w.q.base += it.row * q_pitch + it.k0 * 2;
@@ -455,8 +455,9 @@ hipError_t launch_product_wide(int dtype, bool p_strided, bool q_strided, bool d
                                hipStream_t s) {
   // whole 16-byte slots: the contraction of a contiguous operand, the columns (rows) of a strided one
   if (a.p_ld % 8 != 0 || a.q_ld % 8 != 0 || a.p_group % 8 != 0) return hipErrorInvalidValue;
-  if ((!p_strided || !q_strided) && a.depth % 8 != 0) return hipErrorInvalidValue;
-  if ((p_strided && a.cols % 8 != 0) || (q_strided && a.rows % 8 != 0)) return hipErrorInvalidValue;
+  // (beside a strided P a contiguous Q may end inside a slot, with zeros up to the slot's end)
+  if (!p_strided && a.depth % 8 != 0) return hipErrorInvalidValue;
+  if ((p_strided && a.cols % 8 != 0) || (q_strided && (a.q_cols % 8 != 0 || a.q_cols < a.rows))) return hipErrorInvalidValue;
   if (a.splits > 1 && a.split_steps % 2 != 0) return hipErrorInvalidValue;
   switch (dtype) {
     case kF16: return wide_launch<kF16, 256, 256>(p_strided, q_strided, depth_groups, a, s);

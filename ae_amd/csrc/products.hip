@@ -73,6 +73,11 @@ __global__ __launch_bounds__(kPThreads) void act_grad_kernel(ActGradArgs a) {
       if (in[n]) sum[0] += d[n];
     }
   }
+  // the columns that round dz's rows up to whole slots: zeros, as a contraction takes them along
+  if (a.dz != nullptr && it.ct == col_tiles - 1 && lane < a.dz_ld - a.p.cols) {
+    for (int r = wave; r < it.m; r += kPWaves)
+      reinterpret_cast<typename Elem<DT>::S*>(a.dz)[(static_cast<int64_t>(it.row) + r) * a.dz_ld + a.p.cols + lane] = 0;
+  }
   if (a.sums == nullptr) return;
   // the row tile's own place: row tiles of the groups before it, and of its group before it
   int tile = 0;
@@ -129,6 +134,20 @@ __global__ __launch_bounds__(kSumWaves* kWave) void bias_grad_kernel(ProductArgs
   reinterpret_cast<S*>(grad)[static_cast<int64_t>(g) * p.cols + col] = Elem<DT>::from_f32(v);
 }
 
+// Copies rows of `len` elements, `per` of them in each of the groups, into rows of whole 16-byte slots, with zeros behind.
+template <int DT>
+__global__ __launch_bounds__(kPThreads) void pad_kernel(const char* src, int64_t ld, int64_t group, int64_t per, int len,
+                                                        char* dst, int slots, int64_t rows) {
+  using S = typename Elem<DT>::S;
+  constexpr int kEps = 16 / sizeof(S);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kPWaves + wave_id();
+  if (row >= rows) return;
+  const int64_t g = row / per;
+  const S* from = reinterpret_cast<const S*>(src) + g * group + (row - g * per) * ld;
+  u32x4* to = reinterpret_cast<u32x4*>(dst) + row * slots;
+  for (int s = lane_id(); s < slots; s += kWave) to[s] = load_slot<DT>(from + s * kEps, len - s * kEps);
+}
+
 // Joins the contraction splits: one row per wave, 256 output columns.
 template <int DT>
 __global__ __launch_bounds__(kPThreads) void join_kernel(ProductArgs a, int splits) {
@@ -174,6 +193,7 @@ struct ProductPlan {
   TileShape tile{64, 64, TileShape::kStaged};
   int splits = 1, split_steps = 0;
   int64_t part_bytes = 0;
+  double time = 0;  // estimate, us
 };
 
 // The tiles, with the time of a call in us that n workgroups per CU take: 2.5 + end * n + steps * (first + each * n), a
@@ -210,7 +230,6 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
   const int64_t all = cdiv(depth, kPStep / dtype_bytes(dtype));
   const double mean = depth_groups ? static_cast<double>(depth) / groups : static_cast<double>(depth);
   const double steps = std::max(1.0, mean / (kPStep / dtype_bytes(dtype)));
-  double best = 0;
   for (const TileCost& c : kTileCosts) {
     const TileShape& t = c.t;
     const bool by_rows = t.form == Tile::kRows || t.form == Tile::kRowsStaged;
@@ -233,8 +252,8 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
       if (!by_rows) n = std::ceil(n);
       double time = 2.5 + end * n + steps / splits * (c.first + each * n);
       if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch; partial sums out and in
-      if (best != 0 && time >= best) continue;
-      best = time;
+      if (p.time != 0 && time >= p.time) continue;
+      p.time = time;
       p.tile = t;
       p.split_steps = static_cast<int>(cdiv(cdiv(all, splits), 2) * 2);  // in pairs
       p.splits = splits == 1 ? 1 : static_cast<int>(cdiv(all, p.split_steps));
@@ -308,29 +327,88 @@ int check_pitch(int64_t stride, int64_t len, int64_t es) {
   return stride * es > kPMaxPitch ? SMX_ERR_UNSUPPORTED : SMX_OK;
 }
 
-struct GradLayout {
-  ProductPlan dx, dw;
-  int64_t dz = 0, dz_ld = 0, sums = 0, part = 0, total = 0;
-};
-
 // Whole 16-byte slots: the base and the pitch, and the length of whatever lies side by side.
 bool whole_slots(const void* base, int64_t pitch, int64_t length, int64_t es) {
   return aligned(base, 16) && pitch * es % 16 == 0 && length * es % 16 == 0;
 }
+int64_t whole(int64_t length, int64_t es) { return cdiv(length * es, 16) * 16 / es; }
 
-GradLayout grad_layout(const Sizes& z, bool dx_slots, bool dw_slots) {
-  GradLayout l;
-  l.dx = plan_product(kInputGrad, z.dtype, z.rows, z.K, z.Nw, z.G, false, dx_slots);
-  l.dw = plan_product(kWeightGrad, z.dtype, z.Nw, z.K, z.rows, z.G, false, dw_slots);
-  l.dz_ld = cdiv(z.Nw, 16 / z.es) * (16 / z.es);
-  int64_t at = 0;
-  if (z.act != SMX_ACT_NONE) at += align256(z.rows * l.dz_ld * z.es);
-  l.sums = at;
-  at += align256(max_row_tiles(z.rows, z.G, kGradRows) * z.Nw * 4);
-  l.part = at;
-  at += align256(std::max(l.dx.part_bytes, l.dw.part_bytes));
-  l.total = at;
+// Operands whose rows are no whole slots may be copied into the workspace first, where they are: where the product gains
+// more by it than the copies take (2 us each and their bytes at 4 TB/s; 3000 rows of 1999 -> 1333 in bf16: 51 us
+// without, 31 with).
+double copy_time(int64_t elems, int64_t es) { return 2.0 + 2.0 * elems * es / 4e6; }
+
+struct Layout {
+  ProductPlan plan;
+  bool pad = false;
+  int64_t x = 0, w = 0, part = 0, total = 0;  // offsets of the copies and the partial sums; bytes in all
+};
+
+Layout forward_layout(const Sizes& z, bool slots, bool may_pad) {
+  Layout l;
+  l.plan = plan_product(kForward, z.dtype, z.rows, z.Nw, z.K, z.G, z.Nw != z.N, slots);
+  if (!slots && may_pad && z.K * z.es % 16 != 0 && z.G * z.Nw <= kMaxSize) {
+    const int64_t k = whole(z.K, z.es);
+    const ProductPlan fast = plan_product(kForward, z.dtype, z.rows, z.Nw, k, z.G, z.Nw != z.N, true);
+    if (fast.time + copy_time(z.rows * k, z.es) + copy_time(z.G * z.Nw * k, z.es) < l.plan.time) {
+      l.plan = fast;
+      l.pad = true;
+      l.w = align256(z.rows * k * z.es);
+      l.part = l.w + align256(z.G * z.Nw * k * z.es);
+    }
+  }
+  l.total = l.part + align256(l.plan.part_bytes);
   return l;
+}
+
+struct GradLayout {
+  ProductPlan dx, dw;
+  bool pad_w = false, pad_x = false;
+  int64_t dz = 0, dz_ld = 0, sums = 0, copy = 0, part = 0, total = 0;
+};
+
+// w_slots, x_slots: the weight's and x's rows are whole slots; dz's always are.
+GradLayout grad_layout(const Sizes& z, bool w_slots, bool x_slots, bool may_pad) {
+  GradLayout l;
+  l.dx = plan_product(kInputGrad, z.dtype, z.rows, z.K, z.Nw, z.G, false, w_slots);
+  l.dw = plan_product(kWeightGrad, z.dtype, z.Nw, z.K, z.rows, z.G, false, x_slots);
+  const int64_t k = whole(z.K, z.es);
+  int64_t copy = 0;
+  if (may_pad && z.K * z.es % 16 != 0 && z.rows > 0 && z.G * z.Nw <= kMaxSize) {
+    ProductPlan fast = plan_product(kInputGrad, z.dtype, z.rows, k, z.Nw, z.G, false, true);
+    if (!w_slots && fast.time + copy_time(z.G * z.Nw * k, z.es) < l.dx.time) {
+      l.dx = fast;
+      l.pad_w = true;
+      copy = z.G * z.Nw * k * z.es;
+    }
+    fast = plan_product(kWeightGrad, z.dtype, z.Nw, k, z.rows, z.G, false, true);
+    if (!x_slots && fast.time + copy_time(z.rows * k, z.es) < l.dw.time) {
+      l.dw = fast;
+      l.pad_x = true;
+      copy = std::max(copy, z.rows * k * z.es);
+    }
+  }
+  l.dz_ld = whole(z.Nw, z.es);
+  l.sums = align256(z.rows * l.dz_ld * z.es);
+  l.copy = l.sums + align256(max_row_tiles(z.rows, z.G, kGradRows) * z.Nw * 4);
+  l.part = l.copy + align256(copy);
+  l.total = l.part + align256(std::max(l.dx.part_bytes, l.dw.part_bytes));
+  return l;
+}
+
+// Rows (per group: `per`) of len elements into rows of whole slots.
+hipError_t launch_pad(int dtype, const void* src, int64_t ld, int64_t group, int64_t groups, int64_t per, int64_t len,
+                      char* dst, hipStream_t s) {
+  const int64_t rows = groups * per;
+  const unsigned blocks = static_cast<unsigned>(cdiv(rows, kPWaves));
+  const int slots = static_cast<int>(cdiv(len * dtype_bytes(dtype), 16)), n = static_cast<int>(len);
+  const char* p = static_cast<const char*>(src);
+  switch (dtype) {
+    case kF32: pad_kernel<kF32><<<blocks, kPThreads, 0, s>>>(p, ld, group, per, n, dst, slots, rows); break;
+    case kF16: pad_kernel<kF16><<<blocks, kPThreads, 0, s>>>(p, ld, group, per, n, dst, slots, rows); break;
+    default: pad_kernel<kBF16><<<blocks, kPThreads, 0, s>>>(p, ld, group, per, n, dst, slots, rows); break;
+  }
+  return hipGetLastError();
 }
 
 struct Groups {
@@ -376,19 +454,32 @@ int forward(const Sizes& z, const void* x, int64_t x_stride, const void* weight,
     return SMX_ERR_MISALIGNED;
   const bool slots = whole_slots(x, x_stride, z.K, z.es) && whole_slots(weight, weight_stride, z.K, z.es) &&
                      g.stride * z.es % 16 == 0;
-  const ProductPlan plan = plan_product(kForward, z.dtype, z.rows, z.Nw, z.K, z.G, z.Nw != z.N, slots);
-  if (plan.part_bytes > 0) {
-    if (!workspace || workspace_bytes < static_cast<size_t>(plan.part_bytes)) return SMX_ERR_WORKSPACE;
+  const Layout l = forward_layout(z, slots, g.slots == nullptr);
+  if (l.total > 0) {
+    if (!workspace || workspace_bytes < static_cast<size_t>(l.total)) return SMX_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return SMX_ERR_MISALIGNED;
   }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
   ProductArgs a = group_args(z, g);
   a.q = static_cast<const char*>(x);
   a.q_ld = x_stride;
   a.p = static_cast<const char*>(weight);
   a.p_ld = weight_stride;
   a.p_group = g.stride;
+  int64_t depth = z.K;
+  if (l.pad) {
+    depth = whole(z.K, z.es);
+    hipError_t err = launch_pad(z.dtype, x, x_stride, 0, 1, z.rows, z.K, ws + l.x, s);
+    if (err == hipSuccess) err = launch_pad(z.dtype, weight, weight_stride, g.stride, z.G, z.Nw, z.K, ws + l.w, s);
+    if (err != hipSuccess) return static_cast<int>(err);
+    a.q = ws + l.x;
+    a.p = ws + l.w;
+    a.q_ld = a.p_ld = depth;
+    a.p_group = z.Nw * depth;
+  }
   a.cols = static_cast<int>(z.Nw);
-  a.depth = static_cast<int>(z.K);
+  a.depth = static_cast<int>(depth);
   a.gated = z.Nw != z.N;
   a.out = static_cast<char*>(y);
   a.out_ld = y_stride;
@@ -398,13 +489,13 @@ int forward(const Sizes& z, const void* x, int64_t x_stride, const void* weight,
   a.res_ld = residual_stride;
   a.z = preact;
   a.z_ld = z.Nw;
-  a.part = static_cast<float*>(workspace);
+  a.part = reinterpret_cast<float*>(ws + l.part);
   a.act = a.gated ? kActNone : z.act;
   a.out_cols = static_cast<int>(z.N);
   const int64_t v = 4 * z.es;
   a.vec = z.N % 4 == 0 && y_stride % 4 == 0 && aligned(y, v) && aligned(bias, v) && aligned(preact, 16) &&
           (!residual || (residual_stride % 4 == 0 && aligned(residual, v)));
-  return run_product(kForward, z.dtype, plan, a, fill, static_cast<hipStream_t>(stream));
+  return run_product(kForward, z.dtype, l.plan, a, fill, s);
 }
 
 int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* preact, const void* x, int64_t x_stride,
@@ -416,12 +507,10 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
   if (rc == SMX_OK) rc = check_pitch(dy_stride, z.N, z.es);
   if (rc != SMX_OK) return rc;
   if (g.slots && (grad_weight || grad_bias)) return SMX_ERR_INVALID_ARG;
-  // dz is dy itself, or rows of whole slots in the workspace
-  const bool own_dz = z.act != SMX_ACT_NONE;
-  const bool dz_slots = z.Nw * z.es % 16 == 0 && (own_dz || whole_slots(dy, dy_stride, z.N, z.es));
-  const bool dx_slots = dz_slots && whole_slots(weight, weight_stride, z.K, z.es) && g.stride * z.es % 16 == 0;
-  const bool dw_slots = dz_slots && whole_slots(x, x_stride, z.K, z.es);
-  const GradLayout l = grad_layout(z, dx_slots, dw_slots);
+  // dz is dy itself where that is all right, or rows of whole slots in the workspace
+  const bool own_dz = z.act != SMX_ACT_NONE || !whole_slots(dy, dy_stride, z.N, z.es);
+  const GradLayout l = grad_layout(z, whole_slots(weight, weight_stride, z.K, z.es) && g.stride * z.es % 16 == 0,
+                                   whole_slots(x, x_stride, z.K, z.es), g.slots == nullptr);
   if (l.dz_ld * z.es > kPMaxPitch || z.K * z.es > kPMaxPitch) return SMX_ERR_UNSUPPORTED;
   if (z.rows > 0) {
     if (!dy || (grad_weight && !x) || (grad_x && !weight) || (z.act != SMX_ACT_NONE && !preact)) return SMX_ERR_INVALID_ARG;
@@ -441,18 +530,20 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
   ag.p.gated = z.Nw != z.N;
   ag.p.act = z.act;
   ag.max_tiles = static_cast<int>(max_row_tiles(z.rows, z.G, kGradRows));
-  if (z.rows > 0 && (z.act != SMX_ACT_NONE || grad_bias)) {
+  if (z.rows > 0 && (own_dz || grad_bias)) {
     ag.dy = static_cast<const char*>(dy);
     ag.dy_ld = dy_stride;
     ag.p.vec = z.N % 4 == 0 && dy_stride % 4 == 0 && aligned(dy, 4 * z.es);
+    if (own_dz) {
+      ag.dz = ws + l.dz;
+      ag.dz_ld = l.dz_ld;
+      dz = ag.dz;
+      dz_ld = l.dz_ld;
+    }
     if (z.act != SMX_ACT_NONE) {
       ag.z = preact;
       ag.z_ld = z.Nw;
-      ag.dz = ws + l.dz;
-      ag.dz_ld = l.dz_ld;
       ag.p.vec = ag.p.vec && aligned(preact, 16);
-      dz = ag.dz;
-      dz_ld = l.dz_ld;
     }
     if (grad_bias) ag.sums = reinterpret_cast<float*>(ws + l.sums);
     const int64_t blocks = max_row_tiles(z.rows, z.G, kGradRows) * cdiv(z.N, kGradCols);
@@ -480,6 +571,7 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return static_cast<int>(err);
   }
+  const int64_t padded = whole(z.K, z.es);
   if (grad_x && z.rows > 0) {
     ProductArgs a = group_args(z, g);
     a.q = static_cast<const char*>(dz);
@@ -488,6 +580,14 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
     a.p_ld = weight_stride;
     a.p_group = g.stride;
     a.cols = a.out_cols = static_cast<int>(z.K);
+    if (l.pad_w) {
+      hipError_t err = launch_pad(z.dtype, weight, weight_stride, g.stride, z.G, z.Nw, z.K, ws + l.copy, s);
+      if (err != hipSuccess) return static_cast<int>(err);
+      a.p = ws + l.copy;
+      a.p_ld = padded;
+      a.p_group = z.Nw * padded;
+      a.cols = static_cast<int>(padded);
+    }
     a.depth = static_cast<int>(z.Nw);
     a.out = static_cast<char*>(grad_x);
     a.out_ld = z.K;
@@ -500,10 +600,18 @@ int gradients(const Sizes& z, const void* dy, int64_t dy_stride, const float* pr
     ProductArgs a = group_args(z, g);
     a.q = static_cast<const char*>(dz);
     a.q_ld = dz_ld;
+    a.q_cols = static_cast<int>(own_dz ? l.dz_ld : z.Nw);
     a.p = static_cast<const char*>(x);
     a.p_ld = x_stride;
     a.rows = static_cast<int>(z.Nw);
     a.cols = a.out_cols = static_cast<int>(z.K);
+    if (l.pad_x) {
+      hipError_t err = launch_pad(z.dtype, x, x_stride, 0, 1, z.rows, z.K, ws + l.copy, s);
+      if (err != hipSuccess) return static_cast<int>(err);
+      a.p = ws + l.copy;
+      a.p_ld = padded;
+      a.cols = static_cast<int>(padded);
+    }
     a.depth = static_cast<int>(z.rows);
     a.out = static_cast<char*>(grad_weight);
     a.out_ld = z.K;
@@ -525,9 +633,11 @@ extern "C" {
 size_t smx_linear_workspace_size(int64_t rows, int64_t K, int64_t N, int64_t G, int activation, int dtype) {
   Sizes z;
   if (check_sizes(rows, K, N, G, activation, dtype, z) != SMX_OK) return 0;
-  // whatever the alignment
-  return static_cast<size_t>(std::max(plan_product(kForward, dtype, rows, z.Nw, K, z.G, z.Nw != N, true).part_bytes,
-                                      plan_product(kForward, dtype, rows, z.Nw, K, z.G, z.Nw != N, false).part_bytes));
+  // whatever the alignment, with and without a slot map
+  int64_t n = 0;
+  for (const bool slots : {true, false})
+    for (const bool may_pad : {true, false}) n = std::max(n, forward_layout(z, slots, may_pad).total);
+  return static_cast<size_t>(n);
 }
 
 int smx_linear(const void* x, int64_t x_stride, int dtype, int64_t rows, int64_t K, const void* weight,
@@ -556,7 +666,11 @@ int smx_grouped_linear(const void* x, int64_t x_stride, int dtype, int64_t rows,
 size_t smx_linear_grad_workspace_size(int64_t rows, int64_t K, int64_t N, int64_t G, int activation, int dtype) {
   Sizes z;
   if (check_sizes(rows, K, N, G, activation, dtype, z) != SMX_OK) return 0;
-  return static_cast<size_t>(std::max(grad_layout(z, true, true).total, grad_layout(z, false, false).total));
+  int64_t n = 0;
+  for (const bool w : {true, false})
+    for (const bool x : {true, false})
+      for (const bool may_pad : {true, false}) n = std::max(n, grad_layout(z, w, x, may_pad).total);
+  return static_cast<size_t>(n);
 }
 
 int smx_linear_grad(const void* dy, int64_t dy_stride, const float* preact, const void* x, int64_t x_stride, int dtype,

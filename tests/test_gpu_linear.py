@@ -94,6 +94,29 @@ def _check_grouped(x, w, off, b, r, act, dy=None, slots=None, what=""):
 
 # rows, columns of x, columns of y: single elements, odd sizes, one more and one less than tiles, few rows
 # and many, aligned and not
+# (large products of whole and of odd sizes run on other tiles, and on padded copies)
+LARGE = [(4096, 512, 1024), (2048, 2048, 264), (3000, 1001, 777), (1100, 4100, 520), (700, 328, 4104), (260, 9000, 300),
+         (5000, 72, 1600), (40, 2056, 4096), (100, 1030, 2050)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,k,n", LARGE)
+def test_large_dense(rows, k, n, dtype):
+    act = ACTS[(rows + k + n) % len(ACTS)]
+    x, w, b, r, dy = _inputs(rows, k, n, act, dtype)
+    _check_dense(x, w, b, r, act, dy, what=f"{rows} x {k} x {n} {act}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,k,n,groups,act", [(9000, 512, 768, 5, "swiglu"), (6000, 264, 520, 40, None),
+                                                 (4000, 1025, 515, 3, "gelu"), (700, 1024, 704, 70, "silu")])
+def test_large_grouped(rows, k, n, groups, act, dtype):
+    x, w, b, r, dy = _inputs(rows, k, n, act, dtype, groups=groups)
+    cut = torch.randint(0, rows + 1, (groups - 1,), generator=torch.Generator().manual_seed(k)).sort().values.tolist()
+    off = torch.tensor([0, *cut, rows - rows // 9 if max(cut) <= rows - rows // 9 else rows], device=DEV)
+    _check_grouped(x, w, off, b, r, act, dy, what=f"{rows} x {k} x {n} in {groups} {act}")
+
+
 SIZES = [(1, 1, 1), (1, 8, 16), (3, 5, 7), (2, 64, 64), (17, 129, 30), (16, 256, 512), (33, 1024, 96), (63, 72, 136),
          (65, 130, 66), (128, 256, 128), (129, 264, 260), (200, 333, 515), (257, 64, 300), (300, 704, 257),
          (512, 512, 512), (1000, 200, 24)]
