@@ -18,7 +18,6 @@ import functools
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._torch import dtype_code, workspace
@@ -209,9 +208,24 @@ class _Product(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        # (the refusal to differentiate twice costs more than the rest of this function: only where a graph of
-        # the backward pass is recorded)
-        return _gradients_once(ctx, dy) if torch.is_grad_enabled() else _gradients(ctx, dy)
+        if not torch.is_grad_enabled():
+            return _gradients(ctx, dy)
+        # a graph of the gradients themselves is recorded: they depend on dy, x and the weight in a way that it cannot
+        # differentiate, and says so if it comes to that
+        with torch.no_grad():
+            grads = _gradients(ctx, dy)
+        deps = (dy, *ctx.saved_tensors[:2])
+        return (*(None if g is None else _Once.apply(g, *deps) for g in grads[:3]), *grads[3:])
+
+
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, *deps):
+        return grad
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("fused_linear and grouped_linear are differentiable once")
 
 
 def _gradients(ctx, dy):
@@ -220,9 +234,6 @@ def _gradients(ctx, dy):
     if need_x or need_w or need_b:
         grads = _backward(ctx.sizes, dy, ctx.saved_tensors, need_x, need_w, need_b)
     return (*grads, dy if need_r else None, None, None, None, None)
-
-
-_gradients_once = once_differentiable(_gradients)
 
 
 def _run(x, weight, bias, activation, residual, offsets, slots, out):

@@ -389,6 +389,61 @@ def test_captured_training_step(rows):
         assert all(torch.equal(p, q) for p, q in zip(got, want)), (i, [torch.equal(p, q) for p, q in zip(got, want)])
 
 
+@pytest.mark.parametrize("act", [a for a in ACTS if a != "relu"])
+def test_gradients_against_differences(act):
+    """Directional derivatives of the kernels' own fp32 loss, in each input."""
+    rows, k, n = 40, 48, 32
+    x, w, b, r, dy = _inputs(rows, k, n, act, F32)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    grads = torch.autograd.grad(fused_linear(x, w, b, act, r), leaves, dy)
+    h = 2.0 ** -7
+    g = _gen(5)
+
+    def loss(args):
+        with torch.no_grad():
+            return (fused_linear(*args[:3], act, args[3]).to(F64) * dy.to(F64)).sum()
+
+    for i, grad in enumerate(grads):
+        v = _randn(g, *leaves[i].shape, dtype=F32)
+        v = v / v.norm()
+        ends = []
+        for s in (h, -h):
+            args = [t.detach() for t in leaves]
+            args[i] = args[i] + s * v
+            ends.append(loss(args))
+        want = float((ends[0] - ends[1]) / (2 * h))
+        got = float((grad.to(F64) * v.to(F64)).sum())
+        # A unit step moves every z by at most |x row| or |w row| (below 4 sqrt(k)) times its share of v; the loss
+        # differs from its tangent by h^2 / 6 times third derivatives (below 2 for every activation, times |up| < 6
+        # for swiglu) of the moved z's, cubes summed: below 40 * |dy| here; and by the rounding of 2 * 1280 outputs of
+        # size 4 in fp32, 2^-24 * 4 each, summed at random, over 2 h
+        slack = h * h / 6 * 12 * 40 * float(dy.abs().max()) + 2 ** -22 * (2 * rows * n) ** 0.5 * 4 / (2 * h)
+        assert abs(got - want) <= slack, (act, i, got, want, slack)
+        # and the slack is small beside what a wrong gradient would show
+        assert slack < 0.5 * float(grad.norm()), (act, i)
+
+
+def test_differentiable_once():
+    x, w, b, _, dy = _inputs(8, 16, 24, "silu", F32)
+    x.requires_grad_()
+    y = fused_linear(x, w, b, "silu")
+    (dx,) = torch.autograd.grad(y, [x], dy, create_graph=True)
+    check(dx.detach(), *product(x.detach(), w, b, "silu", None, F32, dy)["dx"])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(dx.sum(), [x])
+
+
+def test_saved_tensors_may_move():
+    """Activations kept on the host between the passes."""
+    x, w, b, r, dy = _inputs(40, 64, 48, "gelu", BF16, groups=2)
+    off = torch.tensor([0, 10, 40], device=DEV)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(grouped_linear(x, w, off, b, "gelu"), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = grouped_linear(x, w, off, b, "gelu")
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
 def test_refusals_on_the_gpu():
     x, w, b, r, _ = _inputs(8, 16, 24, None, BF16, groups=2)
     off = torch.tensor([0, 4, 8], device=DEV)
