@@ -58,6 +58,7 @@ struct ProductArgs {
   int splits, split_steps;  // contraction splits, steps of kPStep bytes in each
   int act;
   int out_cols;             // columns of out: cols, or half of them where gated
+  int stream;               // results are stored past the caches
   int vec;                  // 4 consecutive outputs are one aligned store in every array
   int item_blocks;          // workgroups of the product; those behind fill rows of no group
   int fill_blocks;
@@ -343,44 +344,63 @@ __device__ __forceinline__ u32x4 load_slot(const typename Elem<DT>::S* at, int h
   return r;
 }
 
-// Four consecutive elements of an array of T (DT), those from column `n` on left alone.
+// Four consecutive elements of an array of T (DT), of which `left` exist: one access where all four do (`vec`: an aligned
+// one).
 template <int DT>
 __device__ __forceinline__ f32x4 load4(const char* base, int64_t at, int left, bool vec) {
   using S = typename Elem<DT>::S;
   const S* s = reinterpret_cast<const S*>(base) + at;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (vec) {
-    if constexpr (DT == kF32) {
-      v = *reinterpret_cast<const f32x4*>(s);
-    } else {
-      const u32x2 b = *reinterpret_cast<const u32x2*>(s);
+  auto widen = [&](const u32x2& b) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = Elem<DT>::to_f32(static_cast<uint16_t>(b[e >> 1] >> (16 * (e & 1))));
-    }
+    for (int e = 0; e < 4; ++e) v[e] = Elem<DT>::to_f32(static_cast<typename Elem<DT>::S>(b[e >> 1] >> (16 * (e & 1))));
+  };
+  if constexpr (DT == kF32) {
+    if (vec) v = *reinterpret_cast<const f32x4*>(s);
+    else if (left >= 4) __builtin_memcpy(&v, s, 16);
   } else {
+    u32x2 b;
+    if (vec) {
+      widen(*reinterpret_cast<const u32x2*>(s));
+    } else if (left >= 4) {
+      __builtin_memcpy(&b, s, 8);
+      widen(b);
+    }
+  }
+  if (!vec && left < 4) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 3; ++e)
       if (e < left) v[e] = Elem<DT>::to_f32(s[e]);
   }
   return v;
 }
 
+// Four values rounded to T, as they lie in memory.
 template <int DT>
-__device__ __forceinline__ void store4(char* base, int64_t at, int left, bool vec, const f32x4& v) {
+__device__ __forceinline__ auto pack4(const f32x4& v) {
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  if constexpr (DT == kF32) return v;
+  else if constexpr (DT == kBF16) return __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
+  else return __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4));
+}
+
+// stream: past the caches.
+template <int DT>
+__device__ __forceinline__ void store4(char* base, int64_t at, int left, bool vec, const f32x4& v, bool stream = false) {
   using S = typename Elem<DT>::S;
   S* s = reinterpret_cast<S*>(base) + at;
-  if (vec) {
-    if constexpr (DT == kF32) {
-      *reinterpret_cast<f32x4*>(s) = v;
-    } else {
-      typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-      typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-      if constexpr (DT == kBF16) *reinterpret_cast<u32x2*>(s) = __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
-      else *reinterpret_cast<u32x2*>(s) = __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4));
-    }
+  const auto b = pack4<DT>(v);
+  using B = std::remove_const_t<decltype(b)>;
+  if (vec && stream) {
+    __builtin_nontemporal_store(b, reinterpret_cast<B*>(s));
+  } else if (vec) {
+    *reinterpret_cast<B*>(s) = b;
+  } else if (left >= 4) {
+    __builtin_memcpy(s, &b, sizeof b);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 3; ++e)
       if (e < left) s[e] = Elem<DT>::from_f32(v[e]);
   }
 }
@@ -411,7 +431,7 @@ __device__ __forceinline__ void finish_rows(const ProductArgs& a, const ProductI
   if (a.z != nullptr) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
-      if (in[n]) store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, v[n]);
+      if (in[n]) store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, v[n], a.stream);
   }
   activate_all<DT == kF32>(a.act, v);
   if (a.res != nullptr) {
@@ -420,7 +440,7 @@ __device__ __forceinline__ void finish_rows(const ProductArgs& a, const ProductI
   }
 #pragma unroll
   for (int n = 0; n < N; ++n)
-    if (in[n]) store4<DT>(a.out, it.g * a.out_group + row[n] * a.out_ld + col, left, a.vec, v[n]);
+    if (in[n]) store4<DT>(a.out, it.g * a.out_group + row[n] * a.out_ld + col, left, a.vec, v[n], a.stream);
 }
 
 // The same of a gated product: gate and up columns of outputs col .. col + 3.
@@ -437,8 +457,8 @@ __device__ __forceinline__ void finish_rows_gated(const ProductArgs& a, const in
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       if (!in[n]) continue;
-      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, gate[n]);
-      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + a.out_cols + col, left, a.vec, up[n]);
+      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + col, left, a.vec, gate[n], a.stream);
+      store4<kF32>(reinterpret_cast<char*>(a.z), row[n] * a.z_ld + a.out_cols + col, left, a.vec, up[n], a.stream);
     }
   }
   activate_all<DT == kF32>(kActSilu, gate);
@@ -446,7 +466,7 @@ __device__ __forceinline__ void finish_rows_gated(const ProductArgs& a, const in
   for (int n = 0; n < N; ++n) {
     gate[n] *= up[n];
     if (a.res != nullptr) gate[n] += res[n];
-    if (in[n]) store4<DT>(a.out, row[n] * a.out_ld + col, left, a.vec, gate[n]);
+    if (in[n]) store4<DT>(a.out, row[n] * a.out_ld + col, left, a.vec, gate[n], a.stream);
   }
 }
 
@@ -493,9 +513,10 @@ struct TileShape {
   enum Form { kStaged, kCopied, kWide, kRows, kRowsStaged, kShallow } form;
 };
 // kStaged: 64 x 64. kCopied: 128 x 128, and not grouped along the contraction 64 x 128, 32 x 128.
-// kShallow: 128 x 128, grouped along the contraction.
 hipError_t launch_product_tile(int dtype, bool p_strided, bool q_strided, bool depth_groups, const TileShape& t,
                                const ProductArgs& a, hipStream_t s);
+// kShallow: 128 x 128, grouped along the contraction, no splits.
+hipError_t launch_product_shallow(int dtype, const ProductArgs& a, hipStream_t s);
 // kWide: 16-bit types, 256 x 256.
 hipError_t launch_product_wide(int dtype, bool p_strided, bool q_strided, bool depth_groups, const ProductArgs& a,
                                hipStream_t s);

@@ -116,8 +116,7 @@ struct Waves {
 // the activation's code stands once.
 // c0: first product column of the tile (gated: 16 gate columns, the matching 16 up columns, and so on: twice the
 // first output column). wrow, wcol: the wave's place in the tile.
-// PLAIN: whole sums of a weight gradient, which are only rounded and stored.
-template <int DT, int NI, int NJ, int CJ, bool PLAIN>
+template <int DT, int NI, int NJ, int CJ>
 __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductItem& it, int c0, int wrow, int wcol,
                                             u32x4* lds, const f32x4 (&acc)[NI][NJ]) {
   constexpr int kS = 4 * NI;  // slots of a row
@@ -130,26 +129,6 @@ __device__ __forceinline__ void finish_wave(const ProductArgs& a, const ProductI
   const int s0 = a.gated ? (c >> 2) * 8 + (c & 3) : c;
   const int col = a.gated ? (c0 + wcol) / 2 + 4 * c : c0 + wcol + 4 * c;
   const int left = a.out_cols - col;
-  if constexpr (PLAIN) {
-    const int lc = lane % kS, lr = lane / kS;
-    const int pcol = c0 + wcol + 4 * lc, pleft = a.out_cols - pcol;
-#pragma unroll
-    for (int j0 = 0; j0 < NJ; j0 += CJ) {
-#pragma unroll
-      for (int j = 0; j < CJ; ++j)
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-          st[(j * 16 + (lane & 15)) * kS + ((4 * i + (lane >> 4)) ^ (lane & (kS - 1) & 15))] = acc[i][j0 + j];
-#pragma unroll 4
-      for (int y = lr; y < CJ * 16; y += kWave / kS) {
-        const f32x4 v = st[y * kS + (lc ^ (y & (kS - 1) & 15))];
-        const int r = wrow + j0 * 16 + y;
-        if (r < it.m && pleft > 0)
-          store4<DT>(a.out, it.g * a.out_group + (static_cast<int64_t>(it.row) + r) * a.out_ld + pcol, pleft, a.vec, v);
-      }
-    }
-    return;
-  }
   const bool part = a.splits > 1;
   const f32x4 bias0 = part ? f32x4{} : bias4<DT>(a, it, col, left);
   const f32x4 bias1 = part || !a.gated ? f32x4{} : bias4<DT>(a, it, a.out_cols + col, left);
@@ -275,7 +254,7 @@ __global__ __launch_bounds__(kPThreads) void product_staged_kernel(ProductArgs a
   u32x4* mine = (wave < 2 ? sp : sq) + (wave & 1) * (GP::kSlots / 2);
   static_assert(GP::kSlots == GQ::kSlots, "a square tile");
   constexpr int kChunk = GP::kSlots / 2 / (W::kNI * 64);
-  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ, false>(a, it, c0, wrow, wcol, mine, acc);
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
 }
 
 // Copies of one operand's steps straight into LDS: copy j of wave w fills stage slots 64 (4 j + w) .. in lane order.
@@ -315,12 +294,10 @@ __device__ __forceinline__ void bare_barrier() {  // without a memory fence, whi
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// The same tile with the operands copied straight into LDS. NS = 2 stages: while one step is multiplied the next one's
-// copies are under way, and the other workgroup of the CU covers the waits. One stage, for contractions of a few steps
-// (the weight gradient of groups of few rows): a workgroup is then one chain of latencies, bounds, copies, stores, and
-// four on a CU instead of two overlap them.
-template <int DT, int BM, int BN, int NS, bool PS, bool QS, bool DG>
-__global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_kernel(ProductArgs a) {
+// The same tile with the operands copied straight into LDS, two stages: while one step is multiplied the next one's
+// copies are under way, and the other workgroup of the CU covers the waits.
+template <int DT, int BM, int BN, bool PS, bool QS, bool DG>
+__global__ __launch_bounds__(kPThreads, 2) void product_copied_kernel(ProductArgs a) {
   using GP = Stage<DT, BN, PS>;
   using GQ = Stage<DT, BM, QS>;
   using W = Waves<BM, BN>;
@@ -333,7 +310,7 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
   ProductItem it;
   const int col_tiles = (a.gated ? (a.out_cols + BN / 2 - 1) / (BN / 2) : (a.cols + BN - 1) / BN);
   if (!(DG ? find_depth_item(a, b, BM, col_tiles, it) : find_row_item(a, b, BM, col_tiles, it))) return;
-  __shared__ u32x4 p0[GP::kSlots], q0[GQ::kSlots], p1[NS > 1 ? GP::kSlots : 1], q1[NS > 1 ? GQ::kSlots : 1];
+  __shared__ u32x4 p0[GP::kSlots], p1[GP::kSlots], q0[GQ::kSlots], q1[GQ::kSlots];
 
   const int c0 = it.ct * BN;
   const int cfirst = a.gated ? c0 / 2 : c0;
@@ -364,10 +341,10 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
     cq.copy(sq, wave, s, left);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // one step, with the copies of the step NS later behind it; or one of the last NS, without them
+  // one step, with the copies of the step after the next behind it; or one of the last two, without them
   auto step = [&](u32x4* sp, u32x4* sq, int s, auto more) {
     // this step's copies have landed, the next one's may be under way
-    if constexpr (decltype(more)::value) __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * kCopies));
+    if constexpr (decltype(more)::value) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kCopies));
     else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     bare_barrier();
 #pragma unroll
@@ -385,7 +362,7 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (decltype(more)::value) {
       bare_barrier();  // every wave has read the stage (its fragments are in registers: the MFMAs are issued)
-      copy(sp, sq, s + NS);
+      copy(sp, sq, s + 2);
     }
   };
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
@@ -394,56 +371,47 @@ __global__ __launch_bounds__(kPThreads, NS == 1 ? 4 : 2) void product_copied_ker
   const std::false_type last{};
   if (s0 < s1) {
     copy(p0, q0, s0);
-    if constexpr (NS == 1) {
-      for (int s = s0; s + 1 < s1; ++s) step(p0, q0, s, more);
-      step(p0, q0, s1 - 1, last);
-    } else {
-      copy(p1, q1, s0 + 1);
-      int s = s0;
-      for (; s + 2 < s1; s += 2) {
-        step(p0, q0, s, more);
-        step(p1, q1, s + 1, more);
-        if (DT == kF32 && (s - s0) % kFold == kFold - 2) fold(total, acc);
-      }
-      // (a step past the end multiplies zeros: a branch inside the loop costs waits for all copies)
-      step(p0, q0, s, last);
-      step(p1, q1, s + 1, last);
+    copy(p1, q1, s0 + 1);
+    int s = s0;
+    for (; s + 2 < s1; s += 2) {
+      step(p0, q0, s, more);
+      step(p1, q1, s + 1, more);
+      if (DT == kF32 && (s - s0) % kFold == kFold - 2) fold(total, acc);
     }
+    // (a step past the end multiplies zeros: a branch inside the loop costs waits for all copies)
+    step(p0, q0, s, last);
+    step(p1, q1, s + 1, last);
   }
-  if constexpr (DT == kF32 && NS > 1) {  // (one stage: for short chains)
+  if constexpr (DT == kF32) {
     fold(total, acc);
     fold(acc, total);
   }
   __syncthreads();
-  // the wave's part of LDS
-  u32x4* mine;
+  u32x4* mine = wave == 0 ? p0 : wave == 1 ? p1 : wave == 2 ? q0 : q1;
   constexpr int kSmall = GP::kSlots < GQ::kSlots ? GP::kSlots : GQ::kSlots;
-  if constexpr (NS == 1) mine = (wave < 2 ? p0 : q0) + (wave & 1) * (kSmall / 2);
-  else mine = wave == 0 ? p0 : wave == 1 ? p1 : wave == 2 ? q0 : q1;
-  constexpr int kChunk = (NS == 1 ? kSmall / 2 : kSmall) / (W::kNI * 64);
+  constexpr int kChunk = kSmall / (W::kNI * 64);
   static_assert(kChunk >= 1, "a row tile of the wave fits its LDS");
-  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ, NS == 1>(a, it, c0, wrow, wcol, mine, acc);
+  finish_wave<DT, W::kNI, W::kNJ, kChunk < W::kNJ ? kChunk : W::kNJ>(a, it, c0, wrow, wcol, mine, acc);
 }
 
-template <int DT, int BM, int BN, int NS>
+template <int DT, int BM, int BN>
 static hipError_t copied_launch(bool ps, bool qs, bool dg, const ProductArgs& a, hipStream_t s) {
   const unsigned blocks = static_cast<unsigned>(a.item_blocks + a.fill_blocks);
   // whole 16-byte slots: the contraction of a contiguous operand, the columns (rows) of a strided one
   constexpr int n = 16 / dtype_bytes(DT);
-  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0 || (NS == 1 && a.splits != 1)) return hipErrorInvalidValue;
+  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.p_group % n != 0) return hipErrorInvalidValue;
   // (beside a strided P a contiguous Q may end inside a slot, with zeros up to the slot's end)
   if (!ps && a.depth % n != 0) return hipErrorInvalidValue;
   if ((ps && a.cols % n != 0) || (qs && (a.q_cols % n != 0 || a.q_cols < a.rows))) return hipErrorInvalidValue;
   if (dg) {
     if constexpr (BM == BN) {
       if (!ps || !qs) return hipErrorInvalidValue;
-      product_copied_kernel<DT, BM, BN, NS, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
+      product_copied_kernel<DT, BM, BN, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
     } else return hipErrorInvalidValue;
   } else {
-    if constexpr (NS == 1) return hipErrorInvalidValue;
-    else if (qs) return hipErrorInvalidValue;
-    else if (ps) product_copied_kernel<DT, BM, BN, NS, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
-    else product_copied_kernel<DT, BM, BN, NS, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
+    if (qs) return hipErrorInvalidValue;
+    if (ps) product_copied_kernel<DT, BM, BN, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
+    else product_copied_kernel<DT, BM, BN, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
   }
   return hipGetLastError();
 }
@@ -458,14 +426,190 @@ static hipError_t staged_launch(bool ps, bool qs, bool dg, const ProductArgs& a,
   return hipGetLastError();
 }
 
+// TileCopy of a strided operand in few registers: a wave's copies lie kRows contraction rows apart, and rows twice as
+// far apart share their slot permutation.
+template <int DT, int R>
+struct StridedCopy {
+  using G = Stage<DT, R, true>;
+  static constexpr int kRows = kPThreads / G::kRowSlots;
+  const char* base;
+  int64_t step_bytes;
+  uint32_t copy_bytes;
+  uint32_t off[2];  // copies of even and odd j
+  int k;            // the lane's contraction row within a step, copy 0
+  __device__ __forceinline__ void init(int wave, int64_t pitch, int last) {
+    step_bytes = G::kDepth * pitch;
+    copy_bytes = static_cast<uint32_t>(kRows * pitch);
+    k = (wave * kWave + lane_id()) / G::kRowSlots;
+#pragma unroll
+    for (int o = 0; o < 2; ++o)
+      off[o] = static_cast<uint32_t>(k * pitch) + min(G::perm(k + kRows * o, lane_id() % G::kRowSlots) * 16, last);
+  }
+  __device__ __forceinline__ void copy(u32x4* st, int wave, int step, int left) const {
+    const auto r = make_rsrc(base + step * step_bytes, left > 0 ? kPOutside : 0u);
+#pragma unroll
+    for (int j = 0; j < G::kLoads; ++j) {
+      const uint32_t o = k + kRows * j < left ? off[j & 1] : kPOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          r, (__attribute__((address_space(3))) void*)(st + (j * kPWaves + wave) * kWave), 16, o, j * copy_bytes, 0, 0);
+    }
+  }
+};
+
+// Weight gradients of groups of few rows: 128 x 128 tiles whose contraction is a few steps, so that a tile is a chain of
+// latencies (bounds, copies, stores) and the outputs' bytes bound the whole. One stage of 32 KB, so that four workgroups share
+// a CU; each walks over tiles, and sends the next tile's first copies out before it stores the last one's sums, straight from
+// the accumulators. Sums of two 16-column tiles are joined by a lane swap into 16-byte stores. The stores go out as buffer stores whose
+// lanes outside the result are turned off by their offset: always the same number of them, so that the next tile waits
+// for its copies (older than the stores) and not for the stores.
+// 64 groups of 192 rows on average, 2816 x 2048 (738 MB of results, 142 GFLOP): 256 x 256 tiles 472 us, 128 x 128 in two
+// stages 454, in one stage with a workgroup per tile and the sums through LDS 318, this 252 (2.9 TB/s of results); 16 rows
+// a group 350, 305, 225 and 162 (4.6 TB/s).
+// Past the caches where the tiles' operands are read more than once (more than one step): the results' bytes would drive them
+// out of L2 (192 rows a group 380 -> 250 us). Not for a single step, where nothing is lost and L2 joins the two halves
+// of each 128-byte line that two stores write (16 rows a group 167 us, past the caches 243).
+__device__ __forceinline__ void store_slot(__amdgpu_buffer_rsrc_t r, const u32x4& v, uint32_t off, bool stream) {
+  if (stream) __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, kNonTemporal);
+  else __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductArgs a) {
+  constexpr int kTile = 128;
+  using G = Stage<DT, kTile, true>;
+  using W = Waves<kTile, kTile>;
+  constexpr int64_t kEs = G::kEs;
+  constexpr int kStores = DT == kF32 ? W::kNI * W::kNJ : W::kNI * W::kNJ / 2;  // per wave and tile
+  const int col_tiles = (a.cols + kTile - 1) / kTile;
+  const int lane = lane_id(), wave = wave_id(), r = lane & 15, g = lane >> 4;
+  const int wrow = (wave / W::kColWaves) * W::kNJ * 16, wcol = (wave % W::kColWaves) * W::kNI * 16;
+  const int64_t p_pitch = a.p_ld * kEs, q_pitch = a.q_ld * kEs;
+  const bool slots = a.out_cols % G::kEps == 0 && a.out_ld % G::kEps == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  __shared__ u32x4 sp[G::kSlots], sq[G::kSlots];
+  StridedCopy<DT, kTile> cp, cq;
+  ProductItem it;
+  int b = static_cast<int>(blockIdx.x);
+  if (!find_depth_item(a, b, kTile, col_tiles, it)) return;
+  auto copy = [&](const ProductItem& t, int s) {
+    const int left = t.depth - s * G::kDepth;  // of an empty group: no reads, zeros
+    cp.copy(sp, wave, s, left);
+    cq.copy(sq, wave, s, left);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto first = [&](const ProductItem& t) {
+    const int c0 = t.ct * kTile;
+    cp.base = a.p + t.k0 * p_pitch + c0 * kEs;
+    cq.base = a.q + t.k0 * q_pitch + t.row * kEs;
+    cp.init(wave, p_pitch, static_cast<int>((a.cols - c0) * kEs) - 16);
+    cq.init(wave, q_pitch, static_cast<int>((a.q_cols - t.row) * kEs) - 16);
+    copy(t, 0);
+  };
+  first(it);
+  bool stores = false;  // the last tile's are under way, behind this tile's first copies
+  for (;;) {
+    const int steps = max(1, (it.depth + G::kDepth - 1) / G::kDepth);
+    f32x4 acc[W::kNI][W::kNJ] = {};
+    for (int s = 0; s < steps; ++s) {
+      if (s == 0 && stores) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kStores));
+      else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      bare_barrier();
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 fp[W::kNI], fq[W::kNJ];
+#pragma unroll
+        for (int i = 0; i < W::kNI; ++i) fp[i] = G::frag(sp, wcol + i * 16, u);
+#pragma unroll
+        for (int j = 0; j < W::kNJ; ++j) fq[j] = G::frag(sq, wrow + j * 16, u);
+#pragma unroll
+        for (int i = 0; i < W::kNI; ++i)
+#pragma unroll
+          for (int j = 0; j < W::kNJ; ++j) acc[i][j] = Elem<DT>::mfma(fp[i], fq[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      bare_barrier();  // every wave has read the stage
+      if (s + 1 < steps) copy(it, s + 1);
+    }
+    const ProductItem done = it;
+    b += static_cast<int>(gridDim.x);
+    const bool more = b < a.item_blocks && find_depth_item(a, b, kTile, col_tiles, it);
+    if (more) first(it);
+    const int c0 = done.ct * kTile + wcol;
+    char* base = a.out + (done.g * a.out_group + done.row * a.out_ld) * kEs;
+    if (slots) {
+      const auto rs = make_rsrc(base, kPOutside);
+      auto put = [&](auto stream) {
+#pragma unroll
+        for (int j = 0; j < W::kNJ; ++j) {
+          const int row = wrow + j * 16 + r;
+          const uint32_t at = static_cast<uint32_t>(row * a.out_ld * kEs);
+          if constexpr (DT == kF32) {
+#pragma unroll
+            for (int i = 0; i < W::kNI; ++i) {
+              const int col = c0 + i * 16 + 4 * g;
+              store_slot(rs, __builtin_bit_cast(u32x4, acc[i][j]),
+                         row < done.m && col < a.out_cols ? at + col * static_cast<uint32_t>(kEs) : kPOutside,
+                         decltype(stream)::value);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < W::kNI; i += 2) {
+              const u32x2 lo = pack4<DT>(acc[i][j]), hi = pack4<DT>(acc[i + 1][j]);
+              const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(lo[0], hi[0], false, false));
+              const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(lo[1], hi[1], false, false));
+              const int col = c0 + (i + (g & 1)) * 16 + (g >> 1) * 8;  // the lane's 8 columns of the joined pair
+              store_slot(rs, u32x4{x[0], y[0], x[1], y[1]},
+                         row < done.m && col < a.out_cols ? at + col * static_cast<uint32_t>(kEs) : kPOutside,
+                         decltype(stream)::value);
+            }
+          }
+        }
+      };
+      if (steps > 1) put(std::true_type{});
+      else put(std::false_type{});
+    } else {
+#pragma unroll
+      for (int j = 0; j < W::kNJ; ++j) {
+        const int row = wrow + j * 16 + r;
+        if (row >= done.m) continue;
+#pragma unroll
+        for (int i = 0; i < W::kNI; ++i) {
+          const int col = c0 + i * 16 + 4 * g, left = a.out_cols - col;
+          if (left > 0) store4<DT>(base, row * a.out_ld + col, left, false, acc[i][j]);
+        }
+      }
+    }
+    if (!more) return;
+    stores = slots;
+  }
+}
+
+template <int DT>
+static hipError_t shallow_launch(const ProductArgs& a, hipStream_t s) {
+  constexpr int n = 16 / dtype_bytes(DT);
+  if (a.p_ld % n != 0 || a.q_ld % n != 0 || a.splits != 1 || a.cols % n != 0 || a.q_cols % n != 0 || a.q_cols < a.rows)
+    return hipErrorInvalidValue;
+  // as many workgroups as run at once; a multiple of 8, which keeps a workgroup's tiles on its XCD
+  const unsigned blocks = static_cast<unsigned>(a.item_blocks < 1024 ? a.item_blocks : 1024);
+  product_shallow_kernel<DT><<<blocks, kPThreads, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_product_shallow(int dtype, const ProductArgs& a, hipStream_t s) {
+  switch (dtype) {
+    case kF32: return shallow_launch<kF32>(a, s);
+    case kF16: return shallow_launch<kF16>(a, s);
+    case kBF16: return shallow_launch<kBF16>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 template <int DT>
 static hipError_t tile_launch(bool ps, bool qs, bool dg, const TileShape& t, const ProductArgs& a, hipStream_t s) {
   if (t.form == TileShape::kStaged && t.bm == 64 && t.bn == 64) return staged_launch<DT, 64, 64>(ps, qs, dg, a, s);
-  if (t.form == TileShape::kShallow && t.bm == 128 && t.bn == 128) return copied_launch<DT, 128, 128, 1>(ps, qs, dg, a, s);
   if (t.form != TileShape::kCopied || t.bn != 128) return hipErrorInvalidValue;
-  if (t.bm == 128) return copied_launch<DT, 128, 128, 2>(ps, qs, dg, a, s);
-  if (t.bm == 64) return copied_launch<DT, 64, 128, 2>(ps, qs, dg, a, s);
-  if (t.bm == 32) return copied_launch<DT, 32, 128, 2>(ps, qs, dg, a, s);
+  if (t.bm == 128) return copied_launch<DT, 128, 128>(ps, qs, dg, a, s);
+  if (t.bm == 64) return copied_launch<DT, 64, 128>(ps, qs, dg, a, s);
+  if (t.bm == 32) return copied_launch<DT, 32, 128>(ps, qs, dg, a, s);
   return hipErrorInvalidValue;
 }
 

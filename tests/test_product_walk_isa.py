@@ -98,7 +98,7 @@ def test_copied_walk(asm):
     walks = list(_walks(asm["product_tile.hip"], "product_copied_kernel"))
     seen = 0
     for name, ins in walks:
-        bm, bn, stages = map(int, re.search(r"ILi\dELi(\d+)ELi(\d+)ELi(\d+)E", name).groups())
+        bm, bn = map(int, re.search(r"ILi\dELi(\d+)ELi(\d+)E", name).groups())
         copies = (bm + bn) // 32
         ev = [e for e in _events(ins) if e in ("B", "C") or isinstance(e, int)]
         if "B" not in ev:
@@ -106,8 +106,8 @@ def test_copied_walk(asm):
         seen += 1
         # rotate to the first wait; then per step: wait, barrier, barrier, copies
         steps = ev.count("B") // 2
-        assert ev.count("B") == 2 * steps and steps in (1, 2), name
-        want = [(stages - 1) * copies, "B", "B"] + ["C"] * copies
+        assert ev.count("B") == 2 * steps and steps == 2, name
+        want = [copies, "B", "B"] + ["C"] * copies
         assert ev == want * steps, (name, ev)
     assert seen >= 3 * 3
 
