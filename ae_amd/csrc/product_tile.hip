@@ -457,34 +457,33 @@ struct StridedCopy {
 };
 
 // Weight gradients of groups of few rows: 128 x 128 tiles whose contraction is a few steps, so that a tile is a chain of
-// latencies (bounds, copies, stores) and the outputs' bytes bound the whole. One stage of 32 KB, so that four workgroups share
-// a CU; each walks over tiles, and sends the next tile's first copies out before it stores the last one's sums, straight from
-// the accumulators. Sums of two 16-column tiles are joined by a lane swap into 16-byte stores. The stores go out as buffer stores whose
-// lanes outside the result are turned off by their offset: always the same number of them, so that the next tile waits
-// for its copies (older than the stores) and not for the stores.
-// 64 groups of 192 rows on average, 2816 x 2048 (738 MB of results, 142 GFLOP): 256 x 256 tiles 472 us, 128 x 128 in two
-// stages 454, in one stage with a workgroup per tile and the sums through LDS 318, this 252 (2.9 TB/s of results); 16 rows
-// a group 350, 305, 225 and 162 (4.6 TB/s).
-// Past the caches where the tiles' operands are read more than once (more than one step): the results' bytes would drive them
-// out of L2 (192 rows a group 380 -> 250 us). Not for a single step, where nothing is lost and L2 joins the two halves
-// of each 128-byte line that two stores write (16 rows a group 167 us, past the caches 243).
+// latencies (bounds, copies, stores) and the results' bytes bound the whole. One stage of 32 KB, so that four workgroups
+// share a CU; each walks over tiles, and sends the next tile's first copies out before it stores the last one's sums. Those
+// go out as buffer stores whose lanes outside the result are turned off by their offset: always the same number of
+// them, so that the next tile waits for its copies (older than the stores) and not for the stores. 16-bit sums pass
+// through the stage first, so that a store writes whole lines (8 rows of 128 bytes): halves of lines, 64 bytes of each of
+// 16 rows, cost 474 us past the caches and 423 through them where this takes 351.
+// Large results go past the caches (ProductArgs::stream): their bytes would drive the tiles' operands out of L2.
+// 64 groups of 192 rows on average, 2816 x 2048 (738 MB of results, 142 GFLOP), behind another operator's traffic: 351 us
+// (2.1 TB/s of results; 379 through the caches), repeated alone 249; 16 rows a group 162 (4.6 TB/s) and 209. 256 x 256 tiles
+// 472 and 350 alone, 128 x 128 tiles in two stages 454 and 305.
 __device__ __forceinline__ void store_slot(__amdgpu_buffer_rsrc_t r, const u32x4& v, uint32_t off, bool stream) {
   if (stream) __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, kNonTemporal);
   else __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
 }
 
-template <int DT>
+// SLOTS: the results' rows are whole 16-byte slots too.
+template <int DT, bool SLOTS>
 __global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductArgs a) {
   constexpr int kTile = 128;
   using G = Stage<DT, kTile, true>;
   using W = Waves<kTile, kTile>;
   constexpr int64_t kEs = G::kEs;
-  constexpr int kStores = DT == kF32 ? W::kNI * W::kNJ : W::kNI * W::kNJ / 2;  // per wave and tile
+  constexpr int kStores = DT == kF32 ? W::kNI * W::kNJ : W::kNJ * 2;  // per wave and tile
   const int col_tiles = (a.cols + kTile - 1) / kTile;
   const int lane = lane_id(), wave = wave_id(), r = lane & 15, g = lane >> 4;
   const int wrow = (wave / W::kColWaves) * W::kNJ * 16, wcol = (wave % W::kColWaves) * W::kNI * 16;
   const int64_t p_pitch = a.p_ld * kEs, q_pitch = a.q_ld * kEs;
-  const bool slots = a.out_cols % G::kEps == 0 && a.out_ld % G::kEps == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
   __shared__ u32x4 sp[G::kSlots], sq[G::kSlots];
   StridedCopy<DT, kTile> cp, cq;
   ProductItem it;
@@ -530,56 +529,71 @@ __global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductAr
       if (s + 1 < steps) copy(it, s + 1);
     }
     const ProductItem done = it;
-    b += static_cast<int>(gridDim.x);
-    const bool more = b < a.item_blocks && find_depth_item(a, b, kTile, col_tiles, it);
-    if (more) first(it);
     const int c0 = done.ct * kTile + wcol;
     char* base = a.out + (done.g * a.out_group + done.row * a.out_ld) * kEs;
-    if (slots) {
-      const auto rs = make_rsrc(base, kPOutside);
-      auto put = [&](auto stream) {
-#pragma unroll
-        for (int j = 0; j < W::kNJ; ++j) {
-          const int row = wrow + j * 16 + r;
-          const uint32_t at = static_cast<uint32_t>(row * a.out_ld * kEs);
-          if constexpr (DT == kF32) {
-#pragma unroll
-            for (int i = 0; i < W::kNI; ++i) {
-              const int col = c0 + i * 16 + 4 * g;
-              store_slot(rs, __builtin_bit_cast(u32x4, acc[i][j]),
-                         row < done.m && col < a.out_cols ? at + col * static_cast<uint32_t>(kEs) : kPOutside,
-                         decltype(stream)::value);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < W::kNI; i += 2) {
-              const u32x2 lo = pack4<DT>(acc[i][j]), hi = pack4<DT>(acc[i + 1][j]);
-              const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(lo[0], hi[0], false, false));
-              const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(lo[1], hi[1], false, false));
-              const int col = c0 + (i + (g & 1)) * 16 + (g >> 1) * 8;  // the lane's 8 columns of the joined pair
-              store_slot(rs, u32x4{x[0], y[0], x[1], y[1]},
-                         row < done.m && col < a.out_cols ? at + col * static_cast<uint32_t>(kEs) : kPOutside,
-                         decltype(stream)::value);
-            }
-          }
-        }
-      };
-      if (steps > 1) put(std::true_type{});
-      else put(std::false_type{});
-    } else {
+    // 16-bit sums, rounded, through the wave's quarter of the stage: rows of 64 columns (128 bytes), slots permuted
+    constexpr int kRowsOf = 8;  // rows that one store covers, 8 lanes each
+    constexpr int kPacked = DT == kF32 ? 1 : W::kNJ * 16 / kRowsOf;
+    u32x4 packed[kPacked];
+    int ln = lane;  // (opaque: its addresses would otherwise be kept in registers through the whole walk)
+    asm volatile("" : "+v"(ln));
+    if constexpr (!SLOTS) {  // at once
 #pragma unroll
       for (int j = 0; j < W::kNJ; ++j) {
-        const int row = wrow + j * 16 + r;
+        const int row = wrow + j * 16 + (ln & 15);
         if (row >= done.m) continue;
 #pragma unroll
         for (int i = 0; i < W::kNI; ++i) {
-          const int col = c0 + i * 16 + 4 * g, left = a.out_cols - col;
+          const int col = c0 + i * 16 + 4 * (ln >> 4), left = a.out_cols - col;
           if (left > 0) store4<DT>(base, row * a.out_ld + col, left, false, acc[i][j]);
         }
       }
+    } else if constexpr (DT != kF32) {
+      u32x2* half = reinterpret_cast<u32x2*>((wave < 2 ? sp : sq) + (wave & 1) * (G::kSlots / 2));
+#pragma unroll
+      for (int j = 0; j < W::kNJ; ++j)
+#pragma unroll
+        for (int i = 0; i < W::kNI; ++i)
+          half[((j * 16 + (ln & 15)) * 8 + ((2 * i + (ln >> 5)) ^ (ln & 7))) * 2 + ((ln >> 4) & 1)] = pack4<DT>(acc[i][j]);
+      const u32x4* full = reinterpret_cast<const u32x4*>(half);
+#pragma unroll
+      for (int t = 0; t < kPacked; ++t) packed[t] = full[(t * 8 + (ln >> 3)) * 8 + ((ln & 7) ^ (ln >> 3))];
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt 0
+      bare_barrier();                      // the next tile's copies may come
+    }
+    b += static_cast<int>(gridDim.x);
+    const bool more = b < a.item_blocks && find_depth_item(a, b, kTile, col_tiles, it);
+    if (more) first(it);
+    if constexpr (SLOTS) {
+      const auto rs = make_rsrc(base, kPOutside);
+      auto put = [&](auto stream) {
+        if constexpr (DT == kF32) {
+#pragma unroll
+          for (int j = 0; j < W::kNJ; ++j) {
+            const int row = wrow + j * 16 + (ln & 15);
+#pragma unroll
+            for (int i = 0; i < W::kNI; ++i) {
+              const int col = c0 + i * 16 + 4 * (ln >> 4);
+              store_slot(rs, __builtin_bit_cast(u32x4, acc[i][j]),
+                         row < done.m && col < a.out_cols ? static_cast<uint32_t>((row * a.out_ld + col) * kEs) : kPOutside,
+                         decltype(stream)::value);
+            }
+          }
+        } else {
+          const int col = c0 + 8 * (ln & 7);
+          const uint32_t at = static_cast<uint32_t>(((wrow + (ln >> 3)) * a.out_ld + col) * kEs);
+          const int left = col < a.out_cols ? done.m - wrow - (ln >> 3) : 0;
+#pragma unroll
+          for (int t = 0; t < kPacked; ++t)
+            store_slot(rs, packed[t], t * kRowsOf < left ? at + static_cast<uint32_t>(t * kRowsOf * a.out_ld * kEs) : kPOutside,
+                       decltype(stream)::value);
+        }
+      };
+      if (a.stream) put(std::true_type{});
+      else put(std::false_type{});
     }
     if (!more) return;
-    stores = slots;
+    stores = SLOTS;
   }
 }
 
@@ -590,7 +604,9 @@ static hipError_t shallow_launch(const ProductArgs& a, hipStream_t s) {
     return hipErrorInvalidValue;
   // as many workgroups as run at once; a multiple of 8, which keeps a workgroup's tiles on its XCD
   const unsigned blocks = static_cast<unsigned>(a.item_blocks < 1024 ? a.item_blocks : 1024);
-  product_shallow_kernel<DT><<<blocks, kPThreads, 0, s>>>(a);
+  const bool slots = a.out_cols % n == 0 && a.out_ld % n == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+  if (slots) product_shallow_kernel<DT, true><<<blocks, kPThreads, 0, s>>>(a);
+  else product_shallow_kernel<DT, false><<<blocks, kPThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
