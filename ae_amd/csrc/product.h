@@ -512,7 +512,7 @@ struct TileShape {
   // The kernel: operands through registers (any alignment) or straight into LDS (whole 16-byte slots)
   enum Form { kStaged, kCopied, kWide, kRows, kRowsStaged, kShallow } form;
 };
-// kStaged: 64 x 64. kCopied: 128 x 128, and not grouped along the contraction 64 x 128, 32 x 128.
+// kStaged: 64 x 64. kCopied: 128 x 128, 64 x 64, and not grouped along the contraction 64 x 128, 32 x 128.
 hipError_t launch_product_tile(int dtype, bool p_strided, bool q_strided, bool depth_groups, const TileShape& t,
                                const ProductArgs& a, hipStream_t s);
 // kShallow: 128 x 128, grouped along the contraction, no splits.

@@ -622,6 +622,7 @@ hipError_t launch_product_shallow(int dtype, const ProductArgs& a, hipStream_t s
 template <int DT>
 static hipError_t tile_launch(bool ps, bool qs, bool dg, const TileShape& t, const ProductArgs& a, hipStream_t s) {
   if (t.form == TileShape::kStaged && t.bm == 64 && t.bn == 64) return staged_launch<DT, 64, 64>(ps, qs, dg, a, s);
+  if (t.form == TileShape::kCopied && t.bm == 64 && t.bn == 64) return copied_launch<DT, 64, 64>(ps, qs, dg, a, s);
   if (t.form != TileShape::kCopied || t.bn != 128) return hipErrorInvalidValue;
   if (t.bm == 128) return copied_launch<DT, 128, 128>(ps, qs, dg, a, s);
   if (t.bm == 64) return copied_launch<DT, 64, 128>(ps, qs, dg, a, s);

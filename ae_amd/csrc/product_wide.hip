@@ -350,9 +350,8 @@ __device__ __forceinline__ void wide_item(const ProductArgs& a, const ProductIte
   wide_finish<DT, BM, BN, NT>(a, it, w.wave, mine, acc);
 }
 
-// Two workgroups of the smaller tiles share a CU.
 template <int DT, int BM, int BN, bool PS, bool QS, bool DG>
-__global__ __launch_bounds__(kPThreads, BM * BN > 128 * 128 ? 1 : 2) void product_wide_kernel(ProductArgs a) {
+__global__ __launch_bounds__(kPThreads, 1) void product_wide_kernel(ProductArgs a) {
   using T = WideTile<BM, BN>;
   const int b = static_cast<int>(blockIdx.x);
   if (b >= a.item_blocks) {
@@ -424,12 +423,10 @@ __global__ __launch_bounds__(kPThreads, BM * BN > 128 * 128 ? 1 : 2) void produc
     for (int j = 0; j < T::kQCopies; ++j)
       w.q.off[j] = static_cast<uint32_t>(min(j * 32 + w.wave * 8 + (lane >> 3), it.m - 1) * q_pitch) + slot * 16;
   }
-  if constexpr (QS || BM == 64) {
+  if constexpr (QS) {
     wide_item<DT, BM, BN, T::kRows, PS, QS>(a, it, w, p0, q0, p1, q1);
-  } else if constexpr (BM == 128) {
-    if (it.m <= 64) wide_item<DT, BM, BN, 2, PS, QS>(a, it, w, p0, q0, p1, q1);
-    else wide_item<DT, BM, BN, 4, PS, QS>(a, it, w, p0, q0, p1, q1);
-  } else {
+  } else {  // items of few rows: only the row tiles that they have
+    static_assert(BM == 256, "2, 4, 6 or 8 row tiles per wave");
     switch ((it.m + 63) / 64) {
       case 1: wide_item<DT, BM, BN, 2, PS, QS>(a, it, w, p0, q0, p1, q1); break;
       case 2: wide_item<DT, BM, BN, 4, PS, QS>(a, it, w, p0, q0, p1, q1); break;
@@ -444,10 +441,8 @@ static hipError_t wide_launch(bool ps, bool qs, bool dg, const ProductArgs& a, h
   const unsigned blocks = static_cast<unsigned>(a.item_blocks + a.fill_blocks);
   if (!ps && !qs && !dg) product_wide_kernel<DT, BM, BN, false, false, false><<<blocks, kPThreads, 0, s>>>(a);
   else if (ps && !qs && !dg) product_wide_kernel<DT, BM, BN, true, false, false><<<blocks, kPThreads, 0, s>>>(a);
-  else if constexpr (BM >= 128) {
-    if (ps && qs && dg) product_wide_kernel<DT, BM, BN, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
-    else return hipErrorInvalidValue;
-  } else return hipErrorInvalidValue;
+  else if (ps && qs && dg) product_wide_kernel<DT, BM, BN, true, true, true><<<blocks, kPThreads, 0, s>>>(a);
+  else return hipErrorInvalidValue;
   return hipGetLastError();
 }
 

@@ -202,7 +202,9 @@ struct ProductPlan {
 // 1200, weight gradients of 1 to 100 groups of 3 to 800 rows, unaligned 1 to 3000 rows of 1999 -> 1333); the fit is
 // within about 20 % of what was measured, and where two tiles come closer than that either will do. Both sides of some
 // choices (us): 32 rows, 4096 -> 4096, 16 x 32 rows 11.4, 32 x 128 copied 33; 128 rows 28 and 64 x 64 rows 23; 512 rows
-// 64 x 64 rows 38.5, 64 x 128 copied 36; 2048 rows 128 x 128 73, wide 97; 4096 rows 129 and 117.
+// 64 x 64 rows 38.5, 64 x 128 copied 36; 2048 rows 128 x 128 73, wide 97; 4096 rows 129 and 117. 64 x 64 copied against
+// the tile without it: weight gradients of 1000 rows, 1024 -> 1024 in bf16, 8.4 and 14.2, of 777 rows, 1024 -> 2816 in
+// fp32 48 and 63, forward 200 rows, 2048 -> 6000 16.5 and 21.1, but of 4096 rows, 2048 -> 5632 165 and 100.
 struct TileCost {
   TileShape t;
   float end, first, each;
@@ -212,7 +214,8 @@ struct TileCost {
 using Tile = TileShape;
 constexpr TileCost kTileCosts[] = {
     {{16, 16, Tile::kRows}, 0.3f, 0.085f, 0.052f, 0.06f, 0.f},  {{16, 32, Tile::kRows}, 0.5f, 0.06f, 0.08f, 0.10f, 0.f},
-    {{32, 32, Tile::kRows}, 0.5f, 0.065f, 0.096f, 0.17f, 0.f},  {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
+    {{32, 32, Tile::kRows}, 0.8f, 0.065f, 0.085f, 0.17f, 0.f},  {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
+    {{64, 64, Tile::kCopied}, 1.0f, 0.10f, 0.20f, 0.50f, 1.2f},
     {{32, 128, Tile::kCopied}, 0.7f, 0.20f, 0.22f, 0.52f, 0.f}, {{64, 128, Tile::kCopied}, 1.0f, 0.20f, 0.30f, 1.0f, 0.f},
     {{128, 128, Tile::kCopied}, 3.5f, 0.20f, 0.43f, 1.95f, 4.5f}, {{128, 128, Tile::kShallow}, 1.4f, 0.2f, 0.55f, 2.3f, 1.4f},
     {{256, 256, Tile::kWide}, 10.f, 0.0f, 1.57f, 0.f, 16.f},
@@ -250,7 +253,7 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
     const bool may_split = !by_rows && t.form != Tile::kShallow && !(depth_groups && groups > 1);
     for (int splits = 1; splits <= 16 && (splits == 1 || (may_split && splits * 4 <= steps)); splits *= 2) {
       double n = std::max(1.0, tiles * splits / kCUs);
-      if (!by_rows) n = std::ceil(n);
+      if (!by_rows || t.bm == 64) n = std::ceil(n);  // (of the small tiles several run on a CU at once)
       double time = 2.5 + end * n + steps / splits * (c.first + each * n);
       if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch; partial sums out and in
       if (p.time != 0 && time >= p.time) continue;
