@@ -168,9 +168,11 @@ __device__ __forceinline__ bool find_row_item(const ProductArgs& a, int b, int b
     }
     incl = wave_incl_scan((n + bm - 1) / bm);
   };
+  // (as many tiles as the grid was made for, whatever the caller's bounds hold: bounds that decrease name rows twice)
+  const int most = a.rows / bm + min(a.groups, a.rows);
   for (int base = 0; base < a.groups; base += kWave) {
     scan(base);
-    rt += last_lane(incl);
+    rt = min(rt + last_lane(incl), most);
   }
   const int id = xcd_item(b, rt * col_tiles * a.splits);
   if (id < 0) return false;

@@ -179,6 +179,7 @@ __global__ __launch_bounds__(kPThreads) void join_kernel(ProductArgs a, int spli
 namespace {
 
 constexpr int64_t kMaxSize = int64_t{1} << 30;
+constexpr int64_t kMaxWeight = int64_t{1} << 40;  // bytes
 constexpr int kFillBlocks = 64;
 constexpr int64_t kL2Bytes = int64_t{32} << 20;
 
@@ -459,7 +460,9 @@ int forward(const Sizes& z, const void* x, int64_t x_stride, const void* weight,
   if (rc == SMX_OK) rc = check_pitch(y_stride, z.N, z.es);
   if (rc == SMX_OK && residual) rc = check_pitch(residual_stride, z.N, z.es);
   if (rc != SMX_OK) return rc;
-  if (z.Nw * weight_stride * z.es >= int64_t{kPOutside}) return SMX_ERR_UNSUPPORTED;
+  // (gate and up rows are reached from one base with 32-bit offsets; beyond any memory, a product of sizes gone wrong)
+  const int64_t extent = z.Nw * weight_stride * z.es;
+  if (extent >= (z.Nw != z.N ? int64_t{kPOutside} : kMaxWeight)) return SMX_ERR_UNSUPPORTED;
   if (z.rows == 0) return SMX_OK;
   if (!x || !weight || !y) return SMX_ERR_INVALID_ARG;
   if (!aligned(x, z.es) || !aligned(weight, z.es) || !aligned(y, z.es) || !aligned(bias, z.es) ||

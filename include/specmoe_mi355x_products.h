@@ -23,8 +23,9 @@
  *
  * Element type of every tensor but z and the maps: `dtype`. Rows of x, residual, y and dy lie
  * *_stride elements apart (>= their length), elements of a row side by side. Products are summed
- * in fp32 and y is rounded once. Any rows >= 0, K, N >= 1 up to 2^30 (rows * G tiles within 2^31),
- * pitches below 8 MiB; any alignment of elements (16-byte aligned rows are faster).
+ * in fp32 and y is rounded once. Any rows >= 0, K, N >= 1 up to 2^30, pitches below 8 MiB, as many
+ * output tiles as a grid holds (2^31 workgroups), a swiglu weight (of a group) below 2 GiB; any
+ * alignment of elements (16-byte aligned rows are faster). Other sizes: SMX_ERR_UNSUPPORTED.
  */
 #ifndef SPECMOE_MI355X_PRODUCTS_H
 #define SPECMOE_MI355X_PRODUCTS_H

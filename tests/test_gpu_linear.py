@@ -519,3 +519,62 @@ def test_trained_expert_block_together():
     for p, q in zip(got, torch.autograd.grad(z, c, dy.to(F64))):
         # fp32 sums of up to 130 terms through three layers: 130 * 2^-24 a layer, on the largest gradient
         assert float((p.to(F64) - q).abs().max()) <= 3 * 130 * 2.0 ** -24 * float(q.abs().max())
+
+
+@pytest.mark.parametrize("rows", [40, 700, 5000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_bounds_that_decrease_stay_inside(rows, dtype):
+    """Not a call that means anything, but one that reads and writes its tensors and nothing around them."""
+    k, n = 128, 96
+    x, w, _, _, dy = _inputs(rows, k, n, None, dtype, groups=6)
+    room = torch.full((rows + 64, n), 5.0, dtype=dtype, device=DEV)
+    off = torch.tensor([2, rows - 9, 3, rows + 70, -5, rows // 2, 4], device=DEV)
+    grouped_linear(x, w, off, None, "silu", out=room[32:-32])
+    assert bool((room[:32] == 5).all()) and bool((room[-32:] == 5).all())
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    for t in torch.autograd.grad(grouped_linear(x, w, off, None, "silu"), leaves, dy):
+        assert t.shape in (x.shape, w.shape)
+    torch.cuda.synchronize()
+    _check_grouped(x.detach(), w.detach(), torch.tensor([0, 1, 9, 9, 20, 30, rows], device=DEV), None, None, "silu", dy)
+
+
+@pytest.mark.parametrize("rows", [3, 70, 400])
+def test_weight_beyond_2_gib(rows):
+    """A vocabulary-sized projection: 2.6 GB of weights, forward and gradients, at both of its ends."""
+    k, n = 1296, 1_000_008
+    x = _randn(_gen(rows), rows, k, dtype=BF16).requires_grad_()
+    w = torch.empty(n, k, dtype=BF16, device=DEV).normal_(0, k ** -0.5, generator=_gen(2)).requires_grad_()
+    dy = torch.zeros(rows, n, dtype=BF16, device=DEV)
+    y = fused_linear(x, w)
+    ends = torch.cat([torch.arange(200, device=DEV), torch.arange(n - 200, n, device=DEV)])
+    dy[:, ends] = _randn(_gen(3), rows, 400, dtype=BF16)
+    ref = product(x.detach(), w.detach()[ends], None, None, None, BF16, dy[:, ends])
+    check(y.detach()[:, ends], *ref["y"], what="y")
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    check(dx, *ref["dx"], what="dx")  # (the other columns add zeros)
+    check(dw[ends], *ref["dw"], what="dw")
+    assert not bool(dw[200:-200].any())
+
+
+def test_two_streams_at_once():
+    """Calls of the same leaves that overlap, with scratch memory and without."""
+    x, w, b, r, dy = _inputs(900, 1023, 257, "gelu", BF16, groups=3)
+    off = torch.tensor([0, 100, 500, 900], device=DEV)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+
+    def step():
+        y = grouped_linear(x, w, off, b, "gelu", r)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step())
+    torch.cuda.synchronize()
+    for one in got:
+        assert all(torch.equal(p, q) for p, q in zip(one, want))
