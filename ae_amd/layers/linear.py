@@ -247,11 +247,45 @@ def _run(x, weight, bias, activation, residual, offsets, slots, out):
             raise ValueError("weights reached through weight_slots have no gradient: several groups may share a "
                              "slot. Pass them detached, or index the weights first")
         return _Product.apply(x, weight, bias, residual, offsets, slots, sizes, strides)
-    if out is not None and not out.is_contiguous():
+    if out is not None:
+        _check_out(out, residual, (x, weight, bias, offsets, slots))
+        torch.autograd.graph.increment_version(out)  # a backward pass that has saved its old values says so
+    return _forward(sizes, strides, x, weight, bias, residual, offsets, slots, out, False)[0]
+
+
+def _check_out(out, residual, others):
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out= takes no part in differentiation: it may not require a gradient")
+    if not out.is_contiguous():
         if out.dim() != 2 or (out.shape[1] > 1 and out.stride(1) != 1) or (
                 out.shape[0] > 1 and out.stride(0) < out.shape[1]):
             raise ValueError(f"out rows must be apart, with adjacent elements: strides {out.stride()}")
-    return _forward(sizes, strides, x, weight, bias, residual, offsets, slots, out, False)[0]
+    if residual is not None and (residual.data_ptr() != out.data_ptr() or residual.stride() != out.stride()):
+        others = (*others, residual)
+    if any(t is not None and _overlap(out, t) for t in others):
+        raise ValueError("out may be the residual, but not overlap other operands")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The first byte of t's elements, and the byte behind the last."""
+    first = t.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _overlap(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether they share bytes. Of columns of one matrix (rows of the same pitch) only the columns count."""
+    if out.numel() == 0 or t.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(out), _span(t)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    if out.dim() != 2 or t.dim() != 2 or out.dtype != t.dtype or out.stride(0) != t.stride(0) or t.stride(1) != 1:
+        return True
+    pitch, es = out.stride(0), out.element_size()
+    if pitch < out.shape[1] or pitch < t.shape[1] or (b0 - a0) % es:
+        return True
+    d = (b0 - a0) // es % pitch  # t's first column, from out's
+    return d < out.shape[1] or d + t.shape[1] > pitch
 
 
 def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -263,8 +297,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     residual ``[..., N]``; all of one type (fp32, fp16, bf16), summed in fp32, the result rounded
     once. ``activation``: None, "relu", "gelu" (erf), "gelu_tanh", "silu", or "swiglu", whose
     weight holds N gate rows and N up rows: ``silu(gate) * up``. Otherwise N = Nw. ``out`` receives
-    the result where no gradient is recorded; it may be the residual. Differentiable once in x, weight,
-    bias and residual."""
+    the result where no gradient is recorded; it may be the residual, but not overlap another
+    operand. Differentiable once in x, weight, bias and residual."""
     return _run(x, weight, bias, activation, residual, None, None, out)
 
 

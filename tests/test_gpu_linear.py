@@ -578,3 +578,31 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for one in got:
         assert all(torch.equal(p, q) for p, q in zip(one, want))
+
+
+def test_out_counts_as_a_change():
+    x, w, _, _, _ = _inputs(8, 16, 24, None, F32)
+    y = fused_linear(x, w)
+    scale = torch.ones_like(y, requires_grad=True)
+    loss = (y * scale).sum()  # saves y
+    fused_linear(x + 1, w, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(ValueError, match="out="):
+        fused_linear(x, w, out=torch.empty_like(y, requires_grad=True))
+    with torch.inference_mode():
+        z = torch.empty_like(y)
+        assert torch.equal(fused_linear(x + 1, w, out=z), y)
+
+
+def test_out_over_operands_is_refused():
+    buf = _randn(_gen(1), 40, 96, dtype=BF16)
+    w, sq = _randn(_gen(2), 32, 32, dtype=BF16), _randn(_gen(3), 64, 64, dtype=BF16)
+    x = buf[:, :32]
+    want = fused_linear(x, w)
+    assert torch.equal(fused_linear(x, w, out=buf[:, 64:]), want)  # other columns of the same rows
+    assert torch.equal(fused_linear(x, w, out=buf[:, 32:64]), want)
+    for x, w, out, res in ((x, w, x, None), (x, w, buf[:, 16:48], None), (buf[:-1, 64:], w, buf[1:, 40:72], None),
+                           (sq, sq, sq, None), (sq[:32, :32], w, w, None), (buf[:, 64:], w, buf[:, :32], buf[:, 8:40])):
+        with pytest.raises(ValueError, match="overlap"):
+            fused_linear(x, w, None, None, res, out=out)
