@@ -205,7 +205,9 @@ struct ProductPlan {
 // choices (us): 32 rows, 4096 -> 4096, 16 x 32 rows 11.4, 32 x 128 copied 33; 128 rows 28 and 64 x 64 rows 23; 512 rows
 // 64 x 64 rows 38.5, 64 x 128 copied 36; 2048 rows 128 x 128 73, wide 97; 4096 rows 129 and 117. 64 x 64 copied against
 // the tile without it: weight gradients of 1000 rows, 1024 -> 1024 in bf16, 8.4 and 14.2, of 777 rows, 1024 -> 2816 in
-// fp32 48 and 63, forward 200 rows, 2048 -> 6000 16.5 and 21.1, but of 4096 rows, 2048 -> 5632 165 and 100.
+// fp32 48 and 63, forward 200 rows, 2048 -> 6000 16.5 and 21.1, but of 4096 rows, 2048 -> 5632 165 and 100. Wide
+// against 128 x 128 at 176 to 192 wide tiles, a part of the CUs: input gradient of 3000 rows, 4096 -> 14336 290 and 354, of
+// 6000 rows, 2048 -> 5632 124 and 145; at 128 tiles (2000 rows, 4096 -> 4096) 86 and 71.
 struct TileCost {
   TileShape t;
   float end, first, each;
@@ -218,8 +220,8 @@ constexpr TileCost kTileCosts[] = {
     {{32, 32, Tile::kRows}, 0.8f, 0.065f, 0.085f, 0.17f, 0.f},  {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
     {{64, 64, Tile::kCopied}, 1.0f, 0.10f, 0.20f, 0.50f, 1.2f},
     {{32, 128, Tile::kCopied}, 0.7f, 0.20f, 0.22f, 0.52f, 0.f}, {{64, 128, Tile::kCopied}, 1.0f, 0.20f, 0.30f, 1.0f, 0.f},
-    {{128, 128, Tile::kCopied}, 3.5f, 0.20f, 0.43f, 1.95f, 4.5f}, {{128, 128, Tile::kShallow}, 1.4f, 0.2f, 0.55f, 2.3f, 1.4f},
-    {{256, 256, Tile::kWide}, 10.f, 0.0f, 1.57f, 0.f, 16.f},
+    {{128, 128, Tile::kCopied}, 3.0f, 0.20f, 0.43f, 1.95f, 4.5f}, {{128, 128, Tile::kShallow}, 1.4f, 0.2f, 0.55f, 2.3f, 1.4f},
+    {{256, 256, Tile::kWide}, 10.f, 0.0f, 1.54f, 0.f, 16.f},
     // any alignment
     {{16, 32, Tile::kRowsStaged}, 0.5f, 0.10f, 0.12f, 0.13f, 0.f}, {{32, 32, Tile::kRowsStaged}, 0.5f, 0.10f, 0.20f, 0.20f, 0.f},
     {{64, 64, Tile::kStaged}, 1.5f, 0.18f, 0.33f, 0.9f, 1.5f},
@@ -253,9 +255,14 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
     // (splits: not of rows tiles, whose waves split the contraction already, and of groups along it only of a single one)
     const bool may_split = !by_rows && t.form != Tile::kShallow && !(depth_groups && groups > 1);
     for (int splits = 1; splits <= 16 && (splits == 1 || (may_split && splits * 4 <= steps)); splits *= 2) {
-      double n = std::max(1.0, tiles * splits / kCUs);
-      if (!by_rows || t.bm == 64) n = std::ceil(n);  // (of the small tiles several run on a CU at once)
-      double time = 2.5 + end * n + steps / splits * (c.first + each * n);
+      // workgroups per CU: of the small tiles and of 128 x 128 in 16 bits several run on a CU at once
+      const double share = tiles * splits / kCUs;
+      double n = std::max(1.0, share);
+      if (!by_rows || t.bm == 64) n = t.bm == 128 && dtype != kF32 ? std::ceil(2 * n) / 2 : std::ceil(n);
+      // a last round of wide tiles on a part of the CUs leaves them more of the power and of the L2s
+      const double last = share - std::floor(share);
+      const double work = t.form == Tile::kWide && last > 0 ? std::floor(share) + 0.65 + 0.35 * last * last : n;
+      double time = 2.5 + end * n + steps / splits * (c.first + each * work);
       if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch; partial sums out and in
       if (p.time != 0 && time >= p.time) continue;
       p.time = time;
