@@ -186,6 +186,7 @@ constexpr int64_t kL2Bytes = int64_t{32} << 20;
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 bool aligned(const void* p, int64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+bool whole_lines(const void* base, int64_t pitch) { return aligned(base, 128) && pitch % 128 == 0; }
 bool valid_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
 
 enum Kind { kForward, kInputGrad, kWeightGrad };
@@ -292,10 +293,13 @@ int run_product(Kind kind, int dtype, const ProductPlan& plan, ProductArgs& a, b
   a.split_steps = plan.split_steps;
   // Results that the L2s (8 of 4 MB) cannot hold are stored past them, where they would only displace the operands that
   // the tiles share: 8192 x 4096 -> 14336 with gelu_tanh 844 -> 782 us, 12282 rows in 64 groups 2048 -> 2 x 1408 with
-  // its pre-activations 281 -> 272. Smaller ones stay for the next operator to read.
+  // its pre-activations 281 -> 272. Smaller ones stay for the next operator to read, and so do those whose rows are no
+  // whole 128-byte lines, which would go to memory in parts: weight gradients of 4 groups of 48 rows, 5208 -> 9184 254 past
+  // the caches and 129 through them, 2000 rows, 64 -> 20008 with pre-activations 126 and 48.
   const int64_t result = (a.out_group != 0 ? a.groups : 1) * static_cast<int64_t>(a.rows) *
                          (a.out_cols * int64_t{dtype_bytes(dtype)} + (a.z != nullptr ? a.cols * int64_t{4} : 0));
-  a.stream = result > kL2Bytes;
+  a.stream = result > kL2Bytes && whole_lines(a.out, a.out_ld * dtype_bytes(dtype)) &&
+             (a.z == nullptr || whole_lines(a.z, a.z_ld * int64_t{4}));
   a.item_blocks = static_cast<int>(items);
   a.fill_blocks = plan.splits > 1 ? 0 : fills;
   const bool ps = kind != kForward, qs = kind == kWeightGrad;
