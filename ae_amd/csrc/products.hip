@@ -208,17 +208,22 @@ struct ProductPlan {
 // the tile without it: weight gradients of 1000 rows, 1024 -> 1024 in bf16, 8.4 and 14.2, of 777 rows, 1024 -> 2816 in
 // fp32 48 and 63, forward 200 rows, 2048 -> 6000 16.5 and 21.1, but of 4096 rows, 2048 -> 5632 165 and 100. Wide
 // against 128 x 128 at 176 to 192 wide tiles, a part of the CUs: input gradient of 3000 rows, 4096 -> 14336 290 and 354, of
-// 6000 rows, 2048 -> 5632 124 and 145; at 128 tiles (2000 rows, 4096 -> 4096) 86 and 71.
+// 6000 rows, 2048 -> 5632 124 and 145; at 128 tiles (2000 rows, 4096 -> 4096) 86 and 71. Rows tiles on a part of the CUs
+// against the tile that their times on all of them would choose: 3 rows, 5424 -> 1376 6.7 and 11.7 (splits of 32 x 128),
+// 92 rows, 3792 -> 392 in fp32 11.1 and 15.5.
 struct TileCost {
   TileShape t;
   float end, first, each;
   float each32;    // fp32 (of the same bytes: half the elements, at a 16th of the matrix rate); 0: not for fp32
   float depth_end; // end of a product grouped along its contraction; 0: not for them
+  float few = 0, few32 = 0;  // a step of at most a workgroup per CU, where it is its reads' latency (both types)
 };
 using Tile = TileShape;
 constexpr TileCost kTileCosts[] = {
-    {{16, 16, Tile::kRows}, 0.3f, 0.085f, 0.052f, 0.06f, 0.f},  {{16, 32, Tile::kRows}, 0.5f, 0.06f, 0.08f, 0.10f, 0.f},
-    {{32, 32, Tile::kRows}, 0.8f, 0.065f, 0.085f, 0.17f, 0.f},  {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
+    {{16, 16, Tile::kRows}, 0.3f, 0.085f, 0.052f, 0.06f, 0.f, 0.05f, 0.072f},
+    {{16, 32, Tile::kRows}, 0.5f, 0.06f, 0.08f, 0.092f, 0.f, 0.075f, 0.095f},
+    {{32, 32, Tile::kRows}, 0.8f, 0.065f, 0.085f, 0.17f, 0.f, 0.088f, 0.16f},
+    {{64, 64, Tile::kRows}, 2.0f, 0.03f, 0.24f, 0.68f, 0.f},
     {{64, 64, Tile::kCopied}, 1.0f, 0.10f, 0.20f, 0.50f, 1.2f},
     {{32, 128, Tile::kCopied}, 0.7f, 0.20f, 0.22f, 0.52f, 0.f}, {{64, 128, Tile::kCopied}, 1.0f, 0.20f, 0.30f, 1.0f, 0.f},
     {{128, 128, Tile::kCopied}, 3.0f, 0.20f, 0.43f, 1.95f, 4.5f}, {{128, 128, Tile::kShallow}, 1.4f, 0.2f, 0.55f, 2.3f, 1.4f},
@@ -263,7 +268,13 @@ ProductPlan plan_product(Kind kind, int dtype, int64_t rows, int64_t cols, int64
       // a last round of wide tiles on a part of the CUs leaves them more of the power and of the L2s
       const double last = share - std::floor(share);
       const double work = t.form == Tile::kWide && last > 0 ? std::floor(share) + 0.65 + 0.35 * last * last : n;
-      double time = 2.5 + end * n + steps / splits * (c.first + each * work);
+      double step = c.first + each * work;
+      if (c.few != 0) {
+        if (share <= 1) step = dtype == kF32 ? c.few32 : c.few;
+        else if (dtype == kF32) step = c.first + each * std::ceil(share);  // bound by the matrix rate
+        else if (share < 2) step = c.few + (share - 1) * (c.first + 2 * each - c.few);
+      }
+      double time = 2.5 + end * n + steps / splits * step;
       if (splits > 1) time += 5.0 + 8.0 * splits * rows * cols / 4e6;  // the joining launch; partial sums out and in
       if (p.time != 0 && time >= p.time) continue;
       p.time = time;
