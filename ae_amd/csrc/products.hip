@@ -327,6 +327,9 @@ int run_product(Kind kind, int dtype, const ProductPlan& plan, ProductArgs& a, b
   if (err != hipSuccess || plan.splits == 1) return static_cast<int>(err);
   const int splits = a.splits;
   a.splits = 1;
+  // Groups along the contraction (a single one where it is split): its bounds are of the operands' rows, and the partial
+  // sums cover every row of the result.
+  if (depth_groups) a.offsets = nullptr;
   const int64_t joins = max_row_tiles(a.rows, a.groups, kJoinRows) * cdiv(a.out_cols, kGradCols);
   if (joins + fills > INT32_MAX) return SMX_ERR_UNSUPPORTED;
   a.item_blocks = static_cast<int>(joins);

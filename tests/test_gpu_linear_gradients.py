@@ -1,0 +1,78 @@
+"""Gradients of the matrix products where a call's form is at its edges: a single group whose weight gradient is
+split along the contraction, into results that hold NaN before the call. Against 64 bits within the bounds of
+tests/product_ref.py."""
+import pytest
+import torch
+
+from ae_amd import _lib
+from tests.product_ref import check, product
+from tests.test_gpu_linear import BF16, DEV, F16, F32, _check_grouped, _inputs
+
+pytestmark = pytest.mark.gpu
+CODES = {F32: _lib.SMX_F32, F16: _lib.SMX_F16, BF16: _lib.SMX_BF16}
+
+
+class Room:
+    """A contiguous tensor of `fill` (its bytes, for scratch memory) with a margin of a known pattern on both sides."""
+
+    MARGIN = 4096
+
+    def __init__(self, shape, dtype, fill=float("nan")):
+        n = torch.Size(shape).numel()
+        self.mark = 0xA5 if dtype == torch.uint8 else 5.0
+        self.all = torch.full((n + 2 * self.MARGIN,), self.mark, dtype=dtype, device=DEV)
+        self.t = self.all[self.MARGIN:self.MARGIN + n].view(shape)
+        self.t.fill_(fill)
+
+    def margins_whole(self):
+        m = self.MARGIN
+        return bool((self.all[:m] == self.mark).all()) and bool((self.all[-m:] == self.mark).all())
+
+
+def _grad_into(dy, z, x, w, off, act):
+    """The C gradient call of a grouped product (contiguous operands, a weight per group) into tensors of NaN; their
+    margins and the workspace's stay as they were."""
+    (rows, k), (groups, nw, _), n = x.shape, w.shape, dy.shape[1]
+    code, a = CODES[x.dtype], _lib.ACTIVATIONS[act]
+    nbytes = _lib.lib().smx_linear_grad_workspace_size(rows, k, n, groups, a, code)
+    dx, dw, db = Room((rows, k), x.dtype), Room((groups, nw, k), x.dtype), Room((groups, nw), x.dtype)
+    ws = Room((nbytes,), torch.uint8, 0xFF)
+    _lib.call("smx_grouped_linear_grad", dy.data_ptr(), n, None if z is None else z.data_ptr(), x.data_ptr(), k, code,
+              rows, k, w.data_ptr(), k, nw * k, groups, n, a, off.data_ptr(), groups, None, dx.t.data_ptr(),
+              dw.t.data_ptr(), db.t.data_ptr(), ws.t.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert all(r.margins_whole() for r in (dx, dw, db, ws))
+    return dx.t, dw.t, db.t
+
+
+# More rows than columns by far: the plan splits the weight gradient 2 to 8 ways. fp32 and 16-bit types; rows of whole
+# 16-byte slots and odd ones; fewer rows than weight rows, and more.
+ONE_GROUP = [(900, 64, 1024, F32), (640, 64, 2816, F32), (1000, 128, 2048, F32), (900, 61, 1001, F32),
+             (2000, 256, 256, BF16), (2300, 64, 2816, BF16), (1500, 99, 2048, BF16), (5000, 333, 1000, BF16),
+             (8192, 256, 2048, BF16), (2000, 64, 2048, F16), (16000, 1000, 4096, F16)]
+BOUNDS = {"all": lambda r: (0, r), "inside": lambda r: (37, r - 37), "few": lambda r: (7, 50), "empty": lambda r: (9, 9),
+          "late": lambda r: (r - 20, r), "clamped": lambda r: (-4, r + 100)}
+
+
+@pytest.mark.parametrize("bounds", BOUNDS)
+@pytest.mark.parametrize("rows,k,n,dtype", ONE_GROUP)
+def test_weight_gradient_of_one_group(rows, k, n, dtype, bounds):
+    """Every row of the weight's gradient, whatever rows of x the group has."""
+    lo, hi = BOUNDS[bounds](rows)
+    x, w, _, _, dy = _inputs(rows, k, n, None, dtype, groups=1, bias=False, residual=False)
+    off = torch.tensor([lo, hi], device=DEV)
+    dx, dw, db = _grad_into(dy, None, x, w, off, None)
+    lo, hi = max(lo, 0), min(hi, rows)
+    ref = product(x[lo:hi], w[0], None, None, None, dtype, dy[lo:hi])
+    check(dw[0], *ref["dw"], what="dw")
+    check(db[0], *ref["db"], what="db")
+    check(dx[lo:hi], *ref["dx"], what="dx")
+    assert not bool(dx[:lo].any()) and not bool(dx[hi:].any())
+
+
+@pytest.mark.parametrize("rows,k,n,dtype,act", [(900, 64, 1024, F32, "gelu"), (2000, 256, 256, BF16, "silu"),
+                                                (1500, 99, 1024, BF16, "swiglu")])
+def test_training_of_one_group(rows, k, n, dtype, act):
+    """The same through grouped_linear: an expert-parallel rank with one local expert and a padded batch."""
+    x, w, b, r, dy = _inputs(rows, k, n, act, dtype, groups=1)
+    _check_grouped(x, w, torch.tensor([5, rows - 300], device=DEV), b, r, act, dy, what=act)
