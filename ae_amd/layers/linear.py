@@ -2,8 +2,8 @@
 
 ``fused_linear`` is ``residual + act(x W^T + b)``; ``grouped_linear`` is the same with a weight
 and a bias per group of consecutive rows, as rows sorted by expert have them
-(``moe_align_block_size(topk_ids, 1, E)`` gives that order). Both are differentiable in x, weight,
-bias and residual. They cover what the fused SwiGLU page of ``stack_fused_moe`` does not: experts
+(``moe_align_block_size(topk_ids, 1, E)`` gives that order). Both are differentiable (reverse mode) in x,
+weight, bias and residual. They cover what the fused SwiGLU page of ``stack_fused_moe`` does not: experts
 with biases or another activation, experts that are trained, dense MLPs and projections. The
 reference has no counterpart: it leaves such products to torch.
 
@@ -18,6 +18,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ._torch import dtype_code, workspace
@@ -229,6 +230,7 @@ class _Once(torch.autograd.Function):
 
 
 def _gradients(ctx, dy):
+    _no_tangents(dy)
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     grads = (None, None, None)
     if need_x or need_w or need_b:
@@ -236,7 +238,15 @@ def _gradients(ctx, dy):
     return (*grads, dy if need_r else None, None, None, None, None)
 
 
+def _no_tangents(*tensors) -> None:
+    """Refuses forward-mode duals, whose tangents the kernels would drop."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("fused_linear and grouped_linear have no forward-mode derivative")
+
+
 def _run(x, weight, bias, activation, residual, offsets, slots, out):
+    _no_tangents(x, weight, bias, residual, out)
     sizes, strides = _check(x, weight, bias, activation, residual, offsets, slots, out)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad) or
@@ -298,7 +308,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     once. ``activation``: None, "relu", "gelu" (erf), "gelu_tanh", "silu", or "swiglu", whose
     weight holds N gate rows and N up rows: ``silu(gate) * up``. Otherwise N = Nw. ``out`` receives
     the result where no gradient is recorded; it may be the residual, but not overlap another
-    operand. Differentiable once in x, weight, bias and residual."""
+    operand. Differentiable once, in reverse mode, in x, weight, bias and residual."""
     return _run(x, weight, bias, activation, residual, None, None, out)
 
 

@@ -3,8 +3,10 @@ split along the contraction, into results that hold NaN before the call. Against
 tests/product_ref.py."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ae_amd import _lib
+from ae_amd.layers import fused_linear, grouped_linear
 from tests.product_ref import check, product
 from tests.test_gpu_linear import BF16, DEV, F16, F32, _check_grouped, _inputs
 
@@ -76,3 +78,18 @@ def test_training_of_one_group(rows, k, n, dtype, act):
     """The same through grouped_linear: an expert-parallel rank with one local expert and a padded batch."""
     x, w, b, r, dy = _inputs(rows, k, n, act, dtype, groups=1)
     _check_grouped(x, w, torch.tensor([5, rows - 300], device=DEV), b, r, act, dy, what=act)
+
+
+def test_forward_mode_refused():
+    """Tangents of the operands, and of the gradient that comes in, would be dropped."""
+    x, w, _, _, dy = _inputs(8, 16, 24, "silu", F32)
+    off = torch.tensor([0, 8], device=DEV)
+    y = fused_linear(x.requires_grad_(), w, None, "silu")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        for call in (lambda: fused_linear(dual, w), lambda: grouped_linear(dual, w[None], off)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, [x], forward_ad.make_dual(dy, torch.ones_like(dy)))
+        fused_linear(x.detach(), w)  # no duals

@@ -6,6 +6,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from ae_amd import _lib
 from ae_amd.layers import fused_linear, grouped_linear
@@ -193,3 +194,20 @@ def test_python_checks_refuse():
     with pytest.raises(TypeError, match="group_offsets"):
         grouped_linear(x, w3, None)
 
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual", "out"])
+def test_forward_mode_refused(which):
+    """A dual tensor's tangent would be dropped: the call says so, before anything else."""
+    t = {"x": _cpu(4, 8), "weight": _cpu(6, 8), "bias": _cpu(6), "residual": _cpu(4, 6), "out": _cpu(4, 6)}
+    g = {"x": t["x"], "weight": _cpu(2, 6, 8), "bias": _cpu(2, 6), "residual": t["residual"], "out": t["out"]}
+    with forward_ad.dual_level():
+        for call, args in ((fused_linear, t), (grouped_linear, {**g, "group_offsets": torch.tensor([0, 2, 4])})):
+            dual = {**args, which: forward_ad.make_dual(args[which], torch.ones_like(args[which]))}
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(**dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call(**dual)
+            with pytest.raises(ValueError, match="GPU"):  # within a level, but no duals: the next check
+                call(**args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda v: fused_linear(**{**t, which: v}), (t[which],), (t[which],))
