@@ -290,11 +290,11 @@ __device__ __forceinline__ void activate_all(int act, f32x4 (&v)[N]) {
   }
 }
 
-// d act / dz. The slope terms vanish faster than any power of z grows: 0 where they underflow, also at infinity.
+// d act / dz of a smooth activation. The slope terms vanish faster than any power of z grows: 0 where they underflow, also
+// at infinity.
 template <bool EXACT>
 __device__ __forceinline__ float activate_grad(int act, float z) {
   switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
     case kActGelu: {
       const float e = bell_f32<EXACT>(z), c = normal_cdf<EXACT>(z, e);
       return e == 0.0f ? c : fmaf(z, 0.398942280f * e, c);
@@ -311,14 +311,18 @@ __device__ __forceinline__ float activate_grad(int act, float z) {
   }
 }
 
-// d *= d act / dz of N groups of four.
+// d times d act / dz, of N groups of four.
 template <bool EXACT, int N>
 __device__ __forceinline__ void activate_grad_all(int act, const f32x4 (&z)[N], f32x4 (&d)[N]) {
   auto each = [&](auto code) {
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d[n][e] *= activate_grad<EXACT>(decltype(code)::value, z[n][e]);
+      for (int e = 0; e < 4; ++e) {
+        // relu selects: a closed one passes nothing on, infinities and NaN neither
+        if constexpr (decltype(code)::value == kActRelu) d[n][e] = z[n][e] > 0.0f ? d[n][e] : (z[n][e] != z[n][e] ? z[n][e] : 0.0f);
+        else d[n][e] *= activate_grad<EXACT>(decltype(code)::value, z[n][e]);
+      }
   };
   switch (act) {
     case kActRelu: each(std::integral_constant<int, kActRelu>{}); break;

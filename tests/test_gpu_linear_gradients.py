@@ -93,3 +93,32 @@ def test_forward_mode_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, [x], forward_ad.make_dual(dy, torch.ones_like(dy)))
         fused_linear(x.detach(), w)  # no duals
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_closed_relu_passes_nothing_on(grouped, dtype):
+    """Where z is negative or zero the gradient is zero whatever comes in, infinities and NaN too; elsewhere they
+    pass."""
+    x, w, b, _, dy = _inputs(40, 64, 48, "relu", dtype, residual=False)
+    w[:8] = 0
+    b[:4], b[4:8] = -2, 0
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    off = torch.tensor([0, 40], device=DEV)
+
+    def grads(dy):
+        y = grouped_linear(x, w[None], off, b[None], "relu") if grouped else fused_linear(x, w, b, "relu")
+        return torch.autograd.grad(y, leaves, dy)
+
+    bad = torch.tensor([float("inf"), float("nan"), float("-inf"), 1.0] * 2, device=DEV, dtype=dtype)
+    dy[:, :8] = 0
+    want = grads(dy)
+    dy[3, :8] = bad
+    for p, q in zip(grads(dy), want):
+        assert bool(torch.isfinite(p).all()) and torch.equal(p, q)
+    with torch.no_grad():
+        b[8] = 60.0  # (far beyond any product here)
+    dy[3, 8] = float("inf")
+    dx, dw, db = grads(dy)
+    assert not bool(torch.isfinite(dx[3]).any()) and not bool(torch.isfinite(dw[8]).any()) and not bool(torch.isfinite(db[8]))
+    assert bool(torch.isfinite(dx[4:]).all()) and bool(torch.isfinite(dw[9:]).all()) and bool(torch.isfinite(db[9:]).all())
