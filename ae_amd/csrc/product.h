@@ -93,8 +93,8 @@ __device__ __forceinline__ int64_t group_weight(const ProductArgs& a, int g) {
   return s >= 0 && s < a.weights ? s : -1;
 }
 
-// fp32 sums run in chains of kFold steps (256 products), whose results are added up: a single chain of thousands of
-// products would lose a bit or two more than blocked sums do.
+// fp32 sums run in chains of kFold steps (256 products; 288 where three stages are walked), whose results are added up: a
+// single chain of thousands of products would lose a bit or two more than blocked sums do.
 constexpr int kFold = 8;
 template <int NI, int NJ>
 __device__ __forceinline__ void fold(f32x4 (&total)[NI][NJ], f32x4 (&acc)[NI][NJ]) {

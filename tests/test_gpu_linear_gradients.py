@@ -122,3 +122,47 @@ def test_closed_relu_passes_nothing_on(grouped, dtype):
     dx, dw, db = grads(dy)
     assert not bool(torch.isfinite(dx[3]).any()) and not bool(torch.isfinite(dw[8]).any()) and not bool(torch.isfinite(db[8]))
     assert bool(torch.isfinite(dx[4:]).all()) and bool(torch.isfinite(dw[9:]).all()) and bool(torch.isfinite(db[9:]).all())
+
+
+# Products of 1 and 1 + 2^-15: every sum of up to 288 of them is exact in fp32 (a multiple of 2^-15 below 512), while one
+# chain of n loses the low bits of whatever it adds once it has passed 4096 (steps of 2^-11): at least 2^-13 of every four
+# products, 0.24 in all at n = 12000. Sums of chains of 256 to 288 of them round by at most 2^-11 (half a step below 16384)
+# per chain, and per split or wave of the walk, of which there are at most 20.
+TERM = 1 + 2.0 ** -15
+
+
+def _check_chains(got, n):
+    assert 8000 < n < 16000
+    off = float((got.to(torch.float64) - n * TERM).abs().max())
+    assert off <= (n / 256 + 20) * 2.0 ** -11, (off, n)
+
+
+# one group has nearly all rows: groups of few rows by their mean (aligned and not), of more, and a single one
+@pytest.mark.parametrize("rows,k,n,groups", [(12800, 256, 256, 64), (12100, 512, 640, 64), (12100, 511, 640, 64),
+                                             (12100, 257, 512, 64), (12000, 256, 256, 16), (12000, 128, 256, 1)])
+def test_long_fp32_weight_gradients_run_in_chains(rows, k, n, groups):
+    x = torch.ones(rows, k, device=DEV)
+    w = torch.zeros(groups, n, k, device=DEV)
+    dy = torch.full((rows, n), TERM, device=DEV)
+    hot = groups // 3
+    off = torch.tensor([g if g <= hot else rows - groups + g for g in range(groups + 1)], device=DEV)
+    _, dw, _ = _grad_into(dy, None, x, w, off, None)
+    _check_chains(dw[hot], rows - groups + 1)
+    assert all(bool((dw[g] == TERM).all()) for g in range(groups) if g != hot)
+
+
+@pytest.mark.parametrize("rows,k,n", [(3, 12000, 2048), (3, 12001, 2048), (40, 12000, 1024), (3, 12000, 64), (300, 12001, 65)])
+def test_long_fp32_products_run_in_chains(rows, k, n):
+    y = fused_linear(torch.ones(rows, k, device=DEV), torch.full((n, k), TERM, device=DEV))
+    _check_chains(y, k)
+
+
+def test_long_fp32_groups_of_random_values():
+    """The same tiles walked over groups of many and of few rows in turn, into results of whole slots and odd ones."""
+    for k, n, many in ((264, 200, 32), (511, 640, 56)):
+        cut = [0, 3, 3, 4000, 4031, 4032, 5000] + [5000 + 8 * i for i in range(many)] + [8990, 9000]
+        x, w, _, _, dy = _inputs(9000, k, n, None, F32, groups=len(cut) - 1, bias=False, residual=False)
+        off = torch.tensor(cut, device=DEV)
+        _, dw, _ = _grad_into(dy, None, x, w, off, None)
+        for g, (lo, hi) in enumerate(zip(cut, cut[1:])):
+            check(dw[g], *product(x[lo:hi], w[g], None, None, None, F32, dy[lo:hi])["dw"], what=f"{k} x {n}, group {g}")
