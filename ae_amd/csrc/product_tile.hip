@@ -510,30 +510,48 @@ __global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductAr
     f32x4 acc[W::kNI][W::kNJ] = {};
     // fp32 chains (see fold): four workgroups per CU leave no registers for a second set of sums, so those of a group of
     // more than one chain wait in the result's own place: `more`: on top of what is there; `leave`: left there. A single
-    // group of 12737 rows then takes 1122 us where one chain took 946 (64 groups, 256 x 256), 16384 rows in groups of 512
-    // (512 x 1024) 145 and 144, groups of at most 256 rows the same.
-    auto fold_out = [&](bool more, bool leave) {
+    // group of 12737 rows (of 64, 256 x 256) then takes 1083 us where one chain took 953, 16384 rows in groups of 512
+    // (512 x 1024) 146 and 145; groups of at most 256 rows have no such chain.
+    auto fold_out = [&](bool more, auto leave) {
       int ln = lane;
       asm volatile("" : "+v"(ln));
       char* base = a.out + (it.g * a.out_group + it.row * a.out_ld) * kEs;
+      const auto from = make_rsrc(base, more ? kPOutside : 0u);  // (an empty buffer: zeros)
+      const auto to = make_rsrc(base, kPOutside);
 #pragma unroll
       for (int j = 0; j < W::kNJ; ++j) {
         const int row = wrow + j * 16 + (ln & 15);
-        if (row >= it.m) continue;
+        const int64_t at = row * a.out_ld + it.ct * kTile + wcol + 4 * (ln >> 4);
+        const int left = row < it.m ? a.out_cols - (it.ct * kTile + wcol + 4 * (ln >> 4)) : 0;
+        if constexpr (SLOTS) {
+          uint32_t off[W::kNI];
+          f32x4 sum[W::kNI];
 #pragma unroll
-        for (int i = 0; i < W::kNI; ++i) {
-          const int col = it.ct * kTile + wcol + i * 16 + 4 * (ln >> 4), left = a.out_cols - col;
-          if (left <= 0) continue;
-          const int64_t at = row * a.out_ld + col;
-          if (more) acc[i][j] = load4<DT>(base, at, left, SLOTS) + acc[i][j];
-          if (leave) store4<DT>(base, at, left, SLOTS, acc[i][j]);
+          for (int i = 0; i < W::kNI; ++i) {
+            off[i] = left > 16 * i ? static_cast<uint32_t>((at + 16 * i) * kEs) : kPOutside;
+            sum[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, off[i], 0, 0));
+          }
+#pragma unroll
+          for (int i = 0; i < W::kNI; ++i) {
+            acc[i][j] += sum[i];
+            if constexpr (decltype(leave)::value) store_slot(to, __builtin_bit_cast(u32x4, acc[i][j]), off[i], false);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < W::kNI; ++i) {
+            if (left <= 16 * i) continue;
+            if (more) acc[i][j] += load4<DT>(base, at + 16 * i, left - 16 * i, false);
+            if constexpr (decltype(leave)::value) store4<DT>(base, at + 16 * i, left - 16 * i, false, acc[i][j]);
+          }
         }
       }
-      if (!leave) return;
+      if constexpr (decltype(leave)::value) {
 #pragma unroll
-      for (int i = 0; i < W::kNI; ++i)
+        for (int i = 0; i < W::kNI; ++i)
 #pragma unroll
-        for (int j = 0; j < W::kNJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int j = 0; j < W::kNJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
     };
     for (int s = 0; s < steps; ++s) {
       if (s == 0 && stores) __builtin_amdgcn_s_waitcnt(vmcnt_imm(kStores));
@@ -554,9 +572,9 @@ __global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductAr
       }
       bare_barrier();  // every wave has read the stage
       if (s + 1 < steps) copy(it, s + 1);
-      if (DT == kF32 && s % kFold == kFold - 1 && s + 1 < steps) fold_out(s >= kFold, true);
+      if (DT == kF32 && s % kFold == kFold - 1 && s + 1 < steps) fold_out(s >= kFold, std::true_type{});
     }
-    if (DT == kF32 && steps > kFold) fold_out(true, false);
+    if (DT == kF32 && steps > kFold) fold_out(true, std::false_type{});
     const ProductItem done = it;
     const int c0 = done.ct * kTile + wcol;
     char* base = a.out + (done.g * a.out_group + done.row * a.out_ld) * kEs;
