@@ -166,3 +166,23 @@ def test_long_fp32_groups_of_random_values():
         _, dw, _ = _grad_into(dy, None, x, w, off, None)
         for g, (lo, hi) in enumerate(zip(cut, cut[1:])):
             check(dw[g], *product(x[lo:hi], w[g], None, None, None, F32, dy[lo:hi])["dw"], what=f"{k} x {n}, group {g}")
+
+
+@pytest.mark.parametrize("rows,k,n", [(40, 128, 96), (700, 128, 96), (5000, 128, 96), (5000, 131, 77)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("act", ["gelu", "swiglu"])
+def test_gradients_of_bounds_that_decrease_stay_inside(act, dtype, rows, k, n):
+    """Bounds that mean nothing name rows twice: more row tiles than rows, whose column sums and results have no place.
+    Nothing outside the results and the workspace is written (_grad_into looks), and a call that means something
+    comes out right behind it."""
+    x, w, b, _, dy = _inputs(rows, k, n, act, dtype, groups=6, residual=False)
+    z = torch.randn(rows, w.shape[1], device=DEV, generator=torch.Generator(device=DEV).manual_seed(rows))
+    for bounds in ([2, rows - 9, 3, rows + 70, -5, rows // 2, 4], [rows, 0, rows, 0, rows, 0, rows],
+                   [0, rows, 0, rows, 0, rows, 0], [2 ** 40, -2 ** 40, 2 ** 62, 0, rows, 1, 2 ** 62]):
+        off = torch.tensor(bounds, device=DEV)
+        y = Room((rows, n), dtype)
+        with torch.no_grad():
+            grouped_linear(x, w, off, b, act, out=y.t)
+        assert y.margins_whole()
+        _grad_into(dy, z, x, w, off, act)
+    _check_grouped(x, w, torch.tensor([0, 1, 9, 9, 20, 30, rows], device=DEV), b, None, act, dy)
