@@ -460,7 +460,8 @@ struct StridedCopy {
 // latencies (bounds, copies, stores) and the results' bytes bound the whole. One stage of 32 KB, so that four workgroups
 // share a CU; each walks over tiles, and sends the next tile's first copies out before it stores the last one's sums. Those
 // go out as buffer stores whose lanes outside the result are turned off by their offset: always the same number of
-// them, so that the next tile waits for its copies (older than the stores) and not for the stores. 16-bit sums pass
+// them, so that the barrier in front of the next tile waits for its copies (older than the stores) and not for the stores
+// (behind it the compiler waits for these too, before it reads what the copies brought). 16-bit sums pass
 // through the stage first, so that a store writes whole lines (8 rows of 128 bytes): halves of lines, 64 bytes of each of
 // 16 rows, cost 474 us past the caches and 423 through them where this takes 351.
 // Large results go past the caches (ProductArgs::stream): their bytes would drive the tiles' operands out of L2.
@@ -621,9 +622,9 @@ __global__ __launch_bounds__(kPThreads, 4) void product_shallow_kernel(ProductAr
 #pragma unroll
             for (int i = 0; i < W::kNI; ++i) {
               const int col = c0 + i * 16 + 4 * (ln >> 4);
-              store_slot(rs, __builtin_bit_cast(u32x4, acc[i][j]),
-                         row < done.m && col < a.out_cols ? static_cast<uint32_t>((row * a.out_ld + col) * kEs) : kPOutside,
-                         decltype(stream)::value);
+              uint32_t off = row < done.m && col < a.out_cols ? static_cast<uint32_t>((row * a.out_ld + col) * kEs) : kPOutside;
+              asm volatile("" : "+v"(off));  // (one store for both cases, not one in each: they are counted)
+              store_slot(rs, __builtin_bit_cast(u32x4, acc[i][j]), off, decltype(stream)::value);
             }
           }
         } else {
