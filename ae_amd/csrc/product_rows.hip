@@ -276,7 +276,8 @@ static hipError_t rows_launch(const TileShape& t, const ProductArgs& a, hipStrea
   // of a short walk. One row, swiglu weights, us with two and with three: 88 workgroups, bf16, 1024 columns 5.0 and 5.4, 2048
   // 6.9 and 7.1, 4096 10.5 and 10.5, 8192 17.9 and 16.7, fp32, 1024 columns 7.6 and 7.5, 4096 20.6 and 17.7, 8192 39.2 and
   // 35.1; 352 workgroups, bf16, 2048 columns 12.7 and 13.4, 4096 24.3 and 25.5, 8192 49.0 and 49.1, fp32, 2048 columns 25.2 and
-  // 27.0, 8192 91.0 and 90.9; 512 workgroups, fp32, 4096 columns 62.8 and 60.4.
+  // 27.0, 8192 91.0 and 90.9; 512 workgroups, fp32, 4096 columns 62.8 and 60.4. (Against it: 20 rows, 2048 -> 4096 in fp32 13.2
+  // and 12.4.)
   const bool long_walk = a.depth >= 16384 / dtype_bytes(DT);
   if (t.bm == 16 && t.bn == 16) product_rows_kernel<DT, 1, 1, 4><<<blocks, kPThreads, 0, s>>>(a);
   else if (t.bm == 16 && t.bn == 32 && long_walk) product_rows_kernel<DT, 2, 1, 3><<<blocks, kPThreads, 0, s>>>(a);
