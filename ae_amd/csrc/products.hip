@@ -17,7 +17,7 @@ constexpr int kJoinRows = 4;    // rows of a workgroup that joins splits, one pe
 // dz = dy * act'(z), rounded into dz (unless null), and its fp32 column sums over the workgroup's rows.
 // The rounding is that of an operand of the matrix instructions: the gradients of x and of the weight then err by that and by
 // their own, 2.35e-3 relative in bf16 (1.66e-3 if only the results were rounded; 4096 rows, 2048 -> 5632 with gelu) and 2.9e-4
-// in fp16 (2.1e-4). Carrying what the rounding leaves as a second operand would double the two products (190 of 367 us
+// in fp16 (2.1e-4). Carrying what the rounding leaves as a second operand would double the two products (205 of 367 us
 // there are theirs).
 struct ActGradArgs {
   ProductArgs p;          // groups; rows; cols = columns of z; out_cols; gated; act
