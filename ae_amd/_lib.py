@@ -1,5 +1,5 @@
-"""ctypes binding of libspecmoe_mi355x.so (the C ABI in include/specmoe_mi355x.h and
-include/specmoe_mi355x_products.h).
+"""ctypes binding of libspecmoe_mi355x.so (the C ABI in include/specmoe_mi355x.h,
+include/specmoe_mi355x_products.h and include/specmoe_mi355x_blocks.h).
 
 The library is built in-tree by ``ae_amd.build``. Loading fails loudly when it is missing:
 there is no fallback implementation of any entry point.
@@ -118,6 +118,35 @@ PRODUCT_SIGNATURES = [
                                                 _c_void_p]),
 ]
 
+# The same for include/specmoe_mi355x_blocks.h.
+_f32 = ctypes.c_float
+BLOCK_SIGNATURES = [
+    ("smx_norm", ctypes.c_int,
+     [_i32, _c_void_p, _i64, _c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _c_void_p, _i32, _f32, _c_void_p,
+      _c_void_p, _c_void_p, _c_void_p]),
+    ("smx_norm_grad_workspace_size", _sz, [_i32, _i64, _i64, _i32]),
+    ("smx_norm_grad", ctypes.c_int,
+     [_i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i32, _c_void_p,
+      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p]),
+    ("smx_route_workspace_size", _sz, [_i64, _i64, _i64]),
+    ("smx_route", ctypes.c_int,
+     [_c_void_p, _i64, _i32, _i64, _i64, _i64, _i32, _c_void_p, _i64, _i64, _i32, _f32, _c_void_p, _c_void_p,
+      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _sz, _c_void_p]),
+    ("smx_route_grad", ctypes.c_int,
+     [_c_void_p, _c_void_p, _i64, _i32, _i64, _i64, _i64, _i32, _i32, _f32, _c_void_p, _c_void_p, _c_void_p]),
+    ("smx_dispatch_rows", ctypes.c_int,
+     [_c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    ("smx_combine_rows", ctypes.c_int,
+     [_c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p]),
+    ("smx_combine_rows_grad", ctypes.c_int,
+     [_c_void_p, _i64, _c_void_p, _i64, _i32, _i64, _i64, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p,
+      _c_void_p]),
+]
+
+# enum smx_norm_kind, enum smx_scoring
+SMX_NORM_LAYER, SMX_NORM_RMS = 0, 1
+SCORINGS = {"softmax": 0, "sigmoid": 1}
+
 # enum smx_activation
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
 
@@ -151,7 +180,7 @@ def lib() -> ctypes.CDLL:
             # see torch's device context.
             import torch  # noqa: F401
             handle = ctypes.CDLL(LIB_PATH)
-            for name, restype, argtypes in SIGNATURES + PRODUCT_SIGNATURES:
+            for name, restype, argtypes in SIGNATURES + PRODUCT_SIGNATURES + BLOCK_SIGNATURES:
                 fn = getattr(handle, name)
                 fn.restype = restype
                 fn.argtypes = argtypes

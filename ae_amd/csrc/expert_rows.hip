@@ -1,0 +1,327 @@
+// Rows to the experts and back: a token's row to its picks' places, and the weighted sum of the rows at its places, with
+// gradients. Both walk over tokens, so that what belongs to a token once (its row, the gradient of its sum) is moved once.
+#include <algorithm>
+
+#include "blocks.h"
+
+namespace smx {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPicks = 16;
+constexpr int64_t kMaxCols = int64_t{1} << 24;
+
+struct MoveArgs {
+  const char* x;         // one row a token: x, or the gradient of the sum
+  const char* rows;      // the picks' rows
+  const int32_t* places;
+  const float* weights;  // null: 1
+  const char* residual;
+  int64_t x_ld, rows_ld, residual_ld;
+  int64_t T, picks;      // picks: T k
+  int H, k;
+  int shift;             // log2 of the threads of a token's columns
+  char* y;               // dense: one row a token, or the picks' rows
+  float* grad_weights;
+};
+
+// One thread's elements of a row: a 16-byte chunk, or as many elements a row of threads apart.
+template <int DT, bool kVec> struct Part {
+  static constexpr int kN = Chunk<DT>::kN;
+  using S = typename Elem<DT>::S;
+  int col, step, H;
+
+  __device__ __forceinline__ bool in(int j) const { return col + j * step < H; }
+  __device__ __forceinline__ Chunk<DT> load(const char* base, int64_t row, int64_t ld) const {
+    const S* p = reinterpret_cast<const S*>(base) + row * ld + col;
+    Chunk<DT> r;
+    if constexpr (kVec) {
+      r = __builtin_bit_cast(Chunk<DT>, *reinterpret_cast<const u32x4*>(p));
+    } else {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) r.e[j] = in(j) ? p[j * step] : S{};
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(char* base, int64_t row, const Chunk<DT>& r) const {
+    S* p = reinterpret_cast<S*>(base) + row * H + col;
+    if constexpr (kVec) {
+      *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, r);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if (in(j)) p[j * step] = r.e[j];
+    }
+  }
+};
+
+// The token and the columns of a thread; false behind the end of either.
+template <int DT, bool kVec>
+__device__ __forceinline__ bool part_of(const MoveArgs& a, int64_t& t, Part<DT, kVec>& p) {
+  constexpr int kN = Chunk<DT>::kN;
+  const int width = 1 << a.shift, lane = static_cast<int>(threadIdx.x) & (width - 1);
+  t = static_cast<int64_t>(blockIdx.x) * (kThreads >> a.shift) + (threadIdx.x >> a.shift);
+  const int first = static_cast<int>(blockIdx.y) * width * kN;
+  p.H = a.H;
+  p.col = kVec ? first + lane * kN : first + lane;
+  p.step = kVec ? 1 : width;
+  return t < a.T && p.col < a.H;
+}
+
+// y[t] = residual[t] + sum_j weights[t, j] rows[places[t, j]]. The loads of four picks are on their way at once.
+template <int DT, bool kVec>
+__global__ __launch_bounds__(kThreads) void combine_kernel(MoveArgs a) {
+  constexpr int kN = Chunk<DT>::kN, kBatch = 4;
+  int64_t t;
+  Part<DT, kVec> part;
+  if (!part_of(a, t, part)) return;
+  float sum[kN] = {};
+  const int32_t* at = a.places + t * a.k;
+  for (int j0 = 0; j0 < a.k; j0 += kBatch) {
+    int32_t p[kBatch];
+    float w[kBatch];
+    Chunk<DT> r[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) p[i] = j0 + i < a.k ? at[j0 + i] : -1;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (p[i] >= a.picks) p[i] = -1;
+      w[i] = p[i] >= 0 && a.weights != nullptr ? a.weights[t * a.k + j0 + i] : 1.0f;
+      r[i] = Chunk<DT>{};
+      if (p[i] >= 0) r[i] = part.load(a.rows, p[i], a.rows_ld);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (p[i] < 0) continue;
+#pragma unroll
+      for (int j = 0; j < kN; ++j) sum[j] += w[i] * r[i].get(j);
+    }
+  }
+  Chunk<DT> o;
+  if (a.residual != nullptr) {
+    const Chunk<DT> r = part.load(a.residual, t, a.residual_ld);
+#pragma unroll
+    for (int j = 0; j < kN; ++j) o.e[j] = round_to<DT>(sum[j] + r.get(j));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) o.e[j] = round_to<DT>(sum[j]);
+  }
+  part.store(a.y, t, o);
+}
+
+// y[places[t, j]] = weights[t, j] x[t], zeros for picks of nobody.
+template <int DT, bool kVec>
+__global__ __launch_bounds__(kThreads) void spread_kernel(MoveArgs a) {
+  constexpr int kN = Chunk<DT>::kN;
+  int64_t t;
+  Part<DT, kVec> part;
+  if (!part_of(a, t, part)) return;
+  const Chunk<DT> x = part.load(a.x, t, a.x_ld);
+  const int32_t* at = a.places + t * a.k;
+  for (int j = 0; j < a.k; ++j) {
+    const int32_t p = at[j], q = p < 0 ? ~p : p;
+    if (q >= a.picks) continue;
+    Chunk<DT> o{};
+    if (p >= 0) {
+      if (a.weights != nullptr) {
+        const float w = a.weights[t * a.k + j];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) o.e[i] = round_to<DT>(w * x.get(i));
+      } else {
+        o = x;
+      }
+    }
+    part.store(a.y, q, o);
+  }
+}
+
+// The same with the products <rows[places[t, j]], x[t]>: the row's threads walk over its columns, and add up in the end.
+template <int DT, bool kVec, int TPR, int K>
+__global__ __launch_bounds__(kThreads) void combine_grad_kernel(MoveArgs a) {
+  constexpr int kN = Chunk<DT>::kN;
+  using Sum = RowSum<TPR, K>;
+  __shared__ typename Sum::Lds lds;
+  int turn = 0;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
+  const int tid = static_cast<int>(threadIdx.x) % TPR;
+  if (TPR <= kWave && t >= a.T) return;  // (whole waves; with TPR > kWave a workgroup has one token)
+  int32_t p[K];
+  float w[K], dot[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    p[j] = j < a.k ? a.places[t * a.k + j] : -1;
+    w[j] = j < a.k ? a.weights == nullptr ? 1.0f : a.weights[t * a.k + j] : 0.0f;
+    dot[j] = 0.0f;
+  }
+  for (int first = 0; first < a.H; first += TPR * kN) {
+    Part<DT, kVec> part{kVec ? first + tid * kN : first + tid, kVec ? 1 : TPR, a.H};
+    if (part.col >= a.H) break;
+    const Chunk<DT> x = part.load(a.x, t, a.x_ld);
+    Chunk<DT> r[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      r[j] = Chunk<DT>{};
+      if (p[j] >= 0 && p[j] < a.picks) r[j] = part.load(a.rows, p[j], a.rows_ld);
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const int32_t q = p[j] < 0 ? ~p[j] : p[j];
+      if (j >= a.k || q >= a.picks) continue;
+      Chunk<DT> o{};
+      if (p[j] >= 0) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          dot[j] += r[j].get(i) * x.get(i);
+          o.e[i] = round_to<DT>(w[j] * x.get(i));
+        }
+      }
+      if (a.y != nullptr) part.store(a.y, q, o);
+    }
+  }
+  Sum::all(dot, lds, turn);
+  if (tid == 0) {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j < a.k) a.grad_weights[t * a.k + j] = dot[j];
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+int check_move(int64_t T, int64_t H, int64_t k, int dtype) {
+  if (T < 0 || H <= 0 || k <= 0 || !known_dtype(dtype)) return SMX_ERR_INVALID_ARG;
+  if (H > kMaxCols || k > kMaxPicks || T > INT32_MAX / k) return SMX_ERR_UNSUPPORTED;
+  return SMX_OK;
+}
+
+MoveArgs move_args(int64_t T, int64_t H, int64_t k, const int32_t* places) {
+  MoveArgs a{};
+  a.T = T;
+  a.picks = T * k;
+  a.H = static_cast<int>(H);
+  a.k = static_cast<int>(k);
+  a.places = places;
+  return a;
+}
+
+template <typename Kernel>
+hipError_t launch_parts(Kernel kernel, MoveArgs& a, int64_t es, hipStream_t s) {
+  const int64_t chunks = (a.H * es + 15) / 16;
+  a.shift = 0;
+  while (a.shift < 8 && (int64_t{1} << a.shift) < chunks) ++a.shift;
+  const int64_t tokens = kThreads >> a.shift, width = int64_t{1} << a.shift;
+  const dim3 grid(static_cast<unsigned>((a.T + tokens - 1) / tokens), static_cast<unsigned>((chunks + width - 1) / width));
+  kernel<<<grid, kThreads, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t launch_combine(int dtype, bool vec, MoveArgs& a, hipStream_t s) {
+  switch (dtype) {
+    case kF32: return launch_parts(vec ? combine_kernel<kF32, true> : combine_kernel<kF32, false>, a, 4, s);
+    case kF16: return launch_parts(vec ? combine_kernel<kF16, true> : combine_kernel<kF16, false>, a, 2, s);
+    default: return launch_parts(vec ? combine_kernel<kBF16, true> : combine_kernel<kBF16, false>, a, 2, s);
+  }
+}
+
+hipError_t launch_spread(int dtype, bool vec, MoveArgs& a, hipStream_t s) {
+  switch (dtype) {
+    case kF32: return launch_parts(vec ? spread_kernel<kF32, true> : spread_kernel<kF32, false>, a, 4, s);
+    case kF16: return launch_parts(vec ? spread_kernel<kF16, true> : spread_kernel<kF16, false>, a, 2, s);
+    default: return launch_parts(vec ? spread_kernel<kBF16, true> : spread_kernel<kBF16, false>, a, 2, s);
+  }
+}
+
+template <int DT, bool kVec, int TPR>
+hipError_t launch_grad_picks(const MoveArgs& a, hipStream_t s) {
+  const unsigned n = static_cast<unsigned>((a.T + kThreads / TPR - 1) / (kThreads / TPR));
+  if (a.k <= 2) combine_grad_kernel<DT, kVec, TPR, 2><<<n, kThreads, 0, s>>>(a);
+  else if (a.k <= 4) combine_grad_kernel<DT, kVec, TPR, 4><<<n, kThreads, 0, s>>>(a);
+  else if (a.k <= 8) combine_grad_kernel<DT, kVec, TPR, 8><<<n, kThreads, 0, s>>>(a);
+  else combine_grad_kernel<DT, kVec, TPR, 16><<<n, kThreads, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_grad(bool vec, const MoveArgs& a, hipStream_t s) {
+  // a workgroup a token where there are too few tokens to fill the chip with a wave each
+  if (a.T <= 2048) return vec ? launch_grad_picks<DT, true, 256>(a, s) : launch_grad_picks<DT, false, 256>(a, s);
+  return vec ? launch_grad_picks<DT, true, 64>(a, s) : launch_grad_picks<DT, false, 64>(a, s);
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" {
+
+int smx_dispatch_rows(const void* x, int64_t x_stride, int dtype, int64_t T, int64_t H, const int32_t* places, int64_t k,
+                      void* rows, void* stream) {
+  const int rc = check_move(T, H, k, dtype);
+  if (rc != SMX_OK) return rc;
+  if (x_stride < H) return SMX_ERR_INVALID_ARG;
+  if (T == 0) return SMX_OK;
+  if (!x || !places || !rows) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype);
+  if (!aligned_to(x, es) || !aligned_to(rows, es) || !aligned_to(places, 4)) return SMX_ERR_MISALIGNED;
+  MoveArgs a = move_args(T, H, k, places);
+  a.x = static_cast<const char*>(x);
+  a.x_ld = x_stride;
+  a.y = static_cast<char*>(rows);
+  return static_cast<int>(launch_spread(dtype, whole_chunks(x, x_stride, es) && whole_chunks(rows, H, es), a, static_cast<hipStream_t>(stream)));
+}
+
+int smx_combine_rows(const void* rows, int64_t rows_stride, int dtype, int64_t T, int64_t H, const int32_t* places,
+                     int64_t k, const float* weights, const void* residual, int64_t residual_stride, void* y,
+                     void* stream) {
+  const int rc = check_move(T, H, k, dtype);
+  if (rc != SMX_OK) return rc;
+  if (rows_stride < H || (residual && residual_stride < H)) return SMX_ERR_INVALID_ARG;
+  if (T == 0) return SMX_OK;
+  if (!rows || !places || !y) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype);
+  if (!aligned_to(rows, es) || !aligned_to(residual, es) || !aligned_to(y, es) || !aligned_to(places, 4) || !aligned_to(weights, 4))
+    return SMX_ERR_MISALIGNED;
+  MoveArgs a = move_args(T, H, k, places);
+  a.rows = static_cast<const char*>(rows);
+  a.rows_ld = rows_stride;
+  a.weights = weights;
+  a.residual = static_cast<const char*>(residual);
+  a.residual_ld = residual_stride;
+  a.y = static_cast<char*>(y);
+  const bool vec = whole_chunks(rows, rows_stride, es) && whole_chunks(y, H, es) && (!residual || whole_chunks(residual, residual_stride, es));
+  return static_cast<int>(launch_combine(dtype, vec, a, static_cast<hipStream_t>(stream)));
+}
+
+int smx_combine_rows_grad(const void* grad_y, int64_t grad_y_stride, const void* rows, int64_t rows_stride, int dtype,
+                          int64_t T, int64_t H, const int32_t* places, int64_t k, const float* weights, void* grad_rows,
+                          float* grad_weights, void* stream) {
+  const int rc = check_move(T, H, k, dtype);
+  if (rc != SMX_OK) return rc;
+  if (grad_y_stride < H || (grad_weights && rows_stride < H)) return SMX_ERR_INVALID_ARG;
+  if (T == 0 || (!grad_rows && !grad_weights)) return SMX_OK;
+  if (!grad_y || !places || (grad_weights && !rows)) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype);
+  if (!aligned_to(grad_y, es) || !aligned_to(rows, es) || !aligned_to(grad_rows, es) || !aligned_to(places, 4) || !aligned_to(weights, 4) ||
+      !aligned_to(grad_weights, 4))
+    return SMX_ERR_MISALIGNED;
+  MoveArgs a = move_args(T, H, k, places);
+  a.x = static_cast<const char*>(grad_y);
+  a.x_ld = grad_y_stride;
+  a.weights = weights;
+  a.y = static_cast<char*>(grad_rows);
+  const bool vec = whole_chunks(grad_y, grad_y_stride, es) && whole_chunks(grad_rows, H, es);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!grad_weights) return static_cast<int>(launch_spread(dtype, vec, a, s));
+  a.rows = static_cast<const char*>(rows);
+  a.rows_ld = rows_stride;
+  a.grad_weights = grad_weights;
+  const bool all = vec && whole_chunks(rows, rows_stride, es);
+  switch (dtype) {
+    case kF32: return static_cast<int>(launch_grad<kF32>(all, a, s));
+    case kF16: return static_cast<int>(launch_grad<kF16>(all, a, s));
+    default: return static_cast<int>(launch_grad<kBF16>(all, a, s));
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,447 @@
+// Layer norm and RMS norm with a residual, forward and backward.
+#include <algorithm>
+
+#include "blocks.h"
+
+namespace smx {
+namespace {
+
+constexpr int kMaxNorm = 16384;     // columns
+constexpr int kSmallBlock = 256;    // threads of a workgroup that holds several rows
+constexpr int kFoldWaves = 16;      // waves of a workgroup that adds up the partial weight gradients
+
+struct NormArgs {
+  const char* x;         // forward: x; backward: s
+  const char* residual;  // forward: residual; backward: gradient of the sum
+  const char* dy;
+  int64_t x_ld, residual_ld, dy_ld;
+  int64_t rows;
+  int H;
+  const void* weight;
+  const void* bias;
+  bool wide;             // the weights are fp32 and x is not
+  float eps;
+  char* y;               // forward: y; backward: gradient of x
+  char* sum;
+  float* stats;
+  float* part;           // backward: [2][blocks][H] partial sums, or null
+};
+
+template <int TPR> constexpr int block_threads() { return TPR < kSmallBlock ? kSmallBlock : TPR; }
+
+template <int DT, int TPR, int NV, bool kVec, bool kRms>
+__global__ __launch_bounds__(block_threads<TPR>()) void norm_kernel(NormArgs a) {
+  constexpr int kN = Chunk<DT>::kN, kRows = block_threads<TPR>() / TPR;
+  using S = typename Elem<DT>::S;
+  using Sum = RowSum<TPR, 1>;
+  __shared__ typename Sum::Lds lds;
+  int turn = 0;
+  const RowWalk<DT, TPR, kVec> walk{a.H, static_cast<int>(threadIdx.x) % TPR};
+  const int sub = threadIdx.x / TPR;
+  float w[NV][kN], b[NV][kN];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    walk.params(a.weight, a.wide, 1.0f, c, w[c]);
+    walk.params(a.bias, a.wide, 0.0f, c, b[c]);
+  }
+  const float inv = 1.0f / static_cast<float>(a.H);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  Chunk<DT> xr[NV], rr[NV];
+  auto fetch = [&](int64_t row) {
+    const S* x = reinterpret_cast<const S*>(a.x) + row * a.x_ld;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) xr[c] = walk.load(x, c);
+    if (a.residual != nullptr) {
+      const S* r = reinterpret_cast<const S*>(a.residual) + row * a.residual_ld;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) rr[c] = walk.load(r, c);
+    }
+  };
+  auto clamped = [&](int64_t row) { return row < a.rows ? row : a.rows - 1; };
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  if (row0 < a.rows) fetch(clamped(row0 + sub));
+  for (; row0 < a.rows; row0 += step) {
+    const int64_t row = row0 + sub;
+    const bool live = row < a.rows;
+    float h[NV][kN];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      if (a.residual != nullptr) {
+        Chunk<DT> s;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) s.e[j] = round_to<DT>(xr[c].get(j) + rr[c].get(j));
+        if (live) walk.store(reinterpret_cast<S*>(a.sum) + row * a.H, c, s);
+        xr[c] = s;
+      }
+#pragma unroll
+      for (int j = 0; j < kN; ++j) h[c][j] = xr[c].get(j);
+    }
+    if (row0 + step < a.rows) fetch(clamped(row + step));  // on its way while this row is summed
+    float mean = 0.0f;
+    if constexpr (!kRms) {
+      float s[1] = {0.0f};
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < kN; ++j) s[0] += h[c][j];
+      Sum::all(s, lds, turn);
+      mean = s[0] * inv;
+    }
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        if constexpr (!kRms) h[c][j] = walk.in(c, j) ? h[c][j] - mean : 0.0f;
+        q[0] += h[c][j] * h[c][j];
+      }
+    Sum::all(q, lds, turn);
+    const float rstd = rsqrtf(q[0] * inv + a.eps);
+    if (live) {
+      if (a.stats != nullptr && walk.tid == 0) {
+        if constexpr (kRms) {
+          a.stats[row] = rstd;
+        } else {
+          a.stats[2 * row] = mean;
+          a.stats[2 * row + 1] = rstd;
+        }
+      }
+      S* y = reinterpret_cast<S*>(a.y) + row * a.H;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        Chunk<DT> o;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) o.e[j] = round_to<DT>(h[c][j] * rstd * w[c][j] + b[c][j]);
+        walk.store(y, c, o);
+      }
+    }
+  }
+}
+
+template <int DT, int TPR, int NV, bool kVec, bool kRms>
+__global__ __launch_bounds__(block_threads<TPR>()) void norm_grad_kernel(NormArgs a) {
+  constexpr int kN = Chunk<DT>::kN, kRows = block_threads<TPR>() / TPR;
+  using S = typename Elem<DT>::S;
+  using Sum = RowSum<TPR, kRms ? 1 : 2>;
+  union Shared {
+    typename Sum::Lds sum;
+    float fold[kRows > 1 ? kRows : 1][kRows > 1 ? TPR * NV * kN : 1];
+  };
+  __shared__ Shared lds;
+  int turn = 0;
+  const RowWalk<DT, TPR, kVec> walk{a.H, static_cast<int>(threadIdx.x) % TPR};
+  const int sub = threadIdx.x / TPR;
+  float w[NV][kN], dw[NV][kN] = {}, db[NV][kN] = {};
+#pragma unroll
+  for (int c = 0; c < NV; ++c) walk.params(a.weight, a.wide, 1.0f, c, w[c]);
+  const float inv = 1.0f / static_cast<float>(a.H);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  Chunk<DT> xr[NV], gr[NV], sr[NV];
+  float mean_next = 0.0f, rstd_next = 0.0f;
+  auto fetch = [&](int64_t row) {
+    const S* x = reinterpret_cast<const S*>(a.x) + row * a.x_ld;
+    const S* g = reinterpret_cast<const S*>(a.dy) + row * a.dy_ld;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      xr[c] = walk.load(x, c);
+      gr[c] = walk.load(g, c);
+    }
+    if (a.residual != nullptr) {
+      const S* r = reinterpret_cast<const S*>(a.residual) + row * a.residual_ld;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) sr[c] = walk.load(r, c);
+    }
+    mean_next = kRms ? 0.0f : a.stats[2 * row];
+    rstd_next = kRms ? a.stats[row] : a.stats[2 * row + 1];
+  };
+  auto clamped = [&](int64_t row) { return row < a.rows ? row : a.rows - 1; };
+  int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
+  if (row0 < a.rows) fetch(clamped(row0 + sub));
+  for (; row0 < a.rows; row0 += step) {
+    const int64_t row = row0 + sub;
+    const bool live = row < a.rows;
+    const float mean = mean_next, rstd = rstd_next;
+    float n[NV][kN], g[NV][kN];
+    float s[kRms ? 1 : 2] = {};
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        // (a column behind the row's end has dy = 0; its n stays finite where the row's values are)
+        n[c][j] = walk.in(c, j) ? (xr[c].get(j) - mean) * rstd : 0.0f;
+        const float dy = gr[c].get(j);
+        g[c][j] = dy * w[c][j];
+        if (live) {
+          dw[c][j] += dy * n[c][j];
+          if constexpr (!kRms) db[c][j] += dy;
+        }
+        s[0] += g[c][j] * n[c][j];
+        if constexpr (!kRms) s[1] += g[c][j];
+      }
+    Chunk<DT> keep[NV];
+    if (a.residual != nullptr) {
+#pragma unroll
+      for (int c = 0; c < NV; ++c) keep[c] = sr[c];
+    }
+    if (row0 + step < a.rows) fetch(clamped(row + step));
+    Sum::all(s, lds.sum, turn);
+    if (live && a.y != nullptr) {
+      const float c2 = s[0] * inv, c1 = kRms ? 0.0f : s[kRms ? 0 : 1] * inv;
+      S* dx = reinterpret_cast<S*>(a.y) + row * a.H;
+#pragma unroll
+      for (int c = 0; c < NV; ++c) {
+        Chunk<DT> o;
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+          float v = g[c][j] - n[c][j] * c2;
+          if constexpr (!kRms) v -= c1;
+          v *= rstd;
+          if (a.residual != nullptr) v += keep[c].get(j);
+          o.e[j] = round_to<DT>(v);
+        }
+        walk.store(dx, c, o);
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  // the workgroup's column sums, its rows' threads added up in their order
+#pragma unroll
+  for (int which = 0; which < (kRms ? 1 : 2); ++which) {
+    float (&v)[NV][kN] = which == 0 ? dw : db;
+    float* out = a.part + (static_cast<int64_t>(which) * gridDim.x + blockIdx.x) * a.H;
+    if constexpr (kRows > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < kN; ++j) lds.fold[sub][walk.col(c, j)] = v[c][j];
+      __syncthreads();
+      for (int col = threadIdx.x; col < a.H; col += block_threads<TPR>()) {
+        float t = lds.fold[0][col];
+        for (int r = 1; r < kRows; ++r) t += lds.fold[r][col];
+        out[col] = t;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+          const int col = walk.col(c, j);
+          if (col < a.H) out[col] = v[c][j];
+        }
+    }
+  }
+}
+
+// Column sums of part [2][parts][H] into the gradients of the weight (plane 0) and the bias (plane 1): a workgroup takes 64
+// columns, its waves a share of the parts each.
+template <int DT>
+__global__ __launch_bounds__(kFoldWaves * kWave) void norm_fold_kernel(const float* part, int parts, int H, char* grad_weight,
+                                                                     char* grad_bias) {
+  __shared__ float lds[kFoldWaves][kWave];
+  const int wave = wave_id(), lane = lane_id(), col = static_cast<int>(blockIdx.x) * kWave + lane;
+  char* out = blockIdx.y == 0 ? grad_weight : grad_bias;
+  if (out == nullptr) return;
+  const float* p = part + static_cast<int64_t>(blockIdx.y) * parts * H;
+  float t = 0.0f;
+  if (col < H) {
+#pragma unroll 8
+    for (int i = wave; i < parts; i += kFoldWaves) t += p[static_cast<int64_t>(i) * H + col];
+  }
+  lds[wave][lane] = t;
+  __syncthreads();
+  if (wave != 0 || col >= H) return;
+#pragma unroll
+  for (int w = 1; w < kFoldWaves; ++w) t += lds[w][lane];
+  reinterpret_cast<typename Elem<DT>::S*>(out)[col] = round_to<DT>(t);
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+struct NormShape { int tpr, nv; };
+
+// Threads of a row and 16-byte chunks of a thread.
+NormShape shape_of(int64_t H, int dtype) {
+  const int64_t chunks = (H * dtype_bytes(dtype) + 15) / 16;
+  if (chunks <= 16) return {16, 1};
+  if (chunks <= 32) return {32, 1};
+  if (chunks <= 64) return {64, 1};
+  if (chunks <= 128) return {64, 2};
+  if (chunks <= 256) return {256, 1};
+  if (chunks <= 512) return {512, 1};
+  if (chunks <= 1024) return {1024, 1};
+  if (chunks <= 2048) return {1024, 2};
+  return {1024, 4};
+}
+
+int64_t rows_at_once(const NormShape& s) { return s.tpr < kSmallBlock ? kSmallBlock / s.tpr : 1; }
+
+// Workgroups of the forward pass: as many as the chip holds at once, walking over the rows.
+int64_t forward_blocks(const NormShape& s, int64_t rows) {
+  const int64_t threads = std::max(s.tpr, kSmallBlock);
+  return std::min((rows + rows_at_once(s) - 1) / rows_at_once(s), int64_t{256} * 2048 / threads);
+}
+
+// Of the backward pass: fewer, since each leaves its partial weight gradients.
+int64_t grad_blocks(const NormShape& s, int64_t rows) {
+  const int64_t threads = std::max(s.tpr, kSmallBlock);
+  return std::min((rows + rows_at_once(s) - 1) / rows_at_once(s), int64_t{256} * 1024 / threads);
+}
+
+int check_norm(int kind, int64_t rows, int64_t H, int dtype) {
+  if ((kind != SMX_NORM_LAYER && kind != SMX_NORM_RMS) || rows < 0 || H <= 0 || !known_dtype(dtype)) return SMX_ERR_INVALID_ARG;
+  if (H > kMaxNorm || rows > (int64_t{1} << 40)) return SMX_ERR_UNSUPPORTED;
+  return SMX_OK;
+}
+
+template <bool kGrad, int DT, int TPR, int NV, bool kVec>
+void launch(const NormArgs& a, bool rms, unsigned blocks, hipStream_t s) {
+  constexpr int threads = block_threads<TPR>();
+  if constexpr (kGrad) {
+    if (rms) norm_grad_kernel<DT, TPR, NV, kVec, true><<<blocks, threads, 0, s>>>(a);
+    else norm_grad_kernel<DT, TPR, NV, kVec, false><<<blocks, threads, 0, s>>>(a);
+  } else {
+    if (rms) norm_kernel<DT, TPR, NV, kVec, true><<<blocks, threads, 0, s>>>(a);
+    else norm_kernel<DT, TPR, NV, kVec, false><<<blocks, threads, 0, s>>>(a);
+  }
+}
+
+template <bool kGrad, int DT, bool kVec>
+void launch_shape(const NormShape& f, const NormArgs& a, bool rms, unsigned blocks, hipStream_t s) {
+  switch (f.tpr) {
+    case 16: return launch<kGrad, DT, 16, 1, kVec>(a, rms, blocks, s);
+    case 32: return launch<kGrad, DT, 32, 1, kVec>(a, rms, blocks, s);
+    case 64:
+      if (f.nv == 1) return launch<kGrad, DT, 64, 1, kVec>(a, rms, blocks, s);
+      return launch<kGrad, DT, 64, 2, kVec>(a, rms, blocks, s);
+    case 256: return launch<kGrad, DT, 256, 1, kVec>(a, rms, blocks, s);
+    case 512: return launch<kGrad, DT, 512, 1, kVec>(a, rms, blocks, s);
+    default:
+      if (f.nv == 1) return launch<kGrad, DT, 1024, 1, kVec>(a, rms, blocks, s);
+      if (f.nv == 2) return launch<kGrad, DT, 1024, 2, kVec>(a, rms, blocks, s);
+      if constexpr (DT == kF32) return launch<kGrad, DT, 1024, 4, kVec>(a, rms, blocks, s);
+  }
+}
+
+template <bool kGrad>
+hipError_t launch_norm(int dtype, bool vec, const NormShape& f, const NormArgs& a, bool rms, int64_t blocks, hipStream_t s) {
+  const unsigned n = static_cast<unsigned>(blocks);
+  switch (dtype) {
+    case kF32:
+      vec ? launch_shape<kGrad, kF32, true>(f, a, rms, n, s) : launch_shape<kGrad, kF32, false>(f, a, rms, n, s);
+      break;
+    case kF16:
+      vec ? launch_shape<kGrad, kF16, true>(f, a, rms, n, s) : launch_shape<kGrad, kF16, false>(f, a, rms, n, s);
+      break;
+    default:
+      vec ? launch_shape<kGrad, kBF16, true>(f, a, rms, n, s) : launch_shape<kGrad, kBF16, false>(f, a, rms, n, s);
+      break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" {
+
+int smx_norm(int kind, const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, int dtype,
+             int64_t rows, int64_t H, const void* weight, const void* bias, int weight_dtype, float eps, void* y,
+             void* sum, float* stats, void* stream) {
+  const int rc = check_norm(kind, rows, H, dtype);
+  if (rc != SMX_OK) return rc;
+  const bool any = weight != nullptr || bias != nullptr;
+  if (x_stride < H || (residual && residual_stride < H) || !(eps >= 0.0f) || (any && weight_dtype != dtype && weight_dtype != kF32))
+    return SMX_ERR_INVALID_ARG;
+  if (rows == 0) return SMX_OK;
+  if (!x || !y || (residual == nullptr) != (sum == nullptr)) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype), ws = dtype_bytes(weight_dtype);
+  if (!aligned_to(x, es) || !aligned_to(residual, es) || !aligned_to(y, es) || !aligned_to(sum, es) ||
+      (any && (!aligned_to(weight, ws) || !aligned_to(bias, ws))) || !aligned_to(stats, 4))
+    return SMX_ERR_MISALIGNED;
+  const bool vec = whole_chunks(x, x_stride, es) && whole_chunks(y, H, es) && (!residual || (whole_chunks(residual, residual_stride, es) && whole_chunks(sum, H, es))) &&
+                   aligned_to(weight, 16) && aligned_to(bias, 16);
+  NormArgs a{};
+  a.x = static_cast<const char*>(x);
+  a.x_ld = x_stride;
+  a.residual = static_cast<const char*>(residual);
+  a.residual_ld = residual_stride;
+  a.rows = rows;
+  a.H = static_cast<int>(H);
+  a.weight = weight;
+  a.bias = bias;
+  a.wide = any && weight_dtype != dtype;
+  a.eps = eps;
+  a.y = static_cast<char*>(y);
+  a.sum = static_cast<char*>(sum);
+  a.stats = stats;
+  const NormShape f = shape_of(H, dtype);
+  return static_cast<int>(launch_norm<false>(dtype, vec, f, a, kind == SMX_NORM_RMS, forward_blocks(f, rows), static_cast<hipStream_t>(stream)));
+}
+
+size_t smx_norm_grad_workspace_size(int kind, int64_t rows, int64_t H, int dtype) {
+  if (check_norm(kind, rows, H, dtype) != SMX_OK) return 0;
+  return static_cast<size_t>(grad_blocks(shape_of(H, dtype), rows) * H * 4 * (kind == SMX_NORM_RMS ? 1 : 2));
+}
+
+int smx_norm_grad(int kind, const void* grad_y, int64_t grad_y_stride, const void* grad_sum, int64_t grad_sum_stride,
+                  const void* s, int64_t s_stride, int dtype, int64_t rows, int64_t H, const void* weight,
+                  int weight_dtype, const float* stats, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  const int rc = check_norm(kind, rows, H, dtype);
+  if (rc != SMX_OK) return rc;
+  const bool rms = kind == SMX_NORM_RMS, sums = grad_weight || grad_bias;
+  if (grad_y_stride < H || s_stride < H || (grad_sum && grad_sum_stride < H) || (rms && grad_bias) ||
+      ((weight || sums) && weight_dtype != dtype && weight_dtype != kF32))
+    return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype), ws = dtype_bytes(weight_dtype);
+  if (rows > 0 && (!grad_y || !s || !stats)) return SMX_ERR_INVALID_ARG;
+  if (!aligned_to(grad_y, es) || !aligned_to(grad_sum, es) || !aligned_to(s, es) || !aligned_to(grad_x, es) || !aligned_to(stats, 4) ||
+      ((weight || sums) && (!aligned_to(weight, ws) || !aligned_to(grad_weight, ws) || !aligned_to(grad_bias, ws))))
+    return SMX_ERR_MISALIGNED;
+  const NormShape f = shape_of(H, dtype);
+  const int64_t blocks = grad_blocks(f, rows);
+  if (sums && rows > 0) {
+    if (!workspace || workspace_bytes < smx_norm_grad_workspace_size(kind, rows, H, dtype)) return SMX_ERR_WORKSPACE;
+    if (!aligned_to(workspace, 16)) return SMX_ERR_MISALIGNED;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (rows > 0 && (grad_x || sums)) {
+    NormArgs a{};
+    a.x = static_cast<const char*>(s);
+    a.x_ld = s_stride;
+    a.dy = static_cast<const char*>(grad_y);
+    a.dy_ld = grad_y_stride;
+    a.residual = grad_x ? static_cast<const char*>(grad_sum) : nullptr;
+    a.residual_ld = grad_sum_stride;
+    a.rows = rows;
+    a.H = static_cast<int>(H);
+    a.weight = weight;
+    a.wide = weight && weight_dtype != dtype;
+    a.y = static_cast<char*>(grad_x);
+    a.stats = const_cast<float*>(stats);
+    a.part = sums ? static_cast<float*>(workspace) : nullptr;
+    const bool vec = whole_chunks(s, s_stride, es) && whole_chunks(grad_y, grad_y_stride, es) && whole_chunks(grad_x, H, es) &&
+                     (!a.residual || whole_chunks(grad_sum, grad_sum_stride, es)) && aligned_to(weight, 16);
+    const hipError_t err = launch_norm<true>(dtype, vec, f, a, rms, blocks, st);
+    if (err != hipSuccess) return static_cast<int>(err);
+  }
+  if (sums) {
+    const dim3 grid(static_cast<unsigned>((H + kWave - 1) / kWave), grad_bias ? 2 : 1);
+    const float* part = static_cast<const float*>(workspace);
+    const int parts = rows > 0 ? static_cast<int>(blocks) : 0, n = static_cast<int>(H);
+    char* gw = static_cast<char*>(grad_weight);
+    char* gb = static_cast<char*>(grad_bias);
+    switch (weight_dtype) {
+      case kF32: norm_fold_kernel<kF32><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
+      case kF16: norm_fold_kernel<kF16><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
+      default: norm_fold_kernel<kBF16><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
+    }
+    return static_cast<int>(hipGetLastError());
+  }
+  return SMX_OK;
+}
+
+}  // extern "C"

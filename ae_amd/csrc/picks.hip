@@ -1,0 +1,779 @@
+// Routing for training and serving: each token's best experts with their weights, the picks' order by expert, and the
+// gradient of the logits.
+//
+//   pick_kernel        L lanes a token with PL experts each: scores, groups, the k best, their weights; and where order
+//                      is asked for, each pick's rank among the picks of its expert in the workgroup's tokens, with the
+//                      workgroup's counts per expert. One workgroup does it all for few tokens.
+//   pick_scan_kernel   counts per workgroup and expert -> the picks of an expert before a workgroup's
+//   pick_place_kernel  place = the expert's first + those before the workgroup's + the rank
+//   pick_grad_kernel   the gradient of a token's logits
+//
+// Everything is counted in integers and in the order of the picks, so the order is the stable one on every run.
+#include <algorithm>
+
+#include "blocks.h"
+
+namespace smx {
+namespace {
+
+constexpr int kPickThreads = 256;
+constexpr int kMaxK = 16;
+constexpr int kMaxE = 1024;
+constexpr int kMaxGroups = 64;
+constexpr int kEntry = kMaxK + 1;     // slots of a token's picks: one more, whose distance is looked at
+constexpr int kBlockPicks = 2048;     // picks whose ranks a workgroup holds
+constexpr int kScanWaves = 16;
+constexpr int kOneBlock = 512;        // picks that one workgroup sorts by itself
+
+struct PickArgs {
+  const char* logits;
+  int64_t ld, T;
+  int E, k, ng, tg, gs;
+  bool sigmoid, renorm, grad_dense;
+  float scale;
+  const float* bias;
+  float* weights;
+  int32_t* ids;
+  int32_t* places;     // null: no order
+  int32_t* order;
+  int64_t* offsets;
+  int32_t* counts;     // [blocks][E + 1] picks of the workgroup per expert (E: of nobody)
+  int32_t* totals;     // [E + 1]
+  int wave_tokens;     // consecutive tokens of a wave
+  int blocks;
+  int bits;            // of an expert's number, E among them
+  const float* grad_w;
+  char* grad;
+};
+
+__device__ __forceinline__ void wave_sync() {  // what this wave's lanes wrote to LDS is there for its other lanes
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Values in an order of unsigned numbers: -inf is 0 (nobody's pick), NaN the largest, -0 as +0.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  if (v != v) return 0xffffffffu;
+  if (v == -__builtin_inff()) return 0u;
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  if (k == 0u) return -__builtin_inff();
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);  // (the largest key is a NaN)
+}
+__device__ __forceinline__ uint64_t key_of(double v) {
+  if (v != v) return ~uint64_t{0};
+  if (v == -__builtin_inf()) return 0u;
+  const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+  return (u >> 63) ? ~u : (u | (uint64_t{1} << 63));
+}
+__device__ __forceinline__ double value_of(uint64_t k) {
+  if (k == 0u) return -__builtin_inf();
+  return __builtin_bit_cast(double, (k >> 63) ? (k & ~(uint64_t{1} << 63)) : ~k);
+}
+
+template <int L> __device__ __forceinline__ float sum_over(float v) {
+  return group_reduce<L>(v, [](float a, float b) { return a + b; });
+}
+template <int L> __device__ __forceinline__ float max_over(float v) {
+  return group_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int L> __device__ __forceinline__ uint32_t max_over(uint32_t v) {
+  auto step = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  v = step(v, static_cast<uint32_t>(dpp<kDppXor1>(static_cast<int>(v))));
+  v = step(v, static_cast<uint32_t>(dpp<kDppXor2>(static_cast<int>(v))));
+  v = step(v, static_cast<uint32_t>(dpp<kDppHalfMirror>(static_cast<int>(v))));
+  v = step(v, static_cast<uint32_t>(dpp<kDppMirror>(static_cast<int>(v))));
+  if constexpr (L == kWave) {
+    const int s = static_cast<int>(v);
+    v = step(step(static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 0)), static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 16))),
+             step(static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 32)), static_cast<uint32_t>(__builtin_amdgcn_readlane(s, 48))));
+  }
+  return v;
+}
+
+// PL consecutive logits of a row from e on; -inf behind its end. `whole`: rows and base of aligned runs of PL.
+template <int DT, int PL>
+__device__ __forceinline__ void load_run(const char* base, int64_t at, int e, int E, bool whole, float (&v)[PL]) {
+  using S = typename Elem<DT>::S;
+  const S* p = reinterpret_cast<const S*>(base) + at + e;
+  if (whole) {
+    struct alignas(PL * sizeof(S) < 16 ? PL * sizeof(S) : 16) Run { S s[PL]; } r = {};
+    const bool in = e < E;
+    if (in) r = *reinterpret_cast<const Run*>(p);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) v[i] = in ? Elem<DT>::to_f32(r.s[i]) : -__builtin_inff();
+  } else {
+#pragma unroll
+    for (int i = 0; i < PL; ++i) v[i] = e + i < E ? Elem<DT>::to_f32(p[i]) : -__builtin_inff();
+  }
+}
+
+__device__ __forceinline__ float sigmoid_of(float x) {
+  const float e = expf(-fabsf(x));
+  return (x < 0.0f ? e : 1.0f) / (1.0f + e);  // NaN stays NaN
+}
+
+// LDS of a wave: the picks of its tokens, their keys; the choices of its tokens by key while groups are compared,
+// or those of one token in 64 bits; the picks per expert so far.
+template <int L, int PL> struct PickLds {
+  static constexpr int kTokens = kWave / L;
+  int entry[kTokens * kEntry];
+  uint32_t key[kTokens * kEntry];
+  union {
+    uint32_t choice[kTokens][L * PL];
+    uint64_t exact[L * PL];
+  };
+  uint32_t group[kTokens][kMaxGroups];
+};
+
+// The picks of one token by its choices in 64 bits: the whole wave's work, for tokens whose choices 32 bits cannot tell
+// apart.
+template <int DT>
+__device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint64_t* key, int* entry) {
+  using S = typename Elem<DT>::S;
+  const int lane = lane_id();
+  const S* row = reinterpret_cast<const S*>(a.logits) + t * a.ld;
+  auto top_of = [](uint64_t k) {
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const uint64_t o = __shfl_xor(k, off, kWave);
+      k = o > k ? o : k;
+    }
+    return k;
+  };
+  double m = 0.0, z = 1.0;
+  if (!a.sigmoid) {
+    float top = -__builtin_inff();
+    for (int e = lane; e < a.E; e += kWave) top = fmaxf(top, Elem<DT>::to_f32(row[e]));
+    m = max_over<kWave>(top);
+    z = 0.0;
+    for (int e = lane; e < a.E; e += kWave) z += exp(static_cast<double>(Elem<DT>::to_f32(row[e])) - m);
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) z += __shfl_xor(z, off, kWave);
+  }
+  for (int e = lane; e < a.E; e += kWave) {
+    const double x = Elem<DT>::to_f32(row[e]);
+    const double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - m) / z;
+    key[e] = x == -__builtin_inf() ? 0u : key_of(s + static_cast<double>(a.bias[e]));
+  }
+  wave_sync();
+  if (a.tg < a.ng) {
+    uint64_t mine = 0u;
+    if (lane < a.ng) {
+      uint64_t best = 0u, next = 0u;
+      for (int i = 0; i < a.gs; ++i) {
+        const uint64_t c = key[lane * a.gs + i];
+        if (c > best) {
+          next = best;
+          best = c;
+        } else if (c > next) {
+          next = c;
+        }
+      }
+      mine = best == 0u ? 0u : key_of(value_of(best) + (next == 0u ? 0.0 : value_of(next)));
+    }
+    int before = 0;
+    for (int g = 0; g < a.ng; ++g) {
+      const uint64_t o = __shfl(mine, g, kWave);
+      before += o > mine || (o == mine && g < lane);
+    }
+    const uint64_t kept = ballot(lane < a.ng && before < a.tg);
+    for (int e = lane; e < a.E; e += kWave)
+      if (!((kept >> (e / a.gs)) & 1u)) key[e] = 0u;
+    wave_sync();
+  }
+  for (int j = 0; j < a.k; ++j) {
+    uint64_t best = 0u;
+    int at = a.E;
+    for (int e = lane; e < a.E; e += kWave)
+      if (key[e] > best) {
+        best = key[e];
+        at = e;
+      }
+    const uint64_t top = top_of(best);
+    // ties: the lowest expert
+    int low = top != 0u && best == top ? at : a.E;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) low = min(low, __shfl_xor(low, off, kWave));
+    if (low < a.E && at == low && best == top) key[at] = 0u;
+    if (lane == 0) entry[j] = low;
+    wave_sync();
+  }
+}
+
+// Exclusive prefix sums over n <= 4 * 1025 counts in LDS, by the whole workgroup (of at least one wave).
+__device__ __forceinline__ void block_scan(int32_t* v, int n, int32_t* waves) {
+  const int threads = static_cast<int>(blockDim.x), per = (n + threads - 1) / threads;
+  const int first = static_cast<int>(threadIdx.x) * per;
+  int sum = 0;
+  for (int i = 0; i < per; ++i) sum += first + i < n ? v[first + i] : 0;
+  const int incl = wave_incl_scan(sum);
+  if (lane_id() == kWave - 1) waves[wave_id()] = incl;
+  __syncthreads();
+  int before = incl - sum;
+  for (int w = 0; w < wave_id(); ++w) before += waves[w];
+  for (int i = 0; i < per; ++i) {
+    if (first + i >= n) break;
+    const int c = v[first + i];
+    v[first + i] = before;
+    before += c;
+  }
+  __syncthreads();
+}
+
+template <int DT, int L, int PL, bool kBiased>
+__global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool whole) {
+  constexpr int kTokens = kWave / L;
+  using Lds = PickLds<L, PL>;
+  extern __shared__ __attribute__((aligned(16))) char shared[];
+  const int waves = static_cast<int>(blockDim.x) / kWave, wave = wave_id(), lane = lane_id();
+  Lds& lds = reinterpret_cast<Lds*>(shared)[wave];
+  int32_t* counts = reinterpret_cast<int32_t*>(shared + waves * sizeof(Lds));  // [waves][E + 1], then the first of each expert
+  int32_t* local = counts + (waves + 1) * (a.E + 1);                           // expert and rank of the workgroup's picks
+  const int seg = lane / L, l = lane % L, E = a.E, k = a.k;
+  const bool ordered = a.places != nullptr;
+  int32_t* mine = counts + wave * (E + 1);
+  if (ordered) {
+    for (int e = lane; e <= E; e += kWave) mine[e] = 0;
+    wave_sync();
+  }
+  float b[PL], far = 0.0f;  // the largest finite bias
+  if constexpr (kBiased) {
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      b[i] = l * PL + i < E ? a.bias[l * PL + i] : 0.0f;
+      if (fabsf(b[i]) < __builtin_inff()) far = fmaxf(far, fabsf(b[i]));
+    }
+    far = max_over<L>(far);
+  }
+  const int64_t block_first = static_cast<int64_t>(blockIdx.x) * waves * a.wave_tokens;
+  const int64_t first = block_first + static_cast<int64_t>(wave) * a.wave_tokens;
+  const int64_t last = first + a.wave_tokens < a.T ? first + a.wave_tokens : a.T;
+  int* entry = lds.entry + seg * kEntry;
+  uint32_t* ekey = lds.key + seg * kEntry;
+  for (int64_t t0 = first; t0 < last; t0 += kTokens) {
+    const int64_t t = t0 + seg;
+    const bool live = t < last;
+    const int64_t at = (live ? t : last - 1) * a.ld;
+    float v[PL];
+    load_run<DT, PL>(a.logits, at, l * PL, E, whole, v);
+    float m = 0.0f, z = 1.0f;
+    if (!a.sigmoid && (kBiased || !a.renorm)) {
+      m = v[0];
+#pragma unroll
+      for (int i = 1; i < PL; ++i) m = fmaxf(m, v[i]);
+      m = max_over<L>(m);
+      z = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PL; ++i) z += l * PL + i < E ? expf(v[i] - m) : 0.0f;
+      z = sum_over<L>(z);
+    }
+    uint32_t key[PL];
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      if constexpr (kBiased) {
+        const float s = a.sigmoid ? sigmoid_of(v[i]) : expf(v[i] - m) / z;
+        key[i] = v[i] == -__builtin_inff() ? 0u : key_of(s + b[i]);
+      } else {
+        key[i] = key_of(v[i]);
+      }
+    }
+    bool close = false;  // choices too near for 32 bits
+    if (a.tg < a.ng) {
+#pragma unroll
+      for (int i = 0; i < PL; ++i) lds.choice[seg][l * PL + i] = key[i];
+      wave_sync();
+      for (int g = l; g < a.ng; g += L) {
+        uint32_t best = 0u, next = 0u;
+        for (int i = 0; i < a.gs; ++i) {
+          const uint32_t c = lds.choice[seg][g * a.gs + i];
+          if (kBiased && c <= best) next = c > next ? c : next;
+          if (kBiased && c > best) next = best;
+          best = c > best ? c : best;
+        }
+        if (kBiased && best != 0u && next != 0u) best = key_of(value_of(best) + value_of(next));
+        lds.group[seg][g] = best;
+      }
+      wave_sync();
+      uint64_t kept = 0u;
+      float low = __builtin_inff(), high = -__builtin_inff();
+      for (int g0 = 0; g0 < a.ng; g0 += L) {
+        const int g = g0 + l;
+        bool keep = false;
+        if (g < a.ng) {
+          const uint32_t c = lds.group[seg][g];
+          int before = 0;
+          for (int o = 0; o < a.ng; ++o) {
+            const uint32_t other = lds.group[seg][o];
+            before += other > c || (other == c && o < g);
+          }
+          keep = before < a.tg;
+          if (keep) low = fminf(low, value_of(c));
+          else high = fmaxf(high, value_of(c));
+        }
+        const uint64_t bitsv = ballot(keep);
+        kept |= (L == kWave ? bitsv : (bitsv >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1)) << g0;
+      }
+      if constexpr (kBiased) {
+        low = -max_over<L>(-low);
+        high = max_over<L>(high);
+        // a group's choice is the sum of two scores, each off by 2^-18 at most, and of two biases; three roundings
+        if (low - high <= 0x1p-16f + 0x1p-21f * far) close = true;
+      }
+      const int e0 = l * PL;
+      int g = e0 / a.gs, rest = e0 - g * a.gs;
+#pragma unroll
+      for (int i = 0; i < PL; ++i) {
+        if (!((kept >> (g & 63)) & 1u)) key[i] = 0u;
+        if (++rest == a.gs) {
+          rest = 0;
+          ++g;
+        }
+      }
+      wave_sync();
+    }
+    const int rounds = k + (kBiased ? 1 : 0);
+    for (int j = 0; j < rounds; ++j) {
+      uint32_t top = key[0];
+#pragma unroll
+      for (int i = 1; i < PL; ++i) top = key[i] > top ? key[i] : top;
+      const uint32_t all = max_over<L>(top);
+      const uint64_t who = ballot(top == all && all != 0u);
+      const uint64_t of_token = L == kWave ? who : (who >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
+      const bool winner = of_token != 0u && l == __builtin_ctzll(of_token);
+      int slot = -1;
+#pragma unroll
+      for (int i = PL - 1; i >= 0; --i) slot = winner && key[i] == all ? i : slot;
+#pragma unroll
+      for (int i = 0; i < PL; ++i) key[i] = i == slot ? 0u : key[i];
+      if (winner || (of_token == 0u && l == 0)) {
+        entry[j] = winner ? l * PL + slot : E;
+        ekey[j] = all;
+      }
+    }
+    wave_sync();
+    using S = typename Elem<DT>::S;
+    const S* row = reinterpret_cast<const S*>(a.logits) + at;
+    if constexpr (kBiased) {
+      if (l < k) {
+        const int e = entry[l], n = entry[l + 1];
+        if (e < E && n < E) {
+          const float x = Elem<DT>::to_f32(row[e]), y = Elem<DT>::to_f32(row[n]), p = a.bias[e], q = a.bias[n];
+          const float c = value_of(ekey[l]), d = value_of(ekey[l + 1]);
+          // a score is off by 16 roundings of itself and by those of exp's argument, a choice by one more
+          const float off = fabsf(c - p) * (0x1p-19f + 0x1p-22f * fabsf(x - m)) + fabsf(d - q) * (0x1p-19f + 0x1p-22f * fabsf(y - m)) +
+                            0x1p-22f * (fabsf(c) + fabsf(d)) + 1e-37f;
+          if (c - d <= off && !(x == y && p == q)) close = true;
+        }
+      }
+      uint64_t again = ballot(close && live);
+      while (again != 0u) {
+        const int s = __builtin_ctzll(again) / L;
+        again &= L == kWave ? 0u : ~(((uint64_t{1} << (L % kWave)) - 1) << (s * L));
+        wave_sync();
+        pick_exactly<DT>(a, t0 + s, lds.exact, lds.entry + s * kEntry);
+      }
+    }
+    // the weights: lane j has pick j
+    const int e = l < k ? entry[l] : E;
+    const bool some = e < E;
+    float x = -__builtin_inff();
+    if (some) x = kBiased ? Elem<DT>::to_f32(row[e]) : value_of(ekey[l]);
+    float s;
+    if (a.renorm) {
+      // ratios of scores, scaled by the largest so that they do not vanish together
+      const float lead = a.sigmoid ? fminf(x, 0.0f) : x;
+      const float most = max_over<L>(some ? lead : -__builtin_inff());
+      s = some ? expf(lead - most) : 0.0f;
+      if (a.sigmoid && some) s = (x != x ? x : s) / (1.0f + expf(-fabsf(x)));
+      s = s / sum_over<L>(s);
+    } else {
+      s = a.sigmoid ? sigmoid_of(x) : expf(x - m) / z;
+    }
+    if (live && l < k) {
+      a.weights[t * k + l] = some ? a.scale * s : 0.0f;
+      a.ids[t * k + l] = some ? e : -1;
+    }
+    if (ordered) {
+      // lane p has pick p of the wave's tokens
+      const int of = lane / k, j = lane - of * k;
+      const bool valid = of < kTokens && t0 + of < last;
+      const int who = valid ? lds.entry[of * kEntry + j] : 0;
+      const uint64_t same = same_expert_lanes(who, valid, a.bits);
+      if (valid) {
+        const uint64_t lower = same & ((uint64_t{1} << lane) - 1);
+        const int rank = mine[who] + __builtin_popcountll(lower);
+        local[static_cast<int>(t0 + of - block_first) * k + j] = (rank << 16) | who;
+        wave_sync();
+        if ((same >> lane) == 1u) mine[who] = rank + 1;
+      }
+      wave_sync();
+    }
+    wave_sync();
+  }
+  if (!ordered) return;
+  __syncthreads();
+  const bool alone = gridDim.x == 1;
+  int32_t* starts = counts + waves * (E + 1);
+  for (int e = threadIdx.x; e <= E; e += static_cast<int>(blockDim.x)) {
+    int sum = 0;
+    for (int w = 0; w < waves; ++w) {
+      const int c = counts[w * (E + 1) + e];
+      counts[w * (E + 1) + e] = sum;
+      sum += c;
+    }
+    starts[e] = alone ? sum : 0;
+    if (!alone) a.counts[static_cast<int64_t>(blockIdx.x) * (E + 1) + e] = sum;
+  }
+  __syncthreads();
+  if (alone) {
+    block_scan(starts, E + 1, reinterpret_cast<int32_t*>(shared));
+    for (int e = threadIdx.x; e <= E; e += static_cast<int>(blockDim.x)) a.offsets[e] = starts[e];
+  }
+  const int64_t rest = a.T - block_first;
+  const int tokens = rest < static_cast<int64_t>(waves) * a.wave_tokens ? static_cast<int>(rest) : waves * a.wave_tokens;
+  for (int i = threadIdx.x; i < tokens * k; i += static_cast<int>(blockDim.x)) {
+    const int who = local[i] & 0xffff, w = i / (a.wave_tokens * k);
+    const int place = starts[who] + counts[w * (E + 1) + who] + (local[i] >> 16);
+    a.places[block_first * k + i] = alone && who == E ? ~place : place;
+    if (alone) a.order[place] = who == E ? ~i : i;
+  }
+}
+
+// counts [blocks][E + 1] -> exclusive prefix sums over the workgroups, and the totals. A workgroup takes 64 experts, a wave
+// a share of the rows each.
+__global__ __launch_bounds__(kScanWaves * kWave) void pick_scan_kernel(PickArgs a) {
+  __shared__ int32_t sums[kScanWaves][kWave];
+  const int lane = lane_id(), wave = wave_id(), n = a.E + 1, e = static_cast<int>(blockIdx.x) * kWave + lane;
+  const int per = (a.blocks + kScanWaves - 1) / kScanWaves, first = wave * per;
+  const int end = first + per < a.blocks ? first + per : a.blocks;
+  int32_t* p = a.counts + e;
+  int sum = 0;
+  if (e < n) {
+#pragma unroll 8
+    for (int i = first; i < end; ++i) sum += p[static_cast<int64_t>(i) * n];
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (e >= n) return;
+  int before = 0, all = 0;
+  for (int w = 0; w < kScanWaves; ++w) {
+    if (w < wave) before += sums[w][lane];
+    all += sums[w][lane];
+  }
+  if (wave == 0) a.totals[e] = all;
+#pragma unroll 8
+  for (int i = first; i < end; ++i) {
+    const int c = p[static_cast<int64_t>(i) * n];
+    p[static_cast<int64_t>(i) * n] = before;
+    before += c;
+  }
+}
+
+__global__ __launch_bounds__(kPickThreads) void pick_place_kernel(PickArgs a, int block_tokens, int per_block) {
+  __shared__ int32_t starts[kMaxE + 1];
+  __shared__ int32_t waves[kPickThreads / kWave];
+  const int n = a.E + 1;
+  for (int e = threadIdx.x; e < n; e += kPickThreads) starts[e] = a.totals[e];
+  __syncthreads();
+  block_scan(starts, n, waves);
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e < n; e += kPickThreads) a.offsets[e] = starts[e];
+  const int64_t picks = a.T * a.k, first = static_cast<int64_t>(blockIdx.x) * per_block;
+  const int64_t end = first + per_block < picks ? first + per_block : picks;
+  for (int64_t i = first + threadIdx.x; i < end; i += kPickThreads) {
+    const int id = a.ids[i], who = id < 0 ? a.E : id;
+    const uint32_t block = static_cast<uint32_t>(i) / static_cast<uint32_t>(block_tokens * a.k);
+    const int place = starts[who] + a.counts[static_cast<int64_t>(block) * n + who] + a.places[i];
+    a.places[i] = id < 0 ? ~place : place;
+    a.order[place] = static_cast<int32_t>(id < 0 ? ~i : i);
+  }
+}
+
+__global__ __launch_bounds__(kPickThreads) void no_picks_kernel(int64_t* offsets, int n) {
+  const int e = static_cast<int>(blockIdx.x) * kPickThreads + static_cast<int>(threadIdx.x);
+  if (e < n) offsets[e] = 0;
+}
+
+// With p the weights before the scale, g = scale * grad_w, D = sum over the picks of p g:
+//   softmax              s_e ([e picked] g_e - D)   over all experts
+//   softmax, renormed    p_j (g_j - D)              at the picks
+//   sigmoid              s_j (1 - s_j) g_j          at the picks
+//   sigmoid, renormed    p_j (1 - s_j) (g_j - D)    at the picks
+template <int DT, int L, int PL>
+__global__ __launch_bounds__(kPickThreads) void pick_grad_kernel(PickArgs a, bool whole) {
+  constexpr int kTokens = kWave / L;
+  using S = typename Elem<DT>::S;
+  __shared__ float ds[kPickThreads / kWave][kTokens][kMaxK];
+  __shared__ int es[kPickThreads / kWave][kTokens][kMaxK];
+  const int wave = wave_id(), lane = lane_id(), seg = lane / L, l = lane % L, E = a.E, k = a.k;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kPickThreads / kWave) * kTokens;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kPickThreads / kWave) + wave) * kTokens; t0 < a.T; t0 += step) {
+    const int64_t t = t0 + seg < a.T ? t0 + seg : a.T - 1;
+    const bool live = t0 + seg < a.T;
+    const S* row = reinterpret_cast<const S*>(a.logits) + t * a.ld;
+    float v[PL], m = 0.0f, z = 1.0f;
+    if (a.grad_dense) {
+      load_run<DT, PL>(a.logits, t * a.ld, l * PL, E, whole, v);
+      m = v[0];
+#pragma unroll
+      for (int i = 1; i < PL; ++i) m = fmaxf(m, v[i]);
+      m = max_over<L>(m);
+      z = 0.0f;
+#pragma unroll
+      for (int i = 0; i < PL; ++i) {
+        v[i] = v[i] == -__builtin_inff() ? 0.0f : expf(v[i] - m);
+        z += v[i];
+      }
+      z = sum_over<L>(z);
+    }
+    const int id = l < k ? a.ids[t * k + l] : -1;
+    const bool some = id >= 0 && id < E;
+    const float g = some ? a.scale * a.grad_w[t * k + l] : 0.0f;
+    const float x = some ? Elem<DT>::to_f32(row[id]) : -__builtin_inff();
+    float p, d, dot = 0.0f;
+    if (a.renorm) {
+      const float lead = a.sigmoid ? fminf(x, 0.0f) : x;
+      const float most = max_over<L>(some ? lead : -__builtin_inff());
+      p = some ? expf(lead - most) : 0.0f;
+      if (a.sigmoid && some) p = (x != x ? x : p) / (1.0f + expf(-fabsf(x)));
+      p = p / sum_over<L>(p);
+      dot = sum_over<L>(some ? p * g : 0.0f);
+      d = p * (g - dot);
+      if (a.sigmoid) d *= sigmoid_of(-x);
+    } else if (a.sigmoid) {
+      d = sigmoid_of(x) * sigmoid_of(-x) * g;
+    } else {
+      p = some ? expf(x - m) / z : 0.0f;
+      d = p * g;
+      dot = sum_over<L>(some ? d : 0.0f);
+    }
+    if (l < k) {
+      ds[wave][seg][l] = d;
+      es[wave][seg][l] = some ? id : -1;
+    }
+    wave_sync();
+    float o[PL];
+#pragma unroll
+    for (int i = 0; i < PL; ++i) o[i] = a.grad_dense ? (v[i] == 0.0f ? 0.0f : -(v[i] / z) * dot) : 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const int at = es[wave][seg][j] - l * PL;
+      const float dj = ds[wave][seg][j];
+#pragma unroll
+      for (int i = 0; i < PL; ++i) o[i] += at == i ? dj : 0.0f;
+    }
+    if (live) {
+      S* out = reinterpret_cast<S*>(a.grad) + t * E + l * PL;
+      if (whole) {
+        struct alignas(PL * sizeof(S) < 16 ? PL * sizeof(S) : 16) Run { S s[PL]; } r;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) r.s[i] = round_to<DT>(o[i]);
+        if (l * PL < E) *reinterpret_cast<Run*>(out) = r;
+      } else {
+#pragma unroll
+        for (int i = 0; i < PL; ++i)
+          if (l * PL + i < E) out[i] = round_to<DT>(o[i]);
+      }
+    }
+    wave_sync();
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+struct PickShape { int lanes, each; };
+
+PickShape pick_shape(int64_t E) {
+  if (E <= 16) return {16, 1};
+  if (E <= 64) return {16, 4};
+  if (E <= 128) return {16, 8};
+  if (E <= 256) return {16, 16};
+  if (E <= 512) return {64, 8};
+  return {64, 16};
+}
+
+struct PickPlan {
+  int waves, wave_tokens;
+  int64_t blocks, counts, totals, total;  // workgroups; offsets of the counts and the totals; bytes in all
+};
+
+PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
+  const int tokens = kWave / pick_shape(E).lanes;
+  PickPlan p{};
+  p.waves = kPickThreads / kWave;
+  const int64_t step = p.waves * tokens;                           // tokens that a workgroup takes at once
+  const int64_t most = std::max<int64_t>(1, kBlockPicks / (step * k));  // such steps whose ranks a workgroup can hold
+  int64_t steps = std::max<int64_t>(1, (T + 512 * step - 1) / (512 * step));
+  if (T * k <= kOneBlock) steps = (T + step - 1) / step;           // one workgroup
+  steps = std::max<int64_t>(1, std::min(steps, most));
+  p.wave_tokens = static_cast<int>(steps * tokens);
+  p.blocks = (T + steps * step - 1) / (steps * step);
+  p.totals = (p.blocks * (E + 1) * 4 + 255) / 256 * 256;
+  p.total = p.blocks > 1 ? p.totals + (E + 1) * 4 : 0;
+  return p;
+}
+
+bool whole_runs(const void* p, int64_t pitch, int64_t E, int64_t es, int each) {
+  const int64_t run = std::min<int64_t>(16, each * es);
+  return E % each == 0 && aligned_to(p, run) && pitch * es % run == 0;
+}
+
+template <int DT, int L, int PL>
+hipError_t launch_pick(const PickArgs& a, const PickPlan& p, bool whole, hipStream_t s) {
+  size_t lds = p.waves * sizeof(PickLds<L, PL>);
+  if (a.places) lds += (static_cast<size_t>(p.waves) + 1) * (a.E + 1) * 4 + static_cast<size_t>(p.waves) * p.wave_tokens * a.k * 4;
+  const unsigned blocks = static_cast<unsigned>(p.blocks);
+  const int threads = p.waves * kWave;
+  if (a.bias) pick_kernel<DT, L, PL, true><<<blocks, threads, lds, s>>>(a, whole);
+  else pick_kernel<DT, L, PL, false><<<blocks, threads, lds, s>>>(a, whole);
+  return hipGetLastError();
+}
+
+template <int DT, int L, int PL>
+hipError_t launch_pick_grad(const PickArgs& a, bool whole, hipStream_t s) {
+  const int64_t step = kPickThreads / L;
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.T + step - 1) / step, 2048));
+  pick_grad_kernel<DT, L, PL><<<blocks, kPickThreads, 0, s>>>(a, whole);
+  return hipGetLastError();
+}
+
+template <bool kGrad, int DT>
+hipError_t launch_typed(const PickArgs& a, const PickPlan& p, bool whole, hipStream_t s) {
+  const PickShape f = pick_shape(a.E);
+  auto go = [&](auto lanes, auto each) {
+    constexpr int L = decltype(lanes)::value, PL = decltype(each)::value;
+    if constexpr (kGrad) return launch_pick_grad<DT, L, PL>(a, whole, s);
+    else return launch_pick<DT, L, PL>(a, p, whole, s);
+  };
+  using std::integral_constant;
+  if (f.lanes == 16) {
+    switch (f.each) {
+      case 1: return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+      case 4: return go(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+      case 8: return go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+      default: return go(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+    }
+  }
+  return f.each == 8 ? go(integral_constant<int, 64>{}, integral_constant<int, 8>{}) : go(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+}
+
+template <bool kGrad>
+hipError_t launch_picks(int dtype, const PickArgs& a, const PickPlan& p, bool whole, hipStream_t s) {
+  switch (dtype) {
+    case kF32: return launch_typed<kGrad, kF32>(a, p, whole, s);
+    case kF16: return launch_typed<kGrad, kF16>(a, p, whole, s);
+    default: return launch_typed<kGrad, kBF16>(a, p, whole, s);
+  }
+}
+
+int check_picks(int64_t T, int64_t E, int64_t k, int dtype, int scoring) {
+  if (T < 0 || E <= 0 || k <= 0 || k > E || !known_dtype(dtype) || (scoring != SMX_SCORE_SOFTMAX && scoring != SMX_SCORE_SIGMOID))
+    return SMX_ERR_INVALID_ARG;
+  if (E > kMaxE || k > kMaxK || T > INT32_MAX / k) return SMX_ERR_UNSUPPORTED;
+  return SMX_OK;
+}
+
+}  // namespace
+}  // namespace smx
+
+using namespace smx;
+
+extern "C" {
+
+size_t smx_route_workspace_size(int64_t T, int64_t E, int64_t k) {
+  if (check_picks(T, E, k, kF32, SMX_SCORE_SOFTMAX) != SMX_OK) return 0;
+  return static_cast<size_t>(pick_plan(T, E, k).total);
+}
+
+int smx_route(const void* logits, int64_t logits_stride, int dtype, int64_t T, int64_t E, int64_t k, int scoring,
+              const float* bias, int64_t num_groups, int64_t top_groups, int renormalize, float scale, float* weights,
+              int32_t* ids, int32_t* places, int32_t* order, int64_t* offsets, void* workspace, size_t workspace_bytes,
+              void* stream) {
+  const int rc = check_picks(T, E, k, dtype, scoring);
+  if (rc != SMX_OK) return rc;
+  if (logits_stride < E || num_groups <= 0 || E % num_groups != 0 || top_groups <= 0 || top_groups > num_groups ||
+      k > E / num_groups * top_groups || !(scale - scale == 0.0f))
+    return SMX_ERR_INVALID_ARG;
+  if (num_groups > kMaxGroups) return SMX_ERR_UNSUPPORTED;
+  const bool ordered = places != nullptr;
+  if ((order != nullptr) != ordered && T > 0) return SMX_ERR_INVALID_ARG;
+  if (ordered && !offsets) return SMX_ERR_INVALID_ARG;
+  if (T > 0 && (!logits || !weights || !ids || (offsets && !ordered))) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype);
+  if (!aligned_to(logits, es) || !aligned_to(bias, 4) || !aligned_to(weights, 4) || !aligned_to(ids, 4) || !aligned_to(places, 4) ||
+      !aligned_to(order, 4) || !aligned_to(offsets, 8) || !aligned_to(workspace, 16))
+    return SMX_ERR_MISALIGNED;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const PickPlan p = pick_plan(T, E, k);
+  PickArgs a{};
+  a.T = T;
+  a.E = static_cast<int>(E);
+  a.k = static_cast<int>(k);
+  a.places = places;
+  a.order = order;
+  a.offsets = offsets;
+  a.ids = ids;
+  a.blocks = static_cast<int>(p.blocks);
+  if (ordered && p.total > 0) {
+    if (!workspace || workspace_bytes < static_cast<size_t>(p.total)) return SMX_ERR_WORKSPACE;
+    a.counts = static_cast<int32_t*>(workspace);
+    a.totals = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.totals);
+  }
+  if (T == 0) {
+    if (!offsets) return SMX_OK;
+    no_picks_kernel<<<static_cast<unsigned>((E + kPickThreads) / kPickThreads), kPickThreads, 0, s>>>(offsets, a.E + 1);
+    return static_cast<int>(hipGetLastError());
+  }
+  a.logits = static_cast<const char*>(logits);
+  a.ld = logits_stride;
+  a.ng = static_cast<int>(num_groups);
+  a.tg = static_cast<int>(top_groups);
+  a.gs = static_cast<int>(E / num_groups);
+  a.sigmoid = scoring == SMX_SCORE_SIGMOID;
+  a.renorm = renormalize != 0;
+  a.scale = scale;
+  a.bias = bias;
+  a.weights = weights;
+  a.wave_tokens = p.wave_tokens;
+  while ((E >> a.bits) != 0) ++a.bits;
+  hipError_t err = launch_picks<false>(dtype, a, p, whole_runs(logits, logits_stride, E, es, pick_shape(E).each), s);
+  if (err != hipSuccess || !ordered || p.blocks == 1) return static_cast<int>(err);
+  pick_scan_kernel<<<static_cast<unsigned>((E + 1 + kWave - 1) / kWave), kScanWaves * kWave, 0, s>>>(a);
+  err = hipGetLastError();
+  if (err != hipSuccess) return static_cast<int>(err);
+  const int64_t picks = T * k, per = std::max<int64_t>(kPickThreads, (picks + 2047) / 2048);
+  pick_place_kernel<<<static_cast<unsigned>((picks + per - 1) / per), kPickThreads, 0, s>>>(a, p.waves * p.wave_tokens, static_cast<int>(per));
+  return static_cast<int>(hipGetLastError());
+}
+
+int smx_route_grad(const float* grad_weights, const void* logits, int64_t logits_stride, int dtype, int64_t T, int64_t E,
+                   int64_t k, int scoring, int renormalize, float scale, const int32_t* ids, void* grad_logits, void* stream) {
+  const int rc = check_picks(T, E, k, dtype, scoring);
+  if (rc != SMX_OK) return rc;
+  if (logits_stride < E || !(scale - scale == 0.0f)) return SMX_ERR_INVALID_ARG;
+  if (T == 0) return SMX_OK;
+  if (!grad_weights || !logits || !ids || !grad_logits) return SMX_ERR_INVALID_ARG;
+  const int64_t es = dtype_bytes(dtype);
+  if (!aligned_to(logits, es) || !aligned_to(grad_logits, es) || !aligned_to(grad_weights, 4) || !aligned_to(ids, 4)) return SMX_ERR_MISALIGNED;
+  PickArgs a{};
+  a.T = T;
+  a.E = static_cast<int>(E);
+  a.k = static_cast<int>(k);
+  a.logits = static_cast<const char*>(logits);
+  a.ld = logits_stride;
+  a.sigmoid = scoring == SMX_SCORE_SIGMOID;
+  a.renorm = renormalize != 0;
+  a.grad_dense = !a.sigmoid && !a.renorm;
+  a.scale = scale;
+  a.ids = const_cast<int32_t*>(ids);
+  a.grad_w = grad_weights;
+  a.grad = static_cast<char*>(grad_logits);
+  const int each = pick_shape(E).each;
+  const bool whole = whole_runs(logits, logits_stride, E, es, each) && whole_runs(grad_logits, E, E, es, each);
+  return static_cast<int>(launch_picks<true>(dtype, a, PickPlan{}, whole, static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -7,10 +7,12 @@ from .fused_moe_kernel import (fp32_gemm_outputs_fp16, fused_down_max_tokens, fu
                                set_routing_in_gateup,
                                set_tiled_min_tokens, stack_fused_moe, stack_fused_moe_shared,
                                tiled_min_tokens)
+from .expert_rows import combine_rows, dispatch_rows
 from .linear import fused_linear, grouped_linear
-from .layernorm import RMSNorm, add_rmsnorm_gate
+from .layernorm import RMSNorm, add_rmsnorm_gate, layer_norm, rms_norm
 from .mixtral_moe import MixtralMoE
 from .moe_layer import PostAttentionMoE, moe_layer_forward
+from .routing import Routing, route_experts
 from .shared_moe import DeepseekV2MoE, Qwen2MoeSparseMoeBlock, SharedExpertMoE
 from .topk import fused_topk, grouped_topk, select_experts
 
@@ -20,6 +22,7 @@ __all__ = [
     "stack_fused_moe_shared", "MixtralMoE",
     "SharedExpertMoE", "Qwen2MoeSparseMoeBlock", "DeepseekV2MoE", "fused_topk", "grouped_topk",
     "select_experts", "fused_linear", "grouped_linear",
+    "layer_norm", "rms_norm", "route_experts", "Routing", "dispatch_rows", "combine_rows",
     "RMSNorm", "add_rmsnorm_gate", "PostAttentionMoE", "moe_layer_forward",
     "set_tiled_min_tokens", "tiled_min_tokens", "set_fused_down_max_tokens",
     "fused_down_max_tokens", "set_fp32_gemm_outputs_fp16", "fp32_gemm_outputs_fp16",

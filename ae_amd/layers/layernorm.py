@@ -1,10 +1,15 @@
-"""RMSNorm with the reference's interface, computed by the library's norm kernel.
+"""The norms: RMSNorm with the reference's interface, and layer_norm and rms_norm with gradients.
 
 Reference: specmoe/layers/layernorm.py:7-52. ``forward(x, residual=None)``: with a residual,
 ``residual = x + residual`` and ``x = rmsnorm(residual)`` are written in place and
 ``(x, residual)`` is returned (sglang's fused_add_rmsnorm, :31); without one, a new
 normalized tensor is returned. The arithmetic is the reference's forward_native (:36-52):
 fp32 sum, mean of squares, ``x * rsqrt(var + eps) * weight`` rounded once.
+
+RMSNorm and add_rmsnorm_gate serve: they take no part in differentiation. ``layer_norm`` and ``rms_norm``
+are the norms of a model that is trained (the reference has none). They write nothing in place, and
+normalise the sum as it is kept, rounded to its type, so that their gradients are those of the values the
+backward pass reads again.
 """
 from __future__ import annotations
 
@@ -14,7 +19,8 @@ import torch
 from torch import nn
 
 from .. import _lib
-from ._torch import dtype_code, ptr, require_gpu, stream_of
+from ._torch import (address, dtype_code, no_tangents, once, ptr, raw_stream, records_gradient, require_gpu,
+                     rows_of, stream_of, workspace)
 
 
 def add_rmsnorm_gate(hidden: torch.Tensor, residual: Optional[torch.Tensor],
@@ -72,3 +78,134 @@ class RMSNorm(nn.Module):
 
     def forward_native(self, *args, **kwargs):
         raise NotImplementedError("this build has no CPU RMSNorm path")
+
+
+def _check_norm(x, weight, bias, eps, residual):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must be [..., H], got {tuple(x.shape)}")
+    dtype_code(x.dtype)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    h = x.shape[-1:]
+    for name, t, shape in (("weight", weight, h), ("bias", bias, h), ("residual", residual, x.shape)):
+        if t is None:
+            continue
+        if t.shape != shape:
+            raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+        if t.device != x.device:
+            raise ValueError(f"x is on {x.device}, {name} on {t.device}")
+        if t.dtype != x.dtype and (t is residual or t.dtype != torch.float32):
+            raise TypeError(f"dtype mismatch: x is {x.dtype}, {name} {t.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"dtype mismatch: weight is {weight.dtype}, bias {bias.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"expected a GPU tensor, got one on {x.device}")
+
+
+def _params_dtype(weight, bias, dtype) -> int:
+    return dtype if weight is None and bias is None else dtype_code((bias if weight is None else weight).dtype)
+
+
+def _norm_forward(kind, x, weight, bias, eps, residual, keep: bool):
+    """y, the sum (None without a residual), and the rows' statistics where the gradient needs them."""
+    device = x.device
+    if device.index != torch.cuda.current_device():  # kernels are launched on the current device
+        with torch.cuda.device(device):
+            return _norm_forward(kind, x, weight, bias, eps, residual, keep)
+    h, dtype = x.shape[-1], dtype_code(x.dtype)
+    xm, xs = rows_of(x)
+    rm, rs = (None, 0) if residual is None else rows_of(residual)
+    rows = xm.numel() // h
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    stats = None
+    if keep:
+        stats = torch.empty(rows if kind == _lib.SMX_NORM_RMS else 2 * rows, dtype=torch.float32, device=device)
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    code = _lib.lib().smx_norm(
+        kind, xm.data_ptr(), xs, address(rm), rs, dtype, rows, h, address(w), address(b),
+        _params_dtype(weight, bias, dtype), eps, y.data_ptr(), address(total), address(stats), raw_stream(device.index))
+    if code:
+        _lib.check("smx_norm", code)
+    return y, total, stats
+
+
+def _norm_backward(kind, dy, dsum, s, weight, stats, params, need):
+    device = s.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _norm_backward(kind, dy, dsum, s, weight, stats, params, need)
+    need_x, need_w, need_b = need
+    h, dtype = s.shape[-1], dtype_code(s.dtype)
+    if dy is None:  # only the sum was used
+        zeros = [torch.zeros(h, dtype=params, device=device) if n else None for n in (need_w, need_b)]
+        return dsum if need_x else None, *zeros
+    sm, ss = rows_of(s)
+    dm, ds = rows_of(dy)
+    rm, rs = (None, 0) if dsum is None else rows_of(dsum)
+    rows = sm.numel() // h
+    dx = torch.empty(s.shape, dtype=s.dtype, device=device) if need_x else None
+    dw = torch.empty(h, dtype=params, device=device) if need_w else None
+    db = torch.empty(h, dtype=params, device=device) if need_b else None
+    ws, nbytes = None, 0
+    if need_w or need_b:
+        nbytes = _lib.lib().smx_norm_grad_workspace_size(kind, rows, h, dtype)
+        ws = workspace(nbytes, device)
+    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    code = _lib.lib().smx_norm_grad(
+        kind, dm.data_ptr(), ds, address(rm), rs, sm.data_ptr(), ss, dtype, rows, h, address(w), dtype_code(params),
+        stats.data_ptr(), address(dx), address(dw), address(db), address(ws), nbytes, raw_stream(device.index))
+    if code:
+        _lib.check("smx_norm_grad", code)
+    return dx, dw, db
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, kind, eps):
+        y, total, stats = _norm_forward(kind, x, weight, bias, eps, residual, True)
+        ctx.save_for_backward(x if total is None else total, weight, stats)
+        ctx.kind = kind
+        ctx.params = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+        ctx.set_materialize_grads(False)
+        return y if total is None else (y, total)
+
+    @staticmethod
+    def backward(ctx, dy, dsum=None):
+        no_tangents("a norm", dy, dsum)
+        if dy is None and dsum is None:
+            return (None,) * 6
+        s, weight, stats = ctx.saved_tensors  # as autograd hands them back: perhaps not at their old addresses
+        x, w, b, r = ctx.needs_input_grad[:4]
+        dx, dw, db = once("a norm", lambda: _norm_backward(ctx.kind, dy, dsum, s, weight, stats, ctx.params,
+                                                           (x or r, w, b)), (dy, dsum, s, weight))
+        return dx if x else None, dw, db, dx if r else None, None, None
+
+
+def _norm(kind, x, weight, bias, eps, residual):
+    no_tangents("a norm", x, weight, bias, residual)
+    eps = float(eps)
+    _check_norm(x, weight, bias, eps, residual)
+    if records_gradient(x, weight, bias, residual):
+        return _Norm.apply(x, weight, bias, residual, kind, eps)
+    y, total, _ = _norm_forward(kind, x, weight, bias, eps, residual, False)
+    return y if total is None else (y, total)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, residual: Optional[torch.Tensor] = None
+               ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``(s - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (at most 16384 columns), of
+    ``s = x``, or with a residual of ``s = x + residual``: then ``(y, s)`` is returned, s as it is kept.
+
+    x and residual ``[..., H]`` in fp32, fp16 or bf16; weight and bias ``[H]`` in x's type or fp32, or None.
+    Statistics and sums are fp32, y is rounded once. Differentiable once, in reverse mode, in x, weight,
+    bias and residual; the gradients of weight and bias are summed in fp32, in a fixed order."""
+    return _norm(_lib.SMX_NORM_LAYER, x, weight, bias, eps, residual)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``s / sqrt(mean(s^2) + eps) * weight``; otherwise as layer_norm."""
+    return _norm(_lib.SMX_NORM_RMS, x, weight, None, eps, residual)
