@@ -69,10 +69,6 @@ __device__ __forceinline__ uint64_t key_of(double v) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
   return (u >> 63) ? ~u : (u | (uint64_t{1} << 63));
 }
-__device__ __forceinline__ double value_of(uint64_t k) {
-  if (k == 0u) return -__builtin_inf();
-  return __builtin_bit_cast(double, (k >> 63) ? (k & ~(uint64_t{1} << 63)) : ~k);
-}
 
 template <int L> __device__ __forceinline__ float sum_over(float v) {
   return group_reduce<L>(v, [](float a, float b) { return a + b; });
@@ -154,26 +150,33 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) z += __shfl_xor(z, off, kWave);
   }
-  for (int e = lane; e < a.E; e += kWave) {
+  auto score = [&](int e) {
     const double x = Elem<DT>::to_f32(row[e]);
-    const double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - m) / z;
-    key[e] = x == -__builtin_inf() ? 0u : key_of(s + static_cast<double>(a.bias[e]));
-  }
+    return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - m) / z;
+  };
+  for (int e = lane; e < a.E; e += kWave)
+    key[e] = Elem<DT>::to_f32(row[e]) == -__builtin_inff() ? 0u : key_of(score(e) + static_cast<double>(a.bias[e]));
   wave_sync();
   if (a.tg < a.ng) {
     uint64_t mine = 0u;
     if (lane < a.ng) {
       uint64_t best = 0u, next = 0u;
-      for (int i = 0; i < a.gs; ++i) {
-        const uint64_t c = key[lane * a.gs + i];
-        if (c > best) {
+      int at = 0, after = 0;
+      for (int i = lane * a.gs; i < (lane + 1) * a.gs; ++i) {
+        if (key[i] > best) {
           next = best;
-          best = c;
-        } else if (c > next) {
-          next = c;
+          after = at;
+          best = key[i];
+          at = i;
+        } else if (key[i] > next) {
+          next = key[i];
+          after = i;
         }
       }
-      mine = best == 0u ? 0u : key_of(value_of(best) + (next == 0u ? 0.0 : value_of(next)));
+      // scores and biases each on their own: the sums of biases are exact, so groups that tie tie here
+      mine = best;
+      if (next != 0u)
+        mine = key_of((score(at) + score(after)) + (static_cast<double>(a.bias[at]) + static_cast<double>(a.bias[after])));
     }
     int before = 0;
     for (int g = 0; g < a.ng; ++g) {
@@ -390,6 +393,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       s = some ? expf(lead - most) : 0.0f;
       if (a.sigmoid && some) s = (x != x ? x : s) / (1.0f + expf(-fabsf(x)));
       s = s / sum_over<L>(s);
+      if (kBiased && !a.sigmoid && z != z) s = z;  // (of a NaN score nobody need be picked)
     } else {
       s = a.sigmoid ? sigmoid_of(x) : expf(x - m) / z;
     }
