@@ -32,11 +32,13 @@ template <int DT, bool kVec> struct Part {
   int col, step, H;
 
   __device__ __forceinline__ bool in(int j) const { return col + j * step < H; }
-  __device__ __forceinline__ Chunk<DT> load(const char* base, int64_t row, int64_t ld) const {
+  // kOnce: nothing else reads it soon, so it takes no room in the caches (measured at combine_kernel).
+  template <bool kOnce = false> __device__ __forceinline__ Chunk<DT> load(const char* base, int64_t row, int64_t ld) const {
     const S* p = reinterpret_cast<const S*>(base) + row * ld + col;
     Chunk<DT> r;
     if constexpr (kVec) {
-      r = __builtin_bit_cast(Chunk<DT>, *reinterpret_cast<const u32x4*>(p));
+      const u32x4* q = reinterpret_cast<const u32x4*>(p);
+      r = __builtin_bit_cast(Chunk<DT>, kOnce ? __builtin_nontemporal_load(q) : *q);
     } else {
 #pragma unroll
       for (int j = 0; j < kN; ++j) r.e[j] = in(j) ? p[j * step] : S{};
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(MoveArgs a) {
       if (p[i] >= a.picks) p[i] = -1;
       w[i] = p[i] >= 0 && a.weights != nullptr ? a.weights[t * a.k + j0 + i] : 1.0f;
       r[i] = Chunk<DT>{};
-      if (p[i] >= 0) r[i] = part.load(a.rows, p[i], a.rows_ld);
+      if (p[i] >= 0) r[i] = part.template load<true>(a.rows, p[i], a.rows_ld);
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -135,38 +137,44 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(MoveArgs a) {
   }
 }
 
-// The same with the products <rows[places[t, j]], x[t]>: the row's threads walk over its columns, and add up in the end.
+// The same with the products <rows[places[t, j]], x[t]>: TPR threads walk over a token's columns, and add up in the end. A
+// wave has one token, so that its places, weights and row addresses are scalars.
+template <int TPR> constexpr int grad_threads() { return TPR == kWave ? kThreads : TPR; }
+
 template <int DT, bool kVec, int TPR, int K>
-__global__ __launch_bounds__(kThreads) void combine_grad_kernel(MoveArgs a) {
+__global__ __launch_bounds__(grad_threads<TPR>()) void combine_grad_kernel(MoveArgs a) {
   constexpr int kN = Chunk<DT>::kN;
   using Sum = RowSum<TPR, K>;
   __shared__ typename Sum::Lds lds;
   int turn = 0;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / TPR) + threadIdx.x / TPR;
+  const int64_t t = TPR == kWave ? static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + wave_id() : blockIdx.x;
   const int tid = static_cast<int>(threadIdx.x) % TPR;
-  if (TPR <= kWave && t >= a.T) return;  // (whole waves; with TPR > kWave a workgroup has one token)
-  int32_t p[K];
+  if (t >= a.T) return;  // (whole waves; with TPR > kWave there is a workgroup a token)
+  int p[K];
   float w[K], dot[K];
 #pragma unroll
   for (int j = 0; j < K; ++j) {
-    p[j] = j < a.k ? a.places[t * a.k + j] : -1;
-    w[j] = j < a.k ? a.weights == nullptr ? 1.0f : a.weights[t * a.k + j] : 0.0f;
+    p[j] = j < a.k ? __builtin_amdgcn_readfirstlane(a.places[t * a.k + j]) : INT32_MAX;
+    w[j] = 1.0f;
+    if (a.weights != nullptr && j < a.k)
+      w[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(a.weights[t * a.k + j])));
     dot[j] = 0.0f;
   }
+  const int picks = static_cast<int>(a.picks);
   for (int first = 0; first < a.H; first += TPR * kN) {
-    Part<DT, kVec> part{kVec ? first + tid * kN : first + tid, kVec ? 1 : TPR, a.H};
+    const Part<DT, kVec> part{kVec ? first + tid * kN : first + tid, kVec ? 1 : TPR, a.H};
     if (part.col >= a.H) break;
     const Chunk<DT> x = part.load(a.x, t, a.x_ld);
     Chunk<DT> r[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       r[j] = Chunk<DT>{};
-      if (p[j] >= 0 && p[j] < a.picks) r[j] = part.load(a.rows, p[j], a.rows_ld);
+      if (p[j] >= 0 && p[j] < picks) r[j] = part.template load<true>(a.rows, p[j], a.rows_ld);
     }
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int32_t q = p[j] < 0 ? ~p[j] : p[j];
-      if (j >= a.k || q >= a.picks) continue;
+      const int q = p[j] < 0 ? ~p[j] : p[j];
+      if (q >= picks) continue;
       Chunk<DT> o{};
       if (p[j] >= 0) {
 #pragma unroll
@@ -233,19 +241,26 @@ hipError_t launch_spread(int dtype, bool vec, MoveArgs& a, hipStream_t s) {
 
 template <int DT, bool kVec, int TPR>
 hipError_t launch_grad_picks(const MoveArgs& a, hipStream_t s) {
-  const unsigned n = static_cast<unsigned>((a.T + kThreads / TPR - 1) / (kThreads / TPR));
-  if (a.k <= 2) combine_grad_kernel<DT, kVec, TPR, 2><<<n, kThreads, 0, s>>>(a);
-  else if (a.k <= 4) combine_grad_kernel<DT, kVec, TPR, 4><<<n, kThreads, 0, s>>>(a);
-  else if (a.k <= 8) combine_grad_kernel<DT, kVec, TPR, 8><<<n, kThreads, 0, s>>>(a);
-  else combine_grad_kernel<DT, kVec, TPR, 16><<<n, kThreads, 0, s>>>(a);
+  constexpr int threads = grad_threads<TPR>(), tokens = threads / TPR;
+  const unsigned n = static_cast<unsigned>((a.T + tokens - 1) / tokens);
+  if (a.k <= 2) combine_grad_kernel<DT, kVec, TPR, 2><<<n, threads, 0, s>>>(a);
+  else if (a.k <= 4) combine_grad_kernel<DT, kVec, TPR, 4><<<n, threads, 0, s>>>(a);
+  else if (a.k <= 8) combine_grad_kernel<DT, kVec, TPR, 8><<<n, threads, 0, s>>>(a);
+  else combine_grad_kernel<DT, kVec, TPR, 16><<<n, threads, 0, s>>>(a);
   return hipGetLastError();
+}
+
+template <int DT, bool kVec>
+hipError_t launch_grad_shape(const MoveArgs& a, hipStream_t s) {
+  const int64_t chunks = (a.H * dtype_bytes(DT) + 15) / 16;
+  if (chunks <= 64) return launch_grad_picks<DT, kVec, 64>(a, s);
+  if (chunks <= 128) return launch_grad_picks<DT, kVec, 128>(a, s);
+  return launch_grad_picks<DT, kVec, 256>(a, s);
 }
 
 template <int DT>
 hipError_t launch_grad(bool vec, const MoveArgs& a, hipStream_t s) {
-  // a workgroup a token where there are too few tokens to fill the chip with a wave each
-  if (a.T <= 2048) return vec ? launch_grad_picks<DT, true, 256>(a, s) : launch_grad_picks<DT, false, 256>(a, s);
-  return vec ? launch_grad_picks<DT, true, 64>(a, s) : launch_grad_picks<DT, false, 64>(a, s);
+  return vec ? launch_grad_shape<DT, true>(a, s) : launch_grad_shape<DT, false>(a, s);
 }
 
 }  // namespace

@@ -8,7 +8,8 @@ namespace {
 
 constexpr int kMaxNorm = 16384;     // columns
 constexpr int kSmallBlock = 256;    // threads of a workgroup that holds several rows
-constexpr int kFoldWaves = 16;      // waves of a workgroup that adds up the partial weight gradients
+constexpr int kFoldThreads = 1024;  // of a workgroup that adds up the partial weight gradients
+constexpr int kFoldCols = 32;       // its columns
 
 struct NormArgs {
   const char* x;         // forward: x; backward: s
@@ -233,26 +234,27 @@ __global__ __launch_bounds__(block_threads<TPR>()) void norm_grad_kernel(NormArg
   }
 }
 
-// Column sums of part [2][parts][H] into the gradients of the weight (plane 0) and the bias (plane 1): a workgroup takes 64
-// columns, its waves a share of the parts each.
+// Column sums of part [2][parts][H] into the gradients of the weight (plane 0) and the bias (plane 1): a workgroup takes
+// kFoldCols columns, its threads of a column a share of the parts each.
 template <int DT>
-__global__ __launch_bounds__(kFoldWaves * kWave) void norm_fold_kernel(const float* part, int parts, int H, char* grad_weight,
-                                                                     char* grad_bias) {
-  __shared__ float lds[kFoldWaves][kWave];
-  const int wave = wave_id(), lane = lane_id(), col = static_cast<int>(blockIdx.x) * kWave + lane;
+__global__ __launch_bounds__(kFoldThreads) void norm_fold_kernel(const float* part, int parts, int H, char* grad_weight, char* grad_bias) {
+  constexpr int kShares = kFoldThreads / kFoldCols;
+  __shared__ float lds[kShares][kFoldCols];
+  const int lane = static_cast<int>(threadIdx.x) % kFoldCols, share = static_cast<int>(threadIdx.x) / kFoldCols;
+  const int col = static_cast<int>(blockIdx.x) * kFoldCols + lane;
   char* out = blockIdx.y == 0 ? grad_weight : grad_bias;
   if (out == nullptr) return;
   const float* p = part + static_cast<int64_t>(blockIdx.y) * parts * H;
   float t = 0.0f;
   if (col < H) {
-#pragma unroll 8
-    for (int i = wave; i < parts; i += kFoldWaves) t += p[static_cast<int64_t>(i) * H + col];
+#pragma unroll 16
+    for (int i = share; i < parts; i += kShares) t += p[static_cast<int64_t>(i) * H + col];
   }
-  lds[wave][lane] = t;
+  lds[share][lane] = t;
   __syncthreads();
-  if (wave != 0 || col >= H) return;
+  if (share != 0 || col >= H) return;
 #pragma unroll
-  for (int w = 1; w < kFoldWaves; ++w) t += lds[w][lane];
+  for (int w = 1; w < kShares; ++w) t += lds[w][lane];
   reinterpret_cast<typename Elem<DT>::S*>(out)[col] = round_to<DT>(t);
 }
 
@@ -285,7 +287,7 @@ int64_t forward_blocks(const NormShape& s, int64_t rows) {
 // Of the backward pass: fewer, since each leaves its partial weight gradients.
 int64_t grad_blocks(const NormShape& s, int64_t rows) {
   const int64_t threads = std::max(s.tpr, kSmallBlock);
-  return std::min((rows + rows_at_once(s) - 1) / rows_at_once(s), int64_t{256} * 1024 / threads);
+  return std::min((rows + 4 * rows_at_once(s) - 1) / (4 * rows_at_once(s)), int64_t{256} * 1024 / threads);
 }
 
 int check_norm(int kind, int64_t rows, int64_t H, int dtype) {
@@ -429,15 +431,15 @@ int smx_norm_grad(int kind, const void* grad_y, int64_t grad_y_stride, const voi
     if (err != hipSuccess) return static_cast<int>(err);
   }
   if (sums) {
-    const dim3 grid(static_cast<unsigned>((H + kWave - 1) / kWave), grad_bias ? 2 : 1);
+    const dim3 grid(static_cast<unsigned>((H + kFoldCols - 1) / kFoldCols), grad_bias ? 2 : 1);
     const float* part = static_cast<const float*>(workspace);
     const int parts = rows > 0 ? static_cast<int>(blocks) : 0, n = static_cast<int>(H);
     char* gw = static_cast<char*>(grad_weight);
     char* gb = static_cast<char*>(grad_bias);
     switch (weight_dtype) {
-      case kF32: norm_fold_kernel<kF32><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
-      case kF16: norm_fold_kernel<kF16><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
-      default: norm_fold_kernel<kBF16><<<grid, kFoldWaves * kWave, 0, st>>>(part, parts, n, gw, gb); break;
+      case kF32: norm_fold_kernel<kF32><<<grid, kFoldThreads, 0, st>>>(part, parts, n, gw, gb); break;
+      case kF16: norm_fold_kernel<kF16><<<grid, kFoldThreads, 0, st>>>(part, parts, n, gw, gb); break;
+      default: norm_fold_kernel<kBF16><<<grid, kFoldThreads, 0, st>>>(part, parts, n, gw, gb); break;
     }
     return static_cast<int>(hipGetLastError());
   }

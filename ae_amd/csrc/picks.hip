@@ -4,7 +4,7 @@
 //   pick_kernel        L lanes a token with PL experts each: scores, groups, the k best, their weights; and where order
 //                      is asked for, each pick's rank among the picks of its expert in the workgroup's tokens, with the
 //                      workgroup's counts per expert. One workgroup does it all for few tokens.
-//   pick_scan_kernel   counts per workgroup and expert -> the picks of an expert before a workgroup's
+//   pick_scan_kernel   many workgroups: counts per workgroup and expert -> the picks of an expert before a workgroup's
 //   pick_place_kernel  place = the expert's first + those before the workgroup's + the rank
 //   pick_grad_kernel   the gradient of a token's logits
 //
@@ -16,13 +16,15 @@
 namespace smx {
 namespace {
 
-constexpr int kPickThreads = 256;
+constexpr int kPickThreads = 512;     // most of a workgroup that picks
+constexpr int kGradThreads = 256;
+constexpr int kPlaceThreads = 1024;
 constexpr int kMaxK = 16;
 constexpr int kMaxE = 1024;
 constexpr int kMaxGroups = 64;
-constexpr int kEntry = kMaxK + 1;     // slots of a token's picks: one more, whose distance is looked at
-constexpr int kBlockPicks = 2048;     // picks whose ranks a workgroup holds
-constexpr int kScanWaves = 16;
+constexpr int kEntry = kMaxK + 2;     // slots of a token's picks: two more, whose distances are looked at
+constexpr int kBlockPicks = 1024;     // picks whose ranks a workgroup holds
+constexpr int kScanCols = 16;         // experts of a workgroup that scans
 constexpr int kOneBlock = 512;        // picks that one workgroup sorts by itself
 
 struct PickArgs {
@@ -37,10 +39,11 @@ struct PickArgs {
   int32_t* places;     // null: no order
   int32_t* order;
   int64_t* offsets;
-  int32_t* counts;     // [blocks][E + 1] picks of the workgroup per expert (E: of nobody)
+  int32_t* counts;     // [blocks][pitch] picks of the workgroup per expert (E: of nobody)
   int32_t* totals;     // [E + 1]
   int wave_tokens;     // consecutive tokens of a wave
-  int blocks;
+  int blocks, pitch;
+  bool scanned;        // counts hold the picks before the workgroup's by now
   int bits;            // of an expert's number, E among them
   const float* grad_w;
   char* grad;
@@ -112,14 +115,22 @@ __device__ __forceinline__ float sigmoid_of(float x) {
   return (x < 0.0f ? e : 1.0f) / (1.0f + e);  // NaN stays NaN
 }
 
+// The same and exp for comparisons only: an instruction each, off by |x| 2^-23 and 2^-22 of themselves.
+__device__ __forceinline__ float quick_exp(float x) { return __builtin_amdgcn_exp2f(x * 0x1.715476p+0f); }
+__device__ __forceinline__ float quick_sigmoid(float x) {
+  const float e = quick_exp(-fabsf(x));
+  return (x < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 // LDS of a wave: the picks of its tokens, their keys; the choices of its tokens by key while groups are compared,
-// or those of one token in 64 bits; the picks per expert so far.
+// or the listed ones in 64 bits, or those of one token.
 template <int L, int PL> struct PickLds {
   static constexpr int kTokens = kWave / L;
   int entry[kTokens * kEntry];
   uint32_t key[kTokens * kEntry];
   union {
-    uint32_t choice[kTokens][L * PL];
+    uint64_t fine[kTokens * kEntry];        // the listed choices in 64 bits
+    uint32_t choice[kTokens][L * PL + 16];  // (tokens begin in other banks)
     uint64_t exact[L * PL];
   };
   uint32_t group[kTokens][kMaxGroups];
@@ -132,13 +143,9 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
   using S = typename Elem<DT>::S;
   const int lane = lane_id();
   const S* row = reinterpret_cast<const S*>(a.logits) + t * a.ld;
-  auto top_of = [](uint64_t k) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const uint64_t o = __shfl_xor(k, off, kWave);
-      k = o > k ? o : k;
-    }
-    return k;
+  auto top_of = [](uint64_t v) {  // the wave's largest: the upper halves first
+    const uint32_t high = static_cast<uint32_t>(v >> 32), top = max_over<kWave>(high);
+    return static_cast<uint64_t>(top) << 32 | max_over<kWave>(high == top ? static_cast<uint32_t>(v) : 0u);
   };
   double m = 0.0, z = 1.0;
   if (!a.sigmoid) {
@@ -162,14 +169,16 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
     if (lane < a.ng) {
       uint64_t best = 0u, next = 0u;
       int at = 0, after = 0;
-      for (int i = lane * a.gs; i < (lane + 1) * a.gs; ++i) {
-        if (key[i] > best) {
+      for (int j = 0, r = lane % a.gs; j < a.gs; ++j, r = r + 1 == a.gs ? 0 : r + 1) {  // (each lane from another bank on)
+        const int i = lane * a.gs + r;
+        const uint64_t c = key[i];
+        if (c > best) {
           next = best;
           after = at;
-          best = key[i];
+          best = c;
           at = i;
-        } else if (key[i] > next) {
-          next = key[i];
+        } else if (c > next) {
+          next = c;
           after = i;
         }
       }
@@ -180,7 +189,8 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
     }
     int before = 0;
     for (int g = 0; g < a.ng; ++g) {
-      const uint64_t o = __shfl(mine, g, kWave);
+      const uint64_t o = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), g))) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), g));
       before += o > mine || (o == mine && g < lane);
     }
     const uint64_t kept = ballot(lane < a.ng && before < a.tg);
@@ -198,9 +208,7 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
       }
     const uint64_t top = top_of(best);
     // ties: the lowest expert
-    int low = top != 0u && best == top ? at : a.E;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) low = min(low, __shfl_xor(low, off, kWave));
+    const int low = static_cast<int>(~max_over<kWave>(top != 0u && best == top ? ~static_cast<uint32_t>(at) : ~static_cast<uint32_t>(a.E)));
     if (low < a.E && at == low && best == top) key[at] = 0u;
     if (lane == 0) entry[j] = low;
     wave_sync();
@@ -245,11 +253,10 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
   }
   float b[PL], far = 0.0f;  // the largest finite bias
   if constexpr (kBiased) {
+    load_run<kF32, PL>(reinterpret_cast<const char*>(a.bias), 0, l * PL, E, whole && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0, b);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      b[i] = l * PL + i < E ? a.bias[l * PL + i] : 0.0f;
+    for (int i = 0; i < PL; ++i)
       if (fabsf(b[i]) < __builtin_inff()) far = fmaxf(far, fabsf(b[i]));
-    }
     far = max_over<L>(far);
   }
   const int64_t block_first = static_cast<int64_t>(blockIdx.x) * waves * a.wave_tokens;
@@ -274,71 +281,116 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       for (int i = 0; i < PL; ++i) z += l * PL + i < E ? expf(v[i] - m) : 0.0f;
       z = sum_over<L>(z);
     }
+    const float rz = 1.0f / z;
     uint32_t key[PL];
 #pragma unroll
     for (int i = 0; i < PL; ++i) {
       if constexpr (kBiased) {
-        const float s = a.sigmoid ? sigmoid_of(v[i]) : expf(v[i] - m) / z;
+        const float s = a.sigmoid ? quick_sigmoid(v[i]) : quick_exp(v[i] - m) * rz;
         key[i] = v[i] == -__builtin_inff() ? 0u : key_of(s + b[i]);
       } else {
         key[i] = key_of(v[i]);
       }
     }
-    bool close = false;  // choices too near for 32 bits
+    bool close = false;  // groups too near for 32 bits
     if (a.tg < a.ng) {
-#pragma unroll
-      for (int i = 0; i < PL; ++i) lds.choice[seg][l * PL + i] = key[i];
-      wave_sync();
-      for (int g = l; g < a.ng; g += L) {
-        uint32_t best = 0u, next = 0u;
-        for (int i = 0; i < a.gs; ++i) {
-          const uint32_t c = lds.choice[seg][g * a.gs + i];
-          if (kBiased && c <= best) next = c > next ? c : next;
-          if (kBiased && c > best) next = best;
-          best = c > best ? c : best;
-        }
-        if (kBiased && best != 0u && next != 0u) best = key_of(value_of(best) + value_of(next));
-        lds.group[seg][g] = best;
-      }
-      wave_sync();
       uint64_t kept = 0u;
       float low = __builtin_inff(), high = -__builtin_inff();
-      for (int g0 = 0; g0 < a.ng; g0 += L) {
-        const int g = g0 + l;
-        bool keep = false;
-        if (g < a.ng) {
-          const uint32_t c = lds.group[seg][g];
-          int before = 0;
-          for (int o = 0; o < a.ng; ++o) {
-            const uint32_t other = lds.group[seg][o];
-            before += other > c || (other == c && o < g);
-          }
-          keep = before < a.tg;
-          if (keep) low = fminf(low, value_of(c));
-          else high = fmaxf(high, value_of(c));
+      const int share = a.gs / PL;  // lanes of a group
+      if (L == 16 && share * PL == a.gs && (share & (share - 1)) == 0) {
+        // whole lanes a group: the two best of each lane's, joined over the group's lanes, and ranked over the token's
+        uint32_t best = key[0], next = 0u;
+#pragma unroll
+        for (int i = 1; i < PL; ++i) {
+          const uint32_t less = best < key[i] ? best : key[i];
+          next = next > less ? next : less;
+          best = best > key[i] ? best : key[i];
         }
-        const uint64_t bitsv = ballot(keep);
-        kept |= (L == kWave ? bitsv : (bitsv >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1)) << g0;
+        auto join = [&](auto ctrl) {
+          const uint32_t ob = static_cast<uint32_t>(dpp<decltype(ctrl)::value>(static_cast<int>(best)));
+          const uint32_t on = static_cast<uint32_t>(dpp<decltype(ctrl)::value>(static_cast<int>(next)));
+          const uint32_t less = best < ob ? best : ob;
+          next = next > on ? next : on;
+          next = next > less ? next : less;
+          best = best > ob ? best : ob;
+        };
+        using std::integral_constant;
+        if (share >= 2) join(integral_constant<int, kDppXor1>{});
+        if (share >= 4) join(integral_constant<int, kDppXor2>{});
+        if (share >= 8) join(integral_constant<int, kDppHalfMirror>{});
+        if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
+        int before = 0;  // lanes whose group comes first
+        auto turn = [&](auto steps) {
+          constexpr int kRor = 0x120 + decltype(steps)::value;  // row_ror: lane i has lane i - steps'
+          const uint32_t other = static_cast<uint32_t>(dpp<kRor>(static_cast<int>(best)));
+          const bool lower = dpp<kRor>(l) < l;
+          before += other > best || (lower && other == best);
+        };
+        turn(integral_constant<int, 1>{}); turn(integral_constant<int, 2>{}); turn(integral_constant<int, 3>{});
+        turn(integral_constant<int, 4>{}); turn(integral_constant<int, 5>{}); turn(integral_constant<int, 6>{});
+        turn(integral_constant<int, 7>{}); turn(integral_constant<int, 8>{}); turn(integral_constant<int, 9>{});
+        turn(integral_constant<int, 10>{}); turn(integral_constant<int, 11>{}); turn(integral_constant<int, 12>{});
+        turn(integral_constant<int, 13>{}); turn(integral_constant<int, 14>{}); turn(integral_constant<int, 15>{});
+        // (a lane counts lower lanes of its own group too: fewer than `share`)
+        const bool real = l * PL < E, keep = (before >> __builtin_ctz(share)) < a.tg;
+        if (real && keep) low = value_of(best);
+        if (real && !keep) high = value_of(best);
+        if (!keep) {
+#pragma unroll
+          for (int i = 0; i < PL; ++i) key[i] = 0u;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < PL; ++i) lds.choice[seg][l * PL + i] = key[i];
+        wave_sync();
+        for (int g = l; g < a.ng; g += L) {
+          uint32_t best = 0u, next = 0u;
+          for (int i = 0, r = l % a.gs; i < a.gs; ++i, r = r + 1 == a.gs ? 0 : r + 1) {  // (each lane from another bank on)
+            const uint32_t c = lds.choice[seg][g * a.gs + r], less = best < c ? best : c;
+            next = next > less ? next : less;
+            best = best > c ? best : c;
+          }
+          if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
+          lds.group[seg][g] = best;
+        }
+        wave_sync();
+        for (int g0 = 0; g0 < a.ng; g0 += L) {
+          const int g = g0 + l;
+          bool keep = false;
+          if (g < a.ng) {
+            const uint32_t c = lds.group[seg][g];
+            int before = 0;
+            for (int o = 0; o < a.ng; ++o) {
+              const uint32_t other = lds.group[seg][o];
+              before += other > c || (other == c && o < g);
+            }
+            keep = before < a.tg;
+            if (keep) low = fminf(low, value_of(c));
+            else high = fmaxf(high, value_of(c));
+          }
+          const uint64_t bits = ballot(keep);
+          kept |= (L == kWave ? bits : (bits >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1)) << g0;
+        }
+        int g = l * PL / a.gs, rest = l * PL - g * a.gs;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+          if (!((kept >> (g & 63)) & 1u)) key[i] = 0u;
+          if (++rest == a.gs) {
+            rest = 0;
+            ++g;
+          }
+        }
+        wave_sync();
       }
       if constexpr (kBiased) {
         low = -max_over<L>(-low);
         high = max_over<L>(high);
-        // a group's choice is the sum of two scores, each off by 2^-18 at most, and of two biases; three roundings
-        if (low - high <= 0x1p-16f + 0x1p-21f * far) close = true;
+        // a group's choice is the sum of two scores, each off by 2^-18 at most (a sigmoid by 2^-21), and of two biases; three
+        // roundings
+        if (low - high <= (a.sigmoid ? 0x1p-19f : 0x1p-16f) + 0x1p-21f * far) close = true;
       }
-      const int e0 = l * PL;
-      int g = e0 / a.gs, rest = e0 - g * a.gs;
-#pragma unroll
-      for (int i = 0; i < PL; ++i) {
-        if (!((kept >> (g & 63)) & 1u)) key[i] = 0u;
-        if (++rest == a.gs) {
-          rest = 0;
-          ++g;
-        }
-      }
-      wave_sync();
     }
-    const int rounds = k + (kBiased ? 1 : 0);
+    const int rounds = k + (kBiased ? 2 : 0);
     for (int j = 0; j < rounds; ++j) {
       uint32_t top = key[0];
 #pragma unroll
@@ -361,18 +413,47 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
     using S = typename Elem<DT>::S;
     const S* row = reinterpret_cast<const S*>(a.logits) + at;
     if constexpr (kBiased) {
-      if (l < k) {
-        const int e = entry[l], n = entry[l + 1];
-        if (e < E && n < E) {
-          const float x = Elem<DT>::to_f32(row[e]), y = Elem<DT>::to_f32(row[n]), p = a.bias[e], q = a.bias[n];
-          const float c = value_of(ekey[l]), d = value_of(ekey[l + 1]);
-          // a score is off by 16 roundings of itself and by those of exp's argument, a choice by one more
-          const float off = fabsf(c - p) * (0x1p-19f + 0x1p-22f * fabsf(x - m)) + fabsf(d - q) * (0x1p-19f + 0x1p-22f * fabsf(y - m)) +
-                            0x1p-22f * (fabsf(c) + fabsf(d)) + 1e-37f;
-          if (c - d <= off && !(x == y && p == q)) close = true;
+      // Which neighbours in the order 32 bits cannot tell apart: pick l and l + 1, and lane 0 that behind the last too.
+      const int listing = k < L ? k + 1 : L;  // entries that have a lane
+      const int e = l < listing ? entry[l] : E;
+      auto near = [&](int j) {
+        const int p = entry[j], q = entry[j + 1];
+        if (p >= E || q >= E) return false;
+        const float x = Elem<DT>::to_f32(row[p]), y = Elem<DT>::to_f32(row[q]), bp = a.bias[p], bq = a.bias[q];
+        const float c = value_of(ekey[j]), d = value_of(ekey[j + 1]);
+        // How far the two are off together. A sigmoid: exp, two roundings, and of small ones exp's argument. A softmax: exp of
+        // an argument rounded twice, two products, and the sum, 22 roundings and its terms' (2^-19). A choice: one rounding.
+        const float rel_x = a.sigmoid ? 0x1p-21f + 0x1p-22f * fmaxf(-x, 0.0f) : 0x1p-18f + 0x1p-22f * fabsf(x - m);
+        const float rel_y = a.sigmoid ? 0x1p-21f + 0x1p-22f * fmaxf(-y, 0.0f) : 0x1p-18f + 0x1p-22f * fabsf(y - m);
+        const float off = fabsf(c - bp) * rel_x + fabsf(d - bq) * rel_y + 0x1p-23f * (fabsf(c) + fabsf(d)) + 1e-37f;
+        return c - d <= off && !(x == y && bp == bq);
+      };
+      const bool pair = live && l < k && near(l);             // (of lane k - 1: the last pick and the one behind it)
+      const bool after = live && l == 0 && near(k);           // the one behind the last pick and the next
+      auto of_token = [&](bool flag) {
+        const uint64_t v = ballot(flag);
+        return L == kWave ? v : (v >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
+      };
+      const uint64_t pairs = of_token(pair);
+      const bool edge = (pairs >> (k - 1)) & 1u, open = edge && (k == L || of_token(after) != 0u);
+      // Whole tokens again in 64 bits: where groups are near, or the set of the picks is open past what the list holds.
+      // (A softmax's sum takes the whole token anyway.)
+      uint64_t again = ballot(live && (close || open || (pairs != 0u && !a.sigmoid)));
+      if (ballot(pairs != 0u) & ~again) {
+        // otherwise the list itself in 64 bits, the one behind the last pick among it, and each to its rank
+        const bool listed = e < E;
+        const uint64_t c = listed ? key_of(1.0 / (1.0 + exp(-static_cast<double>(Elem<DT>::to_f32(row[e])))) + static_cast<double>(a.bias[e])) : 0u;
+        if (l < listing) lds.fine[seg * kEntry + l] = c;
+        wave_sync();
+        int rank = 0;
+        for (int j = 0; j < listing; ++j) {
+          const uint64_t o = lds.fine[seg * kEntry + j];
+          rank += o > c || (o == c && o != 0u && entry[j] < e);
         }
+        wave_sync();
+        if (listed && live && pairs != 0u) entry[rank] = e;
+        wave_sync();
       }
-      uint64_t again = ballot(close && live);
       while (again != 0u) {
         const int s = __builtin_ctzll(again) / L;
         again &= L == kWave ? 0u : ~(((uint64_t{1} << (L % kWave)) - 1) << (s * L));
@@ -430,7 +511,9 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       sum += c;
     }
     starts[e] = alone ? sum : 0;
-    if (!alone) a.counts[static_cast<int64_t>(blockIdx.x) * (E + 1) + e] = sum;
+    if (!alone && e == E)
+      for (int pad = E + 1; pad < a.pitch; ++pad) a.counts[static_cast<int64_t>(blockIdx.x) * a.pitch + pad] = 0;
+    if (!alone) a.counts[static_cast<int64_t>(blockIdx.x) * a.pitch + e] = sum;
   }
   __syncthreads();
   if (alone) {
@@ -447,51 +530,78 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
   }
 }
 
-// counts [blocks][E + 1] -> exclusive prefix sums over the workgroups, and the totals. A workgroup takes 64 experts, a wave
-// a share of the rows each.
-__global__ __launch_bounds__(kScanWaves * kWave) void pick_scan_kernel(PickArgs a) {
-  __shared__ int32_t sums[kScanWaves][kWave];
-  const int lane = lane_id(), wave = wave_id(), n = a.E + 1, e = static_cast<int>(blockIdx.x) * kWave + lane;
-  const int per = (a.blocks + kScanWaves - 1) / kScanWaves, first = wave * per;
+// counts [blocks][E + 1] -> exclusive prefix sums over the workgroups, and the totals. A workgroup takes kScanCols experts;
+// 64 threads an expert take a share of the workgroups each.
+__global__ __launch_bounds__(kScanCols * kWave) void pick_scan_kernel(PickArgs a) {
+  __shared__ int32_t sums[kWave][kScanCols + 1];
+  const int col = static_cast<int>(threadIdx.x) % kScanCols, share = static_cast<int>(threadIdx.x) / kScanCols;
+  const int n = a.E + 1, e = static_cast<int>(blockIdx.x) * kScanCols + col;
+  const int per = (a.blocks + kWave - 1) / kWave, first = share * per;
   const int end = first + per < a.blocks ? first + per : a.blocks;
   int32_t* p = a.counts + e;
   int sum = 0;
   if (e < n) {
 #pragma unroll 8
-    for (int i = first; i < end; ++i) sum += p[static_cast<int64_t>(i) * n];
+    for (int i = first; i < end; ++i) sum += p[static_cast<int64_t>(i) * a.pitch];
   }
-  sums[wave][lane] = sum;
+  sums[share][col] = sum;
+  __syncthreads();
+  const int lane = lane_id(), wave = wave_id();  // a wave adds up the shares of an expert
+  const int mine = sums[lane][wave], incl = wave_incl_scan(mine);
+  sums[lane][wave] = incl - mine;
+  if (lane == kWave - 1 && static_cast<int>(blockIdx.x) * kScanCols + wave < n) a.totals[blockIdx.x * kScanCols + wave] = incl;
   __syncthreads();
   if (e >= n) return;
-  int before = 0, all = 0;
-  for (int w = 0; w < kScanWaves; ++w) {
-    if (w < wave) before += sums[w][lane];
-    all += sums[w][lane];
-  }
-  if (wave == 0) a.totals[e] = all;
+  int before = sums[share][col];
 #pragma unroll 8
   for (int i = first; i < end; ++i) {
-    const int c = p[static_cast<int64_t>(i) * n];
-    p[static_cast<int64_t>(i) * n] = before;
+    const int c = p[static_cast<int64_t>(i) * a.pitch];
+    p[static_cast<int64_t>(i) * a.pitch] = before;
     before += c;
   }
 }
 
-__global__ __launch_bounds__(kPickThreads) void pick_place_kernel(PickArgs a, int block_tokens, int per_block) {
-  __shared__ int32_t starts[kMaxE + 1];
-  __shared__ int32_t waves[kPickThreads / kWave];
-  const int n = a.E + 1;
-  for (int e = threadIdx.x; e < n; e += kPickThreads) starts[e] = a.totals[e];
+// The workgroup takes the picks of one that picked, whose number is its own. Of few it adds up the counts before it, and all
+// of them, by itself: four experts a thread, the threads of an expert a share of the workgroups each.
+__global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, int block_picks) {
+  __shared__ int32_t starts[kMaxE + 4], base[kMaxE + 4];
+  __shared__ int32_t waves[kPlaceThreads / kWave];
+  const int n = a.E + 1, tid = static_cast<int>(threadIdx.x);
+  const int64_t block = blockIdx.x;
+  if (a.scanned) {
+    for (int e = tid; e < n; e += kPlaceThreads) {
+      starts[e] = a.totals[e];
+      base[e] = a.counts[block * a.pitch + e];
+    }
+  } else {
+    for (int e = tid; e < a.pitch; e += kPlaceThreads) starts[e] = base[e] = 0;
+    __syncthreads();
+    typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+    const int quads = a.pitch / 4, shares = kPlaceThreads / quads, share = tid / quads, quad = tid - share * quads;
+    if (share < shares) {
+      i32x4 all = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+#pragma unroll 8
+      for (int i = share; i < a.blocks; i += shares) {
+        const i32x4 c = *reinterpret_cast<const i32x4*>(a.counts + static_cast<int64_t>(i) * a.pitch + 4 * quad);
+        all += c;
+        before += i < block ? c : i32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // (integers: any order gives the same)
+        if (all[j] != 0) atomicAdd(&starts[4 * quad + j], all[j]);
+        if (before[j] != 0) atomicAdd(&base[4 * quad + j], before[j]);
+      }
+    }
+  }
   __syncthreads();
   block_scan(starts, n, waves);
-  if (blockIdx.x == 0)
-    for (int e = threadIdx.x; e < n; e += kPickThreads) a.offsets[e] = starts[e];
-  const int64_t picks = a.T * a.k, first = static_cast<int64_t>(blockIdx.x) * per_block;
-  const int64_t end = first + per_block < picks ? first + per_block : picks;
-  for (int64_t i = first + threadIdx.x; i < end; i += kPickThreads) {
+  if (block == 0)
+    for (int e = tid; e < n; e += kPlaceThreads) a.offsets[e] = starts[e];
+  const int64_t picks = a.T * a.k, first = block * block_picks;
+  const int64_t end = first + block_picks < picks ? first + block_picks : picks;
+  for (int64_t i = first + tid; i < end; i += kPlaceThreads) {
     const int id = a.ids[i], who = id < 0 ? a.E : id;
-    const uint32_t block = static_cast<uint32_t>(i) / static_cast<uint32_t>(block_tokens * a.k);
-    const int place = starts[who] + a.counts[static_cast<int64_t>(block) * n + who] + a.places[i];
+    const int place = starts[who] + base[who] + a.places[i];
     a.places[i] = id < 0 ? ~place : place;
     a.order[place] = static_cast<int32_t>(id < 0 ? ~i : i);
   }
@@ -508,14 +618,14 @@ __global__ __launch_bounds__(kPickThreads) void no_picks_kernel(int64_t* offsets
 //   sigmoid              s_j (1 - s_j) g_j          at the picks
 //   sigmoid, renormed    p_j (1 - s_j) (g_j - D)    at the picks
 template <int DT, int L, int PL>
-__global__ __launch_bounds__(kPickThreads) void pick_grad_kernel(PickArgs a, bool whole) {
+__global__ __launch_bounds__(kGradThreads) void pick_grad_kernel(PickArgs a, bool whole) {
   constexpr int kTokens = kWave / L;
   using S = typename Elem<DT>::S;
-  __shared__ float ds[kPickThreads / kWave][kTokens][kMaxK];
-  __shared__ int es[kPickThreads / kWave][kTokens][kMaxK];
+  __shared__ float ds[kGradThreads / kWave][kTokens][kMaxK];
+  __shared__ int es[kGradThreads / kWave][kTokens][kMaxK];
   const int wave = wave_id(), lane = lane_id(), seg = lane / L, l = lane % L, E = a.E, k = a.k;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (kPickThreads / kWave) * kTokens;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kPickThreads / kWave) + wave) * kTokens; t0 < a.T; t0 += step) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kGradThreads / kWave) * kTokens;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * (kGradThreads / kWave) + wave) * kTokens; t0 < a.T; t0 += step) {
     const int64_t t = t0 + seg < a.T ? t0 + seg : a.T - 1;
     const bool live = t0 + seg < a.T;
     const S* row = reinterpret_cast<const S*>(a.logits) + t * a.ld;
@@ -600,22 +710,28 @@ PickShape pick_shape(int64_t E) {
 }
 
 struct PickPlan {
-  int waves, wave_tokens;
-  int64_t blocks, counts, totals, total;  // workgroups; offsets of the counts and the totals; bytes in all
+  int waves, wave_tokens, pitch;
+  bool scan;
+  int64_t blocks, totals, total;  // workgroups; offset of the totals (behind the counts); bytes in all
 };
+
+// Workgroups that add up the counts by themselves: (workgroups) x (experts) up to this.
+constexpr int64_t kOwnCounts = 1 << 17;
 
 PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
   const int tokens = kWave / pick_shape(E).lanes;
   PickPlan p{};
-  p.waves = kPickThreads / kWave;
-  const int64_t step = p.waves * tokens;                           // tokens that a workgroup takes at once
+  p.waves = E <= 256 ? kPickThreads / kWave : kPickThreads / kWave / 2;  // (64 KB of LDS)
+  const int64_t step = p.waves * tokens;                                // tokens that a workgroup takes at once
   const int64_t most = std::max<int64_t>(1, kBlockPicks / (step * k));  // such steps whose ranks a workgroup can hold
-  int64_t steps = std::max<int64_t>(1, (T + 512 * step - 1) / (512 * step));
-  if (T * k <= kOneBlock) steps = (T + step - 1) / step;           // one workgroup
+  int64_t steps = std::max<int64_t>(1, (T + 256 * step - 1) / (256 * step));
+  if (T * k <= kOneBlock) steps = (T + step - 1) / step;                // one workgroup
   steps = std::max<int64_t>(1, std::min(steps, most));
   p.wave_tokens = static_cast<int>(steps * tokens);
   p.blocks = (T + steps * step - 1) / (steps * step);
-  p.totals = (p.blocks * (E + 1) * 4 + 255) / 256 * 256;
+  p.pitch = static_cast<int>((E + 4) / 4 * 4);
+  p.scan = p.blocks * p.pitch > kOwnCounts;
+  p.totals = (p.blocks * p.pitch * 4 + 255) / 256 * 256;
   p.total = p.blocks > 1 ? p.totals + (E + 1) * 4 : 0;
   return p;
 }
@@ -638,9 +754,9 @@ hipError_t launch_pick(const PickArgs& a, const PickPlan& p, bool whole, hipStre
 
 template <int DT, int L, int PL>
 hipError_t launch_pick_grad(const PickArgs& a, bool whole, hipStream_t s) {
-  const int64_t step = kPickThreads / L;
+  const int64_t step = kGradThreads / L;
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.T + step - 1) / step, 2048));
-  pick_grad_kernel<DT, L, PL><<<blocks, kPickThreads, 0, s>>>(a, whole);
+  pick_grad_kernel<DT, L, PL><<<blocks, kGradThreads, 0, s>>>(a, whole);
   return hipGetLastError();
 }
 
@@ -721,6 +837,7 @@ int smx_route(const void* logits, int64_t logits_stride, int dtype, int64_t T, i
   a.offsets = offsets;
   a.ids = ids;
   a.blocks = static_cast<int>(p.blocks);
+  a.pitch = p.pitch;
   if (ordered && p.total > 0) {
     if (!workspace || workspace_bytes < static_cast<size_t>(p.total)) return SMX_ERR_WORKSPACE;
     a.counts = static_cast<int32_t*>(workspace);
@@ -745,11 +862,13 @@ int smx_route(const void* logits, int64_t logits_stride, int dtype, int64_t T, i
   while ((E >> a.bits) != 0) ++a.bits;
   hipError_t err = launch_picks<false>(dtype, a, p, whole_runs(logits, logits_stride, E, es, pick_shape(E).each), s);
   if (err != hipSuccess || !ordered || p.blocks == 1) return static_cast<int>(err);
-  pick_scan_kernel<<<static_cast<unsigned>((E + 1 + kWave - 1) / kWave), kScanWaves * kWave, 0, s>>>(a);
-  err = hipGetLastError();
-  if (err != hipSuccess) return static_cast<int>(err);
-  const int64_t picks = T * k, per = std::max<int64_t>(kPickThreads, (picks + 2047) / 2048);
-  pick_place_kernel<<<static_cast<unsigned>((picks + per - 1) / per), kPickThreads, 0, s>>>(a, p.waves * p.wave_tokens, static_cast<int>(per));
+  if (p.scan) {
+    pick_scan_kernel<<<static_cast<unsigned>((E + kScanCols) / kScanCols), kScanCols * kWave, 0, s>>>(a);
+    err = hipGetLastError();
+    if (err != hipSuccess) return static_cast<int>(err);
+    a.scanned = true;
+  }
+  pick_place_kernel<<<static_cast<unsigned>(p.blocks), kPlaceThreads, 0, s>>>(a, static_cast<int>(p.waves * p.wave_tokens * k));
   return static_cast<int>(hipGetLastError());
 }
 

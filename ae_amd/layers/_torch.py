@@ -60,6 +60,15 @@ def address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def dense(t: torch.Tensor | None) -> torch.Tensor | None:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def empty_rows(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of t's shape and type (empty_like costs half of empty on the host, but keeps other layouts)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def records_gradient(*tensors: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -71,13 +80,13 @@ def no_tangents(name: str, *tensors: torch.Tensor | None) -> None:
         raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
-def once(name: str, make, deps) -> tuple:
-    """make()'s gradients. Where a graph of the gradients themselves is recorded, they depend on deps in a way that
-    it cannot differentiate, and says so if it comes to that."""
+def once(name: str, make, deps, *args) -> tuple:
+    """make(*args), the gradients. Where a graph of the gradients themselves is recorded, they depend on deps in a way
+    that it cannot differentiate, and says so if it comes to that."""
     if not torch.is_grad_enabled():
-        return make()
+        return make(*args)
     with torch.no_grad():
-        grads = make()
+        grads = make(*args)
     deps = [t for t in deps if t is not None]
     return tuple(None if g is None else _Once.apply(name, g, *deps) for g in grads)
 

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._torch import address, dtype_code, no_tangents, once, raw_stream, records_gradient, rows_of
+from ._torch import address, dense, dtype_code, no_tangents, once, raw_stream, records_gradient, rows_of
 
 
 def _check_places(places, tokens, device):
@@ -38,54 +38,58 @@ def _check_matrix(name, t):
 
 
 def _spread(x, places):
-    device = x.device
-    if device.index != torch.cuda.current_device():  # kernels are launched on the current device
-        with torch.cuda.device(device):
+    index = x.device.index
+    if index != torch.cuda.current_device():  # kernels are launched on the current device
+        with torch.cuda.device(index):
             return _spread(x, places)
     (tokens, k), h = places.shape, x.shape[1]
     xm, xs = rows_of(x)
-    rows = torch.empty((tokens * k, h), dtype=x.dtype, device=device)
+    rows = x.new_empty((tokens * k, h))
     code = _lib.lib().smx_dispatch_rows(xm.data_ptr(), xs, dtype_code(x.dtype), tokens, h, places.data_ptr(), k,
-                                        rows.data_ptr(), raw_stream(device.index))
+                                        rows.data_ptr(), raw_stream(index))
     if code:
         _lib.check("smx_dispatch_rows", code)
     return rows
 
 
 def _gather(rows, places, weights, residual):
-    device = rows.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = rows.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return _gather(rows, places, weights, residual)
     (tokens, k), h = places.shape, rows.shape[1]
     m, stride = rows_of(rows)
     r, rs = (None, 0) if residual is None else rows_of(residual)
-    w = weights if weights is None or weights.is_contiguous() else weights.contiguous()
-    y = torch.empty((tokens, h), dtype=rows.dtype, device=device)
+    w = dense(weights)
+    y = rows.new_empty((tokens, h))
     code = _lib.lib().smx_combine_rows(m.data_ptr(), stride, dtype_code(rows.dtype), tokens, h, places.data_ptr(), k,
-                                       address(w), address(r), rs, y.data_ptr(), raw_stream(device.index))
+                                       address(w), address(r), rs, y.data_ptr(), raw_stream(index))
     if code:
         _lib.check("smx_combine_rows", code)
     return y
 
 
 def _gather_backward(dy, rows, places, weights, shape, need_rows, need_w):
-    device = dy.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = dy.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return _gather_backward(dy, rows, places, weights, shape, need_rows, need_w)
     (tokens, k), h = places.shape, shape[1]
     d, ds = rows_of(dy)
     m, ms = (None, 0) if rows is None or not need_w else rows_of(rows)
-    w = weights if weights is None or weights.is_contiguous() else weights.contiguous()
-    drows = torch.empty(shape, dtype=dy.dtype, device=device) if need_rows else None
-    dw = torch.empty((tokens, k), dtype=torch.float32, device=device) if need_w else None
+    w = dense(weights)
+    drows = dy.new_empty(shape) if need_rows else None
+    dw = dy.new_empty((tokens, k), dtype=torch.float32) if need_w else None
     code = _lib.lib().smx_combine_rows_grad(
         d.data_ptr(), ds, address(m), ms, dtype_code(dy.dtype), tokens, h, places.data_ptr(), k, address(w),
-        address(drows), address(dw), raw_stream(device.index))
+        address(drows), address(dw), raw_stream(index))
     if code:
         _lib.check("smx_combine_rows_grad", code)
     return drows, dw
+
+
+def _gather_once(dy, places):
+    return (_gather(dy, places, None, None),)
 
 
 class _Dispatch(torch.autograd.Function):
@@ -98,7 +102,7 @@ class _Dispatch(torch.autograd.Function):
     def backward(ctx, dy):
         no_tangents("dispatch_rows", dy)
         places, = ctx.saved_tensors
-        return *once("dispatch_rows", lambda: (_gather(dy, places, None, None),), (dy,)), None
+        return *once("dispatch_rows", _gather_once, (dy,), dy, places), None
 
 
 class _Combine(torch.autograd.Function):
@@ -115,8 +119,8 @@ class _Combine(torch.autograd.Function):
         need_rows, _, need_w, need_r = ctx.needs_input_grad
         drows = dw = None
         if need_rows or need_w:
-            drows, dw = once("combine_rows", lambda: _gather_backward(dy, rows, places, weights, ctx.shape, need_rows,
-                                                                      need_w), (dy, rows, weights))
+            drows, dw = once("combine_rows", _gather_backward, (dy, rows, weights), dy, rows, places, weights, ctx.shape,
+                             need_rows, need_w)
         return drows, None, dw, dy if need_r else None
 
 

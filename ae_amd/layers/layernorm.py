@@ -13,14 +13,15 @@ backward pass reads again.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
 from torch import nn
 
 from .. import _lib
-from ._torch import (address, dtype_code, no_tangents, once, ptr, raw_stream, records_gradient, require_gpu,
-                     rows_of, stream_of, workspace)
+from ._torch import (address, dense, dtype_code, empty_rows, no_tangents, once, ptr, raw_stream, records_gradient,
+                     require_gpu, rows_of, stream_of)
 
 
 def add_rmsnorm_gate(hidden: torch.Tensor, residual: Optional[torch.Tensor],
@@ -81,81 +82,95 @@ class RMSNorm(nn.Module):
 
 
 def _check_norm(x, weight, bias, eps, residual):
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x must be [..., H], got {tuple(x.shape)}")
-    dtype_code(x.dtype)
+    """The call's sizes: (dtype code, columns), and the type of the parameters."""
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if len(shape) < 1 or shape[-1] == 0:
+        raise ValueError(f"x must be [..., H], got {tuple(shape)}")
+    code = dtype_code(dtype)
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    h = x.shape[-1:]
-    for name, t, shape in (("weight", weight, h), ("bias", bias, h), ("residual", residual, x.shape)):
+    params = dtype
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is None:
             continue
-        if t.shape != shape:
-            raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-        if t.device != x.device:
-            raise ValueError(f"x is on {x.device}, {name} on {t.device}")
-        if t.dtype != x.dtype and (t is residual or t.dtype != torch.float32):
-            raise TypeError(f"dtype mismatch: x is {x.dtype}, {name} {t.dtype}")
+        if t.shape != (shape if t is residual else shape[-1:]):
+            raise ValueError(f"{name} must be {tuple(shape if t is residual else shape[-1:])}, got {tuple(t.shape)}")
+        if t.device != device:
+            raise ValueError(f"x is on {device}, {name} on {t.device}")
+        if t.dtype != dtype and (t is residual or t.dtype != torch.float32):
+            raise TypeError(f"dtype mismatch: x is {dtype}, {name} {t.dtype}")
+        if t is not residual:
+            params = t.dtype
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"dtype mismatch: weight is {weight.dtype}, bias {bias.dtype}")
     if not x.is_cuda:
-        raise ValueError(f"expected a GPU tensor, got one on {x.device}")
+        raise ValueError(f"expected a GPU tensor, got one on {device}")
+    return code, shape[-1], params
 
 
-def _params_dtype(weight, bias, dtype) -> int:
-    return dtype if weight is None and bias is None else dtype_code((bias if weight is None else weight).dtype)
+@functools.lru_cache(maxsize=4096)
+def _grad_workspace(*sizes: int) -> int:
+    return _lib.lib().smx_norm_grad_workspace_size(*sizes)
 
 
-def _norm_forward(kind, x, weight, bias, eps, residual, keep: bool):
+def _norm_forward(kind, sizes, x, weight, bias, eps, residual, keep: bool):
     """y, the sum (None without a residual), and the rows' statistics where the gradient needs them."""
-    device = x.device
-    if device.index != torch.cuda.current_device():  # kernels are launched on the current device
-        with torch.cuda.device(device):
-            return _norm_forward(kind, x, weight, bias, eps, residual, keep)
-    h, dtype = x.shape[-1], dtype_code(x.dtype)
+    index = x.device.index
+    if index != torch.cuda.current_device():  # kernels are launched on the current device
+        with torch.cuda.device(index):
+            return _norm_forward(kind, sizes, x, weight, bias, eps, residual, keep)
+    dtype, h, params = sizes
     xm, xs = rows_of(x)
-    rm, rs = (None, 0) if residual is None else rows_of(residual)
     rows = xm.numel() // h
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=device)
-    stats = None
+    y = empty_rows(x)
+    rm = total = stats = rp = tp = sp = None
+    rs = 0
+    if residual is not None:
+        rm, rs = rows_of(residual)
+        total = torch.empty_like(y)
+        rp, tp = rm.data_ptr(), total.data_ptr()
     if keep:
-        stats = torch.empty(rows if kind == _lib.SMX_NORM_RMS else 2 * rows, dtype=torch.float32, device=device)
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    code = _lib.lib().smx_norm(
-        kind, xm.data_ptr(), xs, address(rm), rs, dtype, rows, h, address(w), address(b),
-        _params_dtype(weight, bias, dtype), eps, y.data_ptr(), address(total), address(stats), raw_stream(device.index))
+        stats = x.new_empty(rows if kind == _lib.SMX_NORM_RMS else 2 * rows, dtype=torch.float32)
+        sp = stats.data_ptr()
+    w, b = dense(weight), dense(bias)
+    code = _lib.lib().smx_norm(kind, xm.data_ptr(), xs, rp, rs, dtype, rows, h, address(w), address(b),
+                               dtype_code(params), eps, y.data_ptr(), tp, sp, raw_stream(index))
     if code:
         _lib.check("smx_norm", code)
     return y, total, stats
 
 
-def _norm_backward(kind, dy, dsum, s, weight, stats, params, need):
-    device = s.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _norm_backward(kind, dy, dsum, s, weight, stats, params, need)
+def _norm_backward(kind, sizes, dy, dsum, s, weight, stats, need):
+    index = s.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _norm_backward(kind, sizes, dy, dsum, s, weight, stats, need)
     need_x, need_w, need_b = need
-    h, dtype = s.shape[-1], dtype_code(s.dtype)
+    dtype, h, params = sizes
     if dy is None:  # only the sum was used
-        zeros = [torch.zeros(h, dtype=params, device=device) if n else None for n in (need_w, need_b)]
-        return dsum if need_x else None, *zeros
+        return dsum if need_x else None, *(s.new_zeros(h, dtype=params) if n else None for n in (need_w, need_b))
     sm, ss = rows_of(s)
     dm, ds = rows_of(dy)
     rm, rs = (None, 0) if dsum is None else rows_of(dsum)
     rows = sm.numel() // h
-    dx = torch.empty(s.shape, dtype=s.dtype, device=device) if need_x else None
-    dw = torch.empty(h, dtype=params, device=device) if need_w else None
-    db = torch.empty(h, dtype=params, device=device) if need_b else None
-    ws, nbytes = None, 0
+    dx = dw = db = ws = xp = wp = bp = workp = None
+    nbytes = 0
+    if need_x:
+        dx = empty_rows(s)
+        xp = dx.data_ptr()
+    if need_w:
+        dw = s.new_empty(h, dtype=params)
+        wp = dw.data_ptr()
+    if need_b:
+        db = s.new_empty(h, dtype=params)
+        bp = db.data_ptr()
     if need_w or need_b:
-        nbytes = _lib.lib().smx_norm_grad_workspace_size(kind, rows, h, dtype)
-        ws = workspace(nbytes, device)
-    w = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    code = _lib.lib().smx_norm_grad(
-        kind, dm.data_ptr(), ds, address(rm), rs, sm.data_ptr(), ss, dtype, rows, h, address(w), dtype_code(params),
-        stats.data_ptr(), address(dx), address(dw), address(db), address(ws), nbytes, raw_stream(device.index))
+        nbytes = _grad_workspace(kind, rows, h, dtype)
+        ws = stats.new_empty(nbytes // 4)  # (fp32 partial sums)
+        workp = ws.data_ptr()
+    w = dense(weight)
+    code = _lib.lib().smx_norm_grad(kind, dm.data_ptr(), ds, address(rm), rs, sm.data_ptr(), ss, dtype, rows, h, address(w),
+                                    dtype_code(params), stats.data_ptr(), xp, wp, bp, workp, nbytes, raw_stream(index))
     if code:
         _lib.check("smx_norm_grad", code)
     return dx, dw, db
@@ -163,11 +178,10 @@ def _norm_backward(kind, dy, dsum, s, weight, stats, params, need):
 
 class _Norm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, kind, eps):
-        y, total, stats = _norm_forward(kind, x, weight, bias, eps, residual, True)
+    def forward(ctx, x, weight, bias, residual, kind, eps, sizes):
+        y, total, stats = _norm_forward(kind, sizes, x, weight, bias, eps, residual, True)
         ctx.save_for_backward(x if total is None else total, weight, stats)
-        ctx.kind = kind
-        ctx.params = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+        ctx.how = kind, sizes
         ctx.set_materialize_grads(False)
         return y if total is None else (y, total)
 
@@ -175,21 +189,22 @@ class _Norm(torch.autograd.Function):
     def backward(ctx, dy, dsum=None):
         no_tangents("a norm", dy, dsum)
         if dy is None and dsum is None:
-            return (None,) * 6
+            return (None,) * 7
+        kind, sizes = ctx.how
         s, weight, stats = ctx.saved_tensors  # as autograd hands them back: perhaps not at their old addresses
         x, w, b, r = ctx.needs_input_grad[:4]
-        dx, dw, db = once("a norm", lambda: _norm_backward(ctx.kind, dy, dsum, s, weight, stats, ctx.params,
-                                                           (x or r, w, b)), (dy, dsum, s, weight))
-        return dx if x else None, dw, db, dx if r else None, None, None
+        dx, dw, db = once("a norm", _norm_backward, (dy, dsum, s, weight), kind, sizes, dy, dsum, s, weight, stats,
+                          (x or r, w, b))
+        return dx if x else None, dw, db, dx if r else None, None, None, None
 
 
 def _norm(kind, x, weight, bias, eps, residual):
     no_tangents("a norm", x, weight, bias, residual)
     eps = float(eps)
-    _check_norm(x, weight, bias, eps, residual)
+    sizes = _check_norm(x, weight, bias, eps, residual)
     if records_gradient(x, weight, bias, residual):
-        return _Norm.apply(x, weight, bias, residual, kind, eps)
-    y, total, _ = _norm_forward(kind, x, weight, bias, eps, residual, False)
+        return _Norm.apply(x, weight, bias, residual, kind, eps, sizes)
+    y, total, _ = _norm_forward(kind, sizes, x, weight, bias, eps, residual, False)
     return y if total is None else (y, total)
 
 

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ._torch import (address, dtype_code, no_tangents, once, raw_stream, records_gradient, rows_of, workspace)
+from ._torch import dense, dtype_code, empty_rows, no_tangents, once, raw_stream, records_gradient, rows_of
 
 
 class Routing(NamedTuple):
@@ -57,41 +57,47 @@ def _check(logits, top_k, scoring, bias, num_groups, top_groups, scale):
 
 
 def _forward(logits, k, scoring, bias, num_groups, top_groups, renormalize, scale):
-    device = logits.device
-    if device.index != torch.cuda.current_device():  # kernels are launched on the current device
-        with torch.cuda.device(device):
+    index = logits.device.index
+    if index != torch.cuda.current_device():  # kernels are launched on the current device
+        with torch.cuda.device(index):
             return _forward(logits, k, scoring, bias, num_groups, top_groups, renormalize, scale)
     t, e = logits.shape
     m, stride = rows_of(logits)
-    weights = torch.empty((t, k), dtype=torch.float32, device=device)
-    ids = torch.empty((t, k), dtype=torch.int32, device=device)
-    places = torch.empty((t, k), dtype=torch.int32, device=device)
-    order = torch.empty(t * k, dtype=torch.int32, device=device)
-    offsets = torch.empty(e + 1, dtype=torch.int64, device=device)
+    weights = logits.new_empty((t, k), dtype=torch.float32)
+    ids = torch.empty_like(weights, dtype=torch.int32)
+    places = torch.empty_like(ids)
+    order = ids.new_empty(t * k)
+    offsets = ids.new_empty(e + 1, dtype=torch.int64)
     nbytes = _workspace_size(t, e, k)
-    ws = workspace(nbytes, device) if nbytes else None
+    ws = workp = biasp = None
+    if nbytes:
+        ws = ids.new_empty(nbytes // 4)  # (counts)
+        workp = ws.data_ptr()
     if bias is not None:
-        bias = bias.to(torch.float32).contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.to(torch.float32).contiguous()
+        biasp = bias.data_ptr()
     code = _lib.lib().smx_route(
-        m.data_ptr(), stride, dtype_code(logits.dtype), t, e, k, scoring, address(bias), num_groups, top_groups,
-        renormalize, scale, weights.data_ptr(), ids.data_ptr(), places.data_ptr(), order.data_ptr(), offsets.data_ptr(),
-        address(ws), nbytes, raw_stream(device.index))
+        m.data_ptr(), stride, dtype_code(logits.dtype), t, e, k, scoring, biasp, num_groups, top_groups, renormalize,
+        scale, weights.data_ptr(), ids.data_ptr(), places.data_ptr(), order.data_ptr(), offsets.data_ptr(), workp, nbytes,
+        raw_stream(index))
     if code:
         _lib.check("smx_route", code)
     return weights, ids, places, order, offsets
 
 
 def _backward(dw, logits, ids, scoring, renormalize, scale):
-    device = logits.device
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    index = logits.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return _backward(dw, logits, ids, scoring, renormalize, scale)
     t, e = logits.shape
     m, stride = rows_of(logits)
-    grad = torch.empty((t, e), dtype=logits.dtype, device=device)
+    grad = empty_rows(logits)
+    dw = dense(dw)
     code = _lib.lib().smx_route_grad(
-        dw.contiguous().data_ptr(), m.data_ptr(), stride, dtype_code(logits.dtype), t, e, ids.shape[1], scoring,
-        renormalize, scale, ids.data_ptr(), grad.data_ptr(), raw_stream(device.index))
+        dw.data_ptr(), m.data_ptr(), stride, dtype_code(logits.dtype), t, e, ids.shape[1], scoring, renormalize, scale,
+        ids.data_ptr(), grad.data_ptr(), raw_stream(index))
     if code:
         _lib.check("smx_route_grad", code)
     return (grad,)
@@ -113,7 +119,7 @@ class _Route(torch.autograd.Function):
         if dw is None:
             return (None,) * 8
         logits, ids = ctx.saved_tensors
-        return *once("route_experts", lambda: _backward(dw, logits, ids, *ctx.how), (dw, logits)), *(None,) * 7
+        return *once("route_experts", _backward, (dw, logits), dw, logits, ids, *ctx.how), *(None,) * 7
 
 
 def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: Optional[torch.Tensor] = None,

@@ -98,6 +98,20 @@ def test_ties(experts):
     _check(torch.zeros(20, experts, device=DEV), 8, "sigmoid", torch.zeros(experts, device=DEV), 4, 2)
 
 
+@pytest.mark.parametrize("k", [1, 2, 15, 16])
+@pytest.mark.parametrize("experts", [16, 60, 256, 300])
+def test_near_choices(experts, k):
+    """Runs of choices that 32 bits cannot tell apart, inside the picks, across their end and past it."""
+    g = _gen(experts + k)
+    logits = _logits(64, experts)
+    score = torch.sigmoid(logits[0].double())
+    step = torch.randint(0, experts // 3 + 1, (experts,), generator=g, device=DEV).double() / 8
+    bias = (step - score).float()  # the choices of a step lie within some 2^-25
+    logits = logits[:1] + torch.randn((64, experts), generator=g, device=DEV) * 1e-7
+    _check(logits, k, "sigmoid", bias)
+    _check(logits, k, "softmax", (step - torch.softmax(logits[0].double(), 0)).float())
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups,top_groups", [(1, 1), (8, 3)])
 def test_choices_that_32_bits_cannot_tell_apart(scoring, groups, top_groups):
