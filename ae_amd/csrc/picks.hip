@@ -18,12 +18,12 @@ namespace {
 
 constexpr int kPickThreads = 512;     // most of a workgroup that picks
 constexpr int kGradThreads = 256;
-constexpr int kPlaceThreads = 1024;
 constexpr int kMaxK = 16;
 constexpr int kMaxE = 1024;
 constexpr int kMaxGroups = 64;
 constexpr int kEntry = kMaxK + 2;     // slots of a token's picks: two more, whose distances are looked at
 constexpr int kBlockPicks = 1024;     // picks whose ranks a workgroup holds
+constexpr int kPlaceThreads = kBlockPicks;
 constexpr int kScanCols = 16;         // experts of a workgroup that scans
 constexpr int kOneBlock = 512;        // picks that one workgroup sorts by itself
 
@@ -53,6 +53,13 @@ __device__ __forceinline__ void wave_sync() {  // what this wave's lanes wrote t
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// v, unknown to the compiler: what a rare branch derives from it stays in the branch, where a wave that does not take it
+// spends nothing on it (a wave takes few tokens, so what is moved out of its loop costs as much as what is in it).
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // Values in an order of unsigned numbers: -inf is 0 (nobody's pick), NaN the largest, -0 as +0.
@@ -105,8 +112,9 @@ __device__ __forceinline__ void load_run(const char* base, int64_t at, int e, in
 #pragma unroll
     for (int i = 0; i < PL; ++i) v[i] = in ? Elem<DT>::to_f32(r.s[i]) : -__builtin_inff();
   } else {
+    const int rest = opaque(E - e);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) v[i] = e + i < E ? Elem<DT>::to_f32(p[i]) : -__builtin_inff();
+    for (int i = 0; i < PL; ++i) v[i] = i < rest ? Elem<DT>::to_f32(p[i]) : -__builtin_inff();
   }
 }
 
@@ -141,7 +149,7 @@ template <int L, int PL> struct PickLds {
 template <int DT>
 __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint64_t* key, int* entry) {
   using S = typename Elem<DT>::S;
-  const int lane = lane_id();
+  const int lane = opaque(lane_id());
   const S* row = reinterpret_cast<const S*>(a.logits) + t * a.ld;
   auto top_of = [](uint64_t v) {  // the wave's largest: the upper halves first
     const uint32_t high = static_cast<uint32_t>(v >> 32), top = max_over<kWave>(high);
@@ -247,11 +255,14 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
   const int seg = lane / L, l = lane % L, E = a.E, k = a.k;
   const bool ordered = a.places != nullptr;
   int32_t* mine = counts + wave * (E + 1);
-  if (ordered) {
-    for (int e = lane; e <= E; e += kWave) mine[e] = 0;
-    wave_sync();
-  }
-  float b[PL], far = 0.0f;  // the largest finite bias
+  const int64_t block_first = static_cast<int64_t>(blockIdx.x) * waves * a.wave_tokens;
+  const int64_t first = block_first + static_cast<int64_t>(wave) * a.wave_tokens;
+  const int64_t last = first + a.wave_tokens < a.T ? first + a.wave_tokens : a.T;
+  int* entry = lds.entry + seg * kEntry;
+  uint32_t* ekey = lds.key + seg * kEntry;
+  auto row_of = [&](int64_t t) { return (t < last ? t : last - 1) * a.ld; };
+  float next[PL], b[PL], far = 0.0f;  // the next tokens' logits; biases, and the largest finite one
+  if (first < last) load_run<DT, PL>(a.logits, row_of(first + seg), l * PL, E, whole, next);
   if constexpr (kBiased) {
     load_run<kF32, PL>(reinterpret_cast<const char*>(a.bias), 0, l * PL, E, whole && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0, b);
 #pragma unroll
@@ -259,17 +270,17 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       if (fabsf(b[i]) < __builtin_inff()) far = fmaxf(far, fabsf(b[i]));
     far = max_over<L>(far);
   }
-  const int64_t block_first = static_cast<int64_t>(blockIdx.x) * waves * a.wave_tokens;
-  const int64_t first = block_first + static_cast<int64_t>(wave) * a.wave_tokens;
-  const int64_t last = first + a.wave_tokens < a.T ? first + a.wave_tokens : a.T;
-  int* entry = lds.entry + seg * kEntry;
-  uint32_t* ekey = lds.key + seg * kEntry;
+  if (ordered) {
+    for (int e = lane; e <= E; e += kWave) mine[e] = 0;
+    wave_sync();
+  }
   for (int64_t t0 = first; t0 < last; t0 += kTokens) {
-    const int64_t t = t0 + seg;
+    const int64_t t = t0 + seg, at = row_of(t);
     const bool live = t < last;
-    const int64_t at = (live ? t : last - 1) * a.ld;
     float v[PL];
-    load_run<DT, PL>(a.logits, at, l * PL, E, whole, v);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) v[i] = next[i];
+    if (t0 + kTokens < last) load_run<DT, PL>(a.logits, row_of(t + kTokens), l * PL, E, whole, next);
     float m = 0.0f, z = 1.0f;
     if (!a.sigmoid && (kBiased || !a.renorm)) {
       m = v[0];
@@ -340,12 +351,13 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
           for (int i = 0; i < PL; ++i) key[i] = 0u;
         }
       } else {
+        const int lo = opaque(l);
 #pragma unroll
-        for (int i = 0; i < PL; ++i) lds.choice[seg][l * PL + i] = key[i];
+        for (int i = 0; i < PL; ++i) lds.choice[seg][lo * PL + i] = key[i];
         wave_sync();
-        for (int g = l; g < a.ng; g += L) {
+        for (int g = lo; g < a.ng; g += L) {
           uint32_t best = 0u, next = 0u;
-          for (int i = 0, r = l % a.gs; i < a.gs; ++i, r = r + 1 == a.gs ? 0 : r + 1) {  // (each lane from another bank on)
+          for (int i = 0, r = lo % a.gs; i < a.gs; ++i, r = r + 1 == a.gs ? 0 : r + 1) {  // (each lane from another bank on)
             const uint32_t c = lds.choice[seg][g * a.gs + r], less = best < c ? best : c;
             next = next > less ? next : less;
             best = best > c ? best : c;
@@ -355,7 +367,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         }
         wave_sync();
         for (int g0 = 0; g0 < a.ng; g0 += L) {
-          const int g = g0 + l;
+          const int g = g0 + lo;
           bool keep = false;
           if (g < a.ng) {
             const uint32_t c = lds.group[seg][g];
@@ -371,7 +383,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
           const uint64_t bits = ballot(keep);
           kept |= (L == kWave ? bits : (bits >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1)) << g0;
         }
-        int g = l * PL / a.gs, rest = l * PL - g * a.gs;
+        int g = lo * PL / a.gs, rest = lo * PL - g * a.gs;
 #pragma unroll
         for (int i = 0; i < PL; ++i) {
           if (!((kept >> (g & 63)) & 1u)) key[i] = 0u;
@@ -399,11 +411,15 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       const uint64_t who = ballot(top == all && all != 0u);
       const uint64_t of_token = L == kWave ? who : (who >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
       const bool winner = of_token != 0u && l == __builtin_ctzll(of_token);
-      int slot = -1;
+      bool open = winner;  // (the first of the winner's that is it)
+      int slot = 0;
 #pragma unroll
-      for (int i = PL - 1; i >= 0; --i) slot = winner && key[i] == all ? i : slot;
-#pragma unroll
-      for (int i = 0; i < PL; ++i) key[i] = i == slot ? 0u : key[i];
+      for (int i = 0; i < PL; ++i) {
+        const bool hit = open && key[i] == all;
+        open = open && !hit;
+        key[i] = hit ? 0u : key[i];
+        slot = hit ? i : slot;
+      }
       if (winner || (of_token == 0u && l == 0)) {
         entry[j] = winner ? l * PL + slot : E;
         ekey[j] = all;
@@ -567,7 +583,9 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
   __shared__ int32_t starts[kMaxE + 4], base[kMaxE + 4];
   __shared__ int32_t waves[kPlaceThreads / kWave];
   const int n = a.E + 1, tid = static_cast<int>(threadIdx.x);
-  const int64_t block = blockIdx.x;
+  const int64_t block = blockIdx.x, picks = a.T * a.k, pick = block * block_picks + tid;  // (block_picks <= kBlockPicks)
+  const bool some = tid < block_picks && pick < picks;
+  const int id = some ? a.ids[pick] : 0, rank = some ? a.places[pick] : 0, who = id < 0 ? a.E : id;
   if (a.scanned) {
     for (int e = tid; e < n; e += kPlaceThreads) {
       starts[e] = a.totals[e];
@@ -577,14 +595,22 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
     for (int e = tid; e < a.pitch; e += kPlaceThreads) starts[e] = base[e] = 0;
     __syncthreads();
     typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kBatch = 18;  // loads on their way at once
     const int quads = a.pitch / 4, shares = kPlaceThreads / quads, share = tid / quads, quad = tid - share * quads;
     if (share < shares) {
       i32x4 all = {0, 0, 0, 0}, before = {0, 0, 0, 0};
-#pragma unroll 8
-      for (int i = share; i < a.blocks; i += shares) {
-        const i32x4 c = *reinterpret_cast<const i32x4*>(a.counts + static_cast<int64_t>(i) * a.pitch + 4 * quad);
-        all += c;
-        before += i < block ? c : i32x4{0, 0, 0, 0};
+      for (int i0 = share; i0 < a.blocks; i0 += kBatch * shares) {
+        i32x4 c[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + j * shares;
+          c[j] = i < a.blocks ? *reinterpret_cast<const i32x4*>(a.counts + static_cast<int64_t>(i) * a.pitch + 4 * quad) : i32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          all += c[j];
+          if (i0 + j * shares < block) before += c[j];
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // (integers: any order gives the same)
@@ -597,13 +623,10 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
   block_scan(starts, n, waves);
   if (block == 0)
     for (int e = tid; e < n; e += kPlaceThreads) a.offsets[e] = starts[e];
-  const int64_t picks = a.T * a.k, first = block * block_picks;
-  const int64_t end = first + block_picks < picks ? first + block_picks : picks;
-  for (int64_t i = first + tid; i < end; i += kPlaceThreads) {
-    const int id = a.ids[i], who = id < 0 ? a.E : id;
-    const int place = starts[who] + base[who] + a.places[i];
-    a.places[i] = id < 0 ? ~place : place;
-    a.order[place] = static_cast<int32_t>(id < 0 ? ~i : i);
+  if (some) {
+    const int place = starts[who] + base[who] + rank;
+    a.places[pick] = id < 0 ? ~place : place;
+    a.order[place] = static_cast<int32_t>(id < 0 ? ~pick : pick);
   }
 }
 
@@ -722,6 +745,7 @@ PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
   const int tokens = kWave / pick_shape(E).lanes;
   PickPlan p{};
   p.waves = E <= 256 ? kPickThreads / kWave : kPickThreads / kWave / 2;  // (64 KB of LDS)
+  p.waves = static_cast<int>(std::min<int64_t>(p.waves, std::max<int64_t>(1, (T + tokens - 1) / tokens)));
   const int64_t step = p.waves * tokens;                                // tokens that a workgroup takes at once
   const int64_t most = std::max<int64_t>(1, kBlockPicks / (step * k));  // such steps whose ranks a workgroup can hold
   int64_t steps = std::max<int64_t>(1, (T + 256 * step - 1) / (256 * step));
