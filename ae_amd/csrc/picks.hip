@@ -130,12 +130,11 @@ __device__ __forceinline__ float quick_sigmoid(float x) {
   return (x < 0.0f ? e : 1.0f) * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// LDS of a wave: the picks of its tokens, their keys; the choices of its tokens by key while groups are compared,
+// LDS of a wave: the picks of its tokens; the choices of its tokens by key while groups are compared,
 // or the listed ones in 64 bits, or those of one token.
 template <int L, int PL> struct PickLds {
   static constexpr int kTokens = kWave / L;
-  int entry[kTokens * kEntry];
-  uint32_t key[kTokens * kEntry];
+  alignas(8) int entry[kTokens * kEntry];
   union {
     uint64_t fine[kTokens * kEntry];        // the listed choices in 64 bits
     uint32_t choice[kTokens][L * PL + 16];  // (tokens begin in other banks)
@@ -144,9 +143,9 @@ template <int L, int PL> struct PickLds {
   uint32_t group[kTokens][kMaxGroups];
 };
 
-// The picks of one token by its choices in 64 bits: the whole wave's work, for tokens whose choices 32 bits cannot tell
-// apart.
-template <int DT>
+// The picks of one token by its choices in 64 bits (without a bias the logits themselves): the whole wave's work, for tokens
+// whose choices the keys cannot tell apart.
+template <int DT, bool kBiased>
 __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint64_t* key, int* entry) {
   using S = typename Elem<DT>::S;
   const int lane = opaque(lane_id());
@@ -156,7 +155,7 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
     return static_cast<uint64_t>(top) << 32 | max_over<kWave>(high == top ? static_cast<uint32_t>(v) : 0u);
   };
   double m = 0.0, z = 1.0;
-  if (!a.sigmoid) {
+  if (kBiased && !a.sigmoid) {
     float top = -__builtin_inff();
     for (int e = lane; e < a.E; e += kWave) top = fmaxf(top, Elem<DT>::to_f32(row[e]));
     m = max_over<kWave>(top);
@@ -169,8 +168,11 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
     const double x = Elem<DT>::to_f32(row[e]);
     return a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - m) / z;
   };
-  for (int e = lane; e < a.E; e += kWave)
-    key[e] = Elem<DT>::to_f32(row[e]) == -__builtin_inff() ? 0u : key_of(score(e) + static_cast<double>(a.bias[e]));
+  for (int e = lane; e < a.E; e += kWave) {
+    const float x = Elem<DT>::to_f32(row[e]);
+    if constexpr (kBiased) key[e] = x == -__builtin_inff() ? 0u : key_of(score(e) + static_cast<double>(a.bias[e]));
+    else key[e] = key_of(static_cast<double>(x));
+  }
   wave_sync();
   if (a.tg < a.ng) {
     uint64_t mine = 0u;
@@ -192,7 +194,7 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
       }
       // scores and biases each on their own: the sums of biases are exact, so groups that tie tie here
       mine = best;
-      if (next != 0u)
+      if (kBiased && next != 0u)
         mine = key_of((score(at) + score(after)) + (static_cast<double>(a.bias[at]) + static_cast<double>(a.bias[after])));
     }
     int before = 0;
@@ -243,9 +245,17 @@ __device__ __forceinline__ void block_scan(int32_t* v, int n, int32_t* waves) {
   __syncthreads();
 }
 
+// The keys that the rounds compare are the choices' with the expert's number in their low bits, so that one comparison finds
+// an expert, takes it out and settles ties:
+//   plain logits of 16 bits  all ten bits of it (1023 - e): their fp32 images have 13 low bits that say nothing. The keys of a
+//                            token differ, and are exact.
+//   otherwise                the number within the lane (PL - 1 - i, up to four bits). Lanes that tie in the rest of the key
+//                            are settled by their order. What these bits and fp32 itself leave open is looked at afterwards.
 template <int DT, int L, int PL, bool kBiased>
 __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool whole) {
   constexpr int kTokens = kWave / L;
+  constexpr bool kExact = DT != kF32 && !kBiased;
+  constexpr uint32_t kCode = kExact ? kMaxE - 1 : PL - 1;
   using Lds = PickLds<L, PL>;
   extern __shared__ __attribute__((aligned(16))) char shared[];
   const int waves = static_cast<int>(blockDim.x) / kWave, wave = wave_id(), lane = lane_id();
@@ -259,10 +269,8 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
   const int64_t first = block_first + static_cast<int64_t>(wave) * a.wave_tokens;
   const int64_t last = first + a.wave_tokens < a.T ? first + a.wave_tokens : a.T;
   int* entry = lds.entry + seg * kEntry;
-  uint32_t* ekey = lds.key + seg * kEntry;
   auto row_of = [&](int64_t t) { return (t < last ? t : last - 1) * a.ld; };
-  float next[PL], b[PL], far = 0.0f;  // the next tokens' logits; biases, and the largest finite one
-  if (first < last) load_run<DT, PL>(a.logits, row_of(first + seg), l * PL, E, whole, next);
+  float b[PL], far = 0.0f;  // biases, and the largest finite one
   if constexpr (kBiased) {
     load_run<kF32, PL>(reinterpret_cast<const char*>(a.bias), 0, l * PL, E, whole && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0, b);
 #pragma unroll
@@ -278,9 +286,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
     const int64_t t = t0 + seg, at = row_of(t);
     const bool live = t < last;
     float v[PL];
-#pragma unroll
-    for (int i = 0; i < PL; ++i) v[i] = next[i];
-    if (t0 + kTokens < last) load_run<DT, PL>(a.logits, row_of(t + kTokens), l * PL, E, whole, next);
+    load_run<DT, PL>(a.logits, at, l * PL, E, whole, v);
     float m = 0.0f, z = 1.0f;
     if (!a.sigmoid && (kBiased || !a.renorm)) {
       m = v[0];
@@ -302,7 +308,12 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       } else {
         key[i] = key_of(v[i]);
       }
+      if (kExact && key[i] != 0u) key[i] = (key[i] & ~kCode) | (kMaxE - 1 - (l * PL + i));
     }
+    auto of_token = [&](bool flag) {  // the token's lanes that raise it
+      const uint64_t v = ballot(flag);
+      return L == kWave ? v : (v >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
+    };
     bool close = false;  // groups too near for 32 bits
     if (a.tg < a.ng) {
       uint64_t kept = 0u;
@@ -330,20 +341,18 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         if (share >= 4) join(integral_constant<int, kDppXor2>{});
         if (share >= 8) join(integral_constant<int, kDppHalfMirror>{});
         if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
-        int before = 0;  // lanes whose group comes first
+        int before = 0;  // lanes whose group comes first (of groups that tie neither does)
         auto turn = [&](auto steps) {
           constexpr int kRor = 0x120 + decltype(steps)::value;  // row_ror: lane i has lane i - steps'
-          const uint32_t other = static_cast<uint32_t>(dpp<kRor>(static_cast<int>(best)));
-          const bool lower = dpp<kRor>(l) < l;
-          before += other > best || (lower && other == best);
+          before += static_cast<uint32_t>(dpp<kRor>(static_cast<int>(best))) > best;
         };
         turn(integral_constant<int, 1>{}); turn(integral_constant<int, 2>{}); turn(integral_constant<int, 3>{});
         turn(integral_constant<int, 4>{}); turn(integral_constant<int, 5>{}); turn(integral_constant<int, 6>{});
         turn(integral_constant<int, 7>{}); turn(integral_constant<int, 8>{}); turn(integral_constant<int, 9>{});
         turn(integral_constant<int, 10>{}); turn(integral_constant<int, 11>{}); turn(integral_constant<int, 12>{});
         turn(integral_constant<int, 13>{}); turn(integral_constant<int, 14>{}); turn(integral_constant<int, 15>{});
-        // (a lane counts lower lanes of its own group too: fewer than `share`)
         const bool real = l * PL < E, keep = (before >> __builtin_ctz(share)) < a.tg;
+        if (!kExact && share * a.tg < __builtin_popcountll(of_token(real && keep && best != 0u))) close = true;
         if (real && keep) low = value_of(best);
         if (real && !keep) high = value_of(best);
         if (!keep) {
@@ -380,8 +389,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
             if (keep) low = fminf(low, value_of(c));
             else high = fmaxf(high, value_of(c));
           }
-          const uint64_t bits = ballot(keep);
-          kept |= (L == kWave ? bits : (bits >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1)) << g0;
+          kept |= of_token(keep) << g0;
         }
         int g = lo * PL / a.gs, rest = lo * PL - g * a.gs;
 #pragma unroll
@@ -402,63 +410,73 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         if (low - high <= (a.sigmoid ? 0x1p-19f : 0x1p-16f) + 0x1p-21f * far) close = true;
       }
     }
-    const int rounds = k + (kBiased ? 2 : 0);
-    for (int j = 0; j < rounds; ++j) {
-      uint32_t top = key[0];
+    if constexpr (!kExact) {
 #pragma unroll
-      for (int i = 1; i < PL; ++i) top = key[i] > top ? key[i] : top;
-      const uint32_t all = max_over<L>(top);
-      const uint64_t who = ballot(top == all && all != 0u);
-      const uint64_t of_token = L == kWave ? who : (who >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
-      const bool winner = of_token != 0u && l == __builtin_ctzll(of_token);
-      bool open = winner;  // (the first of the winner's that is it)
-      int slot = 0;
+      for (int i = 0; i < PL; ++i) key[i] = key[i] == 0u ? 0u : (key[i] & ~kCode) | static_cast<uint32_t>(PL - 1 - i);
+    }
+    uint32_t pick = 0u;  // lane j: the key of pick j
+    if constexpr (kExact) {
+      for (int j = 0; j < k; ++j) {
+        uint32_t top = key[0];
 #pragma unroll
-      for (int i = 0; i < PL; ++i) {
-        const bool hit = open && key[i] == all;
-        open = open && !hit;
-        key[i] = hit ? 0u : key[i];
-        slot = hit ? i : slot;
+        for (int i = 1; i < PL; ++i) top = key[i] > top ? key[i] : top;
+        const uint32_t all = max_over<L>(top);
+        pick = l == j ? all : pick;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) key[i] = key[i] == all ? 0u : key[i];
       }
-      if (winner || (of_token == 0u && l == 0)) {
-        entry[j] = winner ? l * PL + slot : E;
-        ekey[j] = all;
+      if (l < k) entry[l] = pick != 0u ? static_cast<int>(kMaxE - 1 - (pick & kCode)) : E;
+    } else {
+      for (int j = 0; j < k + 2; ++j) {
+        uint32_t top = key[0];
+#pragma unroll
+        for (int i = 1; i < PL; ++i) top = key[i] > top ? key[i] : top;
+        const uint32_t all = max_over<L>(top);
+        const uint64_t who = of_token((top ^ all) <= kCode && all != 0u);
+        const bool winner = who != 0u && l == __builtin_ctzll(who);
+        const uint32_t gone = winner ? top : 1u;  // (no key)
+#pragma unroll
+        for (int i = 0; i < PL; ++i) key[i] = key[i] == gone ? 0u : key[i];
+        if (winner || (who == 0u && l == 0)) entry[j] = winner ? l * PL + static_cast<int>(PL - 1 - (top & kCode)) : E;
       }
     }
     wave_sync();
     using S = typename Elem<DT>::S;
     const S* row = reinterpret_cast<const S*>(a.logits) + at;
-    if constexpr (kBiased) {
-      // Which neighbours in the order 32 bits cannot tell apart: pick l and l + 1, and lane 0 that behind the last too.
+    if constexpr (!kExact) {
+      // Which neighbours in the list the keys cannot tell apart: lane j looks at entries j and j + 1.
       const int listing = k < L ? k + 1 : L;  // entries that have a lane
-      const int e = l < listing ? entry[l] : E;
-      auto near = [&](int j) {
-        const int p = entry[j], q = entry[j + 1];
-        if (p >= E || q >= E) return false;
-        const float x = Elem<DT>::to_f32(row[p]), y = Elem<DT>::to_f32(row[q]), bp = a.bias[p], bq = a.bias[q];
-        const float c = value_of(ekey[j]), d = value_of(ekey[j + 1]);
-        // How far the two are off together. A sigmoid: exp, two roundings, and of small ones exp's argument. A softmax: exp of
-        // an argument rounded twice, two products, and the sum, 22 roundings and its terms' (2^-19). A choice: one rounding.
-        const float rel_x = a.sigmoid ? 0x1p-21f + 0x1p-22f * fmaxf(-x, 0.0f) : 0x1p-18f + 0x1p-22f * fabsf(x - m);
-        const float rel_y = a.sigmoid ? 0x1p-21f + 0x1p-22f * fmaxf(-y, 0.0f) : 0x1p-18f + 0x1p-22f * fabsf(y - m);
-        const float off = fabsf(c - bp) * rel_x + fabsf(d - bq) * rel_y + 0x1p-23f * (fabsf(c) + fabsf(d)) + 1e-37f;
-        return c - d <= off && !(x == y && bp == bq);
-      };
-      const bool pair = live && l < k && near(l);             // (of lane k - 1: the last pick and the one behind it)
-      const bool after = live && l == 0 && near(k);           // the one behind the last pick and the next
-      auto of_token = [&](bool flag) {
-        const uint64_t v = ballot(flag);
-        return L == kWave ? v : (v >> (seg * L)) & ((uint64_t{1} << (L % kWave)) - 1);
-      };
-      const uint64_t pairs = of_token(pair);
-      const bool edge = (pairs >> (k - 1)) & 1u, open = edge && (k == L || of_token(after) != 0u);
+      const int e = l < listing ? entry[l] : E, n = l < listing ? entry[l + 1] : E;
+      bool near = false;
+      if (e < E && n < E) {
+        const float x = Elem<DT>::to_f32(row[e]), y = Elem<DT>::to_f32(row[n]);
+        if constexpr (kBiased) {
+          const float p = a.bias[e], q = a.bias[n];
+          const float s = a.sigmoid ? quick_sigmoid(x) : quick_exp(x - m) * rz, r = a.sigmoid ? quick_sigmoid(y) : quick_exp(y - m) * rz;
+          // How far the two are off together, or one of them and any that the list does not hold. A sigmoid: exp, two
+          // roundings (2^-22 of it, and of small ones less than that). A softmax, of the largest: exp of an argument rounded
+          // twice, two products, and the sum, 22 roundings and its terms' (2^-18). The key: a rounding, and the bits that it
+          // lacks (2^-19).
+          const float off = (a.sigmoid ? 0x1p-20f : 0x1p-17f * rz) + 0x1.2p-19f * (fabsf(s + p) + fabsf(r + q)) + 1e-37f;
+          near = (s + p) - (r + q) <= off && !(x == y && p == q);
+        } else {
+          near = x - y <= 0x1p-19f * (fabsf(x) + fabsf(y)) + 1e-37f && x != y;
+        }
+      }
+      const uint64_t pairs = of_token(near && live);
+      const bool inside = pairs & ((uint64_t{1} << k) - 1);  // among the picks and the one behind them
+      const bool edge = (pairs >> (k - 1)) & 1u, open = edge && (k == L || ((pairs >> k) & 1u));
       // Whole tokens again in 64 bits: where groups are near, or the set of the picks is open past what the list holds.
       // (A softmax's sum takes the whole token anyway.)
-      uint64_t again = ballot(live && (close || open || (pairs != 0u && !a.sigmoid)));
-      if (ballot(pairs != 0u) & ~again) {
+      uint64_t again = ballot(live && (close || open || (kBiased && !a.sigmoid && inside)));
+      if (ballot(inside) & ~again) {
         // otherwise the list itself in 64 bits, the one behind the last pick among it, and each to its rank
         const bool listed = e < E;
-        const uint64_t c = listed ? key_of(1.0 / (1.0 + exp(-static_cast<double>(Elem<DT>::to_f32(row[e])))) + static_cast<double>(a.bias[e])) : 0u;
+        uint64_t c = 0u;
+        if (listed) {
+          const double x = Elem<DT>::to_f32(row[e]);
+          c = key_of(kBiased ? 1.0 / (1.0 + exp(-x)) + static_cast<double>(a.bias[e]) : x);
+        }
         if (l < listing) lds.fine[seg * kEntry + l] = c;
         wave_sync();
         int rank = 0;
@@ -467,21 +485,21 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
           rank += o > c || (o == c && o != 0u && entry[j] < e);
         }
         wave_sync();
-        if (listed && live && pairs != 0u) entry[rank] = e;
+        if (listed && live && inside) entry[rank] = e;
         wave_sync();
       }
       while (again != 0u) {
         const int s = __builtin_ctzll(again) / L;
         again &= L == kWave ? 0u : ~(((uint64_t{1} << (L % kWave)) - 1) << (s * L));
         wave_sync();
-        pick_exactly<DT>(a, t0 + s, lds.exact, lds.entry + s * kEntry);
+        pick_exactly<DT, kBiased>(a, t0 + s, lds.exact, lds.entry + s * kEntry);
       }
     }
     // the weights: lane j has pick j
     const int e = l < k ? entry[l] : E;
     const bool some = e < E;
     float x = -__builtin_inff();
-    if (some) x = kBiased ? Elem<DT>::to_f32(row[e]) : value_of(ekey[l]);
+    if (some) x = kExact ? value_of((pick >> 31) != 0u ? pick & ~kCode : pick | kCode) : Elem<DT>::to_f32(row[e]);
     float s;
     if (a.renorm) {
       // ratios of scores, scaled by the largest so that they do not vanish together
@@ -748,7 +766,8 @@ PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
   p.waves = static_cast<int>(std::min<int64_t>(p.waves, std::max<int64_t>(1, (T + tokens - 1) / tokens)));
   const int64_t step = p.waves * tokens;                                // tokens that a workgroup takes at once
   const int64_t most = std::max<int64_t>(1, kBlockPicks / (step * k));  // such steps whose ranks a workgroup can hold
-  int64_t steps = std::max<int64_t>(1, (T + 256 * step - 1) / (256 * step));
+  const int64_t spread = 256 * (E <= 256 ? 1 : 2);                      // workgroups for many tokens
+  int64_t steps = std::max<int64_t>(1, (T + spread * step - 1) / (spread * step));
   if (T * k <= kOneBlock) steps = (T + step - 1) / step;                // one workgroup
   steps = std::max<int64_t>(1, std::min(steps, most));
   p.wave_tokens = static_cast<int>(steps * tokens);

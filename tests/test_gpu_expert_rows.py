@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_amd._lib import SmxError
 from ae_amd.layers import (combine_rows, dispatch_rows, fused_linear, grouped_linear, layer_norm, rms_norm, route_experts,
                            stack_fused_moe)
 from tests.block_ref import F64, combine, order_of
@@ -227,6 +228,18 @@ def test_differentiable_once_and_moved_tensors():
         torch.autograd.grad(d.sum(), [w])
 
 
+def test_refusals_on_the_gpu():
+    x, p = torch.zeros(4, 8, device=DEV), torch.zeros(4, 17, dtype=torch.int32, device=DEV)
+    with pytest.raises(SmxError, match="supported"):
+        dispatch_rows(x, p)
+    with pytest.raises(SmxError, match="supported"):
+        combine_rows(torch.zeros(68, 8, device=DEV), p)
+    with pytest.raises(ValueError, match="places is on"):
+        dispatch_rows(x, p.cpu())
+    with pytest.raises(ValueError, match="weights on"):
+        combine_rows(x[:4], p[:2, :2].contiguous(), torch.zeros(2, 2))
+
+
 # ---- together ------------------------------------------------------------------------------------------
 
 
@@ -303,7 +316,7 @@ def test_trained_block_together(norm, scoring, tokens):
     grads = torch.autograd.grad(want, host, dy.double().cpu())
     # fp32 sums of up to 192 terms through six layers, on the largest output or gradient: 6 * 192 * 2^-24
     bound = 6 * 192 * 2.0 ** -24
-    check(y.detach().cpu(), want.detach(), torch.full_like(want.detach(), bound * float(want.abs().max())))
+    check(y.detach().cpu(), want.detach(), torch.full_like(want.detach(), bound * float(want.detach().abs().max())))
     for name, a, b in zip(("x", "r", *w), got, grads):
         assert float((a.double().cpu() - b).abs().max()) <= bound * float(b.abs().max()), name
 

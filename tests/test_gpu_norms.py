@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_amd._lib import SmxError
 from ae_amd.layers import RMSNorm, layer_norm, rms_norm
 from tests.block_ref import F64, norm
 from tests.product_ref import check
@@ -321,6 +322,16 @@ def test_saved_tensors_may_move():
     with torch.autograd.graph.save_on_cpu():
         outs = layer_norm(x, w, b, residual=r)
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(outs, leaves, [dy, ds]), want))
+
+
+def test_refusals_on_the_gpu():
+    x = torch.zeros(3, 16385, device=DEV)
+    with pytest.raises(SmxError, match="supported"):
+        layer_norm(x)
+    with pytest.raises(ValueError, match="weight on"):
+        rms_norm(x[:, :64], torch.ones(64))
+    with pytest.raises(TypeError, match="mismatch"):
+        rms_norm(x[:, :64].bfloat16(), torch.ones(64, device=DEV).half())
 
 
 def test_a_changed_sum_is_noticed():

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_amd._lib import SmxError
 from ae_amd.layers import route_experts, select_experts
 from tests.block_ref import F64, INF, choose, order_of, route
 from tests.product_ref import check
@@ -96,6 +97,19 @@ def test_ties(experts):
             _check(logits, 8, scoring, b)
             _check(logits, 8, scoring, b, 8, 4)
     _check(torch.zeros(20, experts, device=DEV), 8, "sigmoid", torch.zeros(experts, device=DEV), 4, 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("experts,groups,top_groups", [(16, 8, 2), (64, 1, 1), (64, 8, 3), (256, 8, 4), (160, 8, 3), (512, 8, 4)])
+def test_a_router_of_zeros(experts, groups, top_groups, dtype):
+    """Every choice of every token ties: the first experts of the first groups."""
+    logits = torch.zeros((500, experts), dtype=dtype, device=DEV)
+    size = experts // groups
+    k = min(8, size * top_groups)
+    for bias in (None, torch.zeros(experts, device=DEV)):
+        for scoring in ("softmax", "sigmoid"):
+            out = _check(logits, k, scoring, bias, groups, top_groups)
+            assert (out[1] == torch.arange(k, device=DEV, dtype=torch.int32)).all()
 
 
 @pytest.mark.parametrize("k", [1, 2, 15, 16])
@@ -328,6 +342,22 @@ def test_differentiable_once_and_moved_tensors():
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(d.sum(), [logits])
     assert not route_experts(logits, 3).ids.requires_grad
+
+
+def test_refusals_on_the_gpu():
+    x = _logits(4, 64)
+    with pytest.raises(SmxError, match="supported"):
+        route_experts(x, 17)
+    with pytest.raises(SmxError, match="supported"):
+        route_experts(_logits(2, 1025), 2)
+    with pytest.raises(SmxError, match="supported"):
+        route_experts(_logits(2, 130), 2, num_groups=65)
+    with pytest.raises(ValueError, match="bias on"):
+        route_experts(x, 2, bias=torch.zeros(64))
+    with pytest.raises(ValueError, match="detached"):
+        route_experts(x, 2, bias=torch.zeros(64, device=DEV, requires_grad=True))
+    with torch.no_grad():
+        route_experts(x, 2, bias=torch.zeros(64, device=DEV, requires_grad=True))
 
 
 @pytest.mark.parametrize("renormalize", [True, False])
