@@ -9,6 +9,14 @@
 //   pick_grad_kernel   the gradient of a token's logits
 //
 // Everything is counted in integers and in the order of the picks, so the order is the stable one on every run.
+//
+// Bound by the instructions of the choice, not by the logits' bytes (8191 tokens over 256 experts in fp32: 8.4 MB, 2 us): 4
+// tokens a wave, about 490 vector instructions a token with groups and a bias. Measured, in bf16 unless said:
+//   1 token, 64 experts, 6 picks                                         4.8 us, one launch
+//   8191 tokens, 256 experts in 8 groups, bias, 8 picks, fp32            picks 14.9, places 7.3 us (at first 33, and 12 in two)
+//   65536 tokens, the same                                               68 us with the order, 50 without
+//   65536 tokens, 256 experts, 8 picks, no groups, no bias               42 and 24 us
+//   16384 tokens, 64 experts, 6 picks                                    picks 8.2, places 6.6, gradient 5.5 us
 #include <algorithm>
 
 #include "blocks.h"
@@ -756,7 +764,8 @@ struct PickPlan {
   int64_t blocks, totals, total;  // workgroups; offset of the totals (behind the counts); bytes in all
 };
 
-// Workgroups that add up the counts by themselves: (workgroups) x (experts) up to this.
+// Workgroups that add up the counts by themselves: (workgroups) x (experts) up to this. With 256 x 260 the placing kernel takes
+// 7.3 us that way, and 4.1 behind a scan of 4.8 and another launch; with 512 x 260 the scan is ahead.
 constexpr int64_t kOwnCounts = 1 << 17;
 
 PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
