@@ -10,7 +10,7 @@ import ctypes
 import os
 import threading
 
-from .build import LIB_PATH
+from .build import BINDING_PATH, LIB_PATH
 
 SMX_F32, SMX_F16, SMX_BF16 = 0, 1, 2
 SMX_OK = 0
@@ -186,6 +186,21 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = handle
     return _lib
+
+
+_blocks = None
+
+
+def blocks():
+    """The compiled torch binding of the operators of include/specmoe_mi355x_blocks.h (ae_amd/csrc/torch_blocks.cpp)."""
+    global _blocks
+    if _blocks is None:
+        if not os.path.exists(BINDING_PATH):
+            raise ImportError(f"{BINDING_PATH} is missing: build it with `python -m ae_amd.build`")
+        lib()  # (torch's HIP runtime first)
+        from . import _blocks as module
+        _blocks = module
+    return _blocks
 
 
 # Fields of smx_moe_plan_info, in the order of enum smx_plan_field.

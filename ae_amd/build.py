@@ -1,10 +1,12 @@
-"""Build recipe for libspecmoe_mi355x.so (gfx950) -- compiles in-tree, no JIT cache.
+"""Build recipe for libspecmoe_mi355x.so (gfx950), and for _blocks.so, the torch binding of some of its
+operators -- compiles in-tree, no JIT cache.
 
     python -m ae_amd.build          # or: from ae_amd.build import build_library
     python -m ae_amd.build --changed   # recompile only sources newer than their objects
 
 Each HIP source is compiled to an object under ae_amd/_build/ (in parallel), then linked
-into ae_amd/libspecmoe_mi355x.so. hipcc cross-compiles, so this runs without a GPU.
+into ae_amd/libspecmoe_mi355x.so. hipcc cross-compiles, so this runs without a GPU. The binding is
+host code alone: g++ with torch's headers, linked to torch and to the library beside it.
 """
 from __future__ import annotations
 
@@ -23,6 +25,8 @@ SOURCES = ["routing.hip", "experts.hip", "layer1.hip", "tiles.hip", "wide.hip", 
            "stream_probe.hip", "products.hip", "product_tile.hip", "product_wide.hip", "product_rows.hip",
            "norms.hip", "picks.hip", "expert_rows.hip"]
 ARCH = "gfx950"
+BINDING = "torch_blocks.cpp"
+BINDING_PATH = os.path.join(PKG_DIR, "_blocks.so")
 
 # Packed-fp32 VALU forms are disabled for every HIP translation unit (the host pass warns
 # that it does not know the feature; that warning is harmless).
@@ -52,6 +56,35 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _compile_binding() -> str:
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    obj = os.path.join(BUILD_DIR, os.path.splitext(BINDING)[0] + ".o")
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes),
+           "-c", os.path.join(CSRC, BINDING), "-o", obj]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    return obj
+
+
+def _link_binding(obj: str) -> None:
+    import torch
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = BINDING_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", obj, "-o", tmp, f"-L{libs}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+           "-lc10_hip", f"-L{PKG_DIR}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath-link,{libs}"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"link failed: {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, BINDING_PATH)
+
+
 def _stale(src: str) -> bool:
     """The object of src is missing or older than src or any header in csrc/ or include/."""
     obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
@@ -67,14 +100,16 @@ def _stale(src: str) -> bool:
 
 def build_library(verbose: bool = False, changed_only: bool = False) -> str:
     """Compile the sources (all of them, or with changed_only those whose objects are stale)
-    and link the shared library; returns its path."""
+    and link the shared library and the binding; returns the library's path."""
     os.makedirs(BUILD_DIR, exist_ok=True)
     todo = [s for s in SOURCES if _stale(s)] if changed_only else list(SOURCES)
-    if todo:
-        with concurrent.futures.ThreadPoolExecutor(max_workers=len(todo)) as ex:
-            list(ex.map(_compile, todo))
+    binding = not changed_only or _stale(BINDING)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(todo) + 1) as ex:
+        bound = ex.submit(_compile_binding) if binding else None
+        list(ex.map(_compile, todo))
+        obj = bound.result() if bound else os.path.join(BUILD_DIR, os.path.splitext(BINDING)[0] + ".o")
     if verbose and changed_only:
-        print(f"compiled {todo}")
+        print(f"compiled {todo + [BINDING] * binding}")
     objs = [os.path.join(BUILD_DIR, os.path.splitext(s)[0] + ".o") for s in SOURCES]
     tmp = LIB_PATH + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp]
@@ -82,8 +117,9 @@ def build_library(verbose: bool = False, changed_only: bool = False) -> str:
     if proc.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, LIB_PATH)  # atomic: a concurrent loader never sees a half-written file
+    _link_binding(obj)
     if verbose:
-        print(f"built {LIB_PATH}")
+        print(f"built {LIB_PATH} and {BINDING_PATH}")
     return LIB_PATH
 
 

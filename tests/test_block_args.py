@@ -2,12 +2,15 @@
 C entry points' refusals (before the device is touched) and the Python operators' checks."""
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from ae_amd import _lib
+from ae_amd.build import BINDING_PATH
 from ae_amd.layers import combine_rows, dispatch_rows, layer_norm, rms_norm, route_experts
 from tests.block_ref import F64, INF, choose, combine, norm, order_of, route
 
@@ -99,6 +102,17 @@ def test_exports_every_declared_symbol():
         names = re.findall(r"^(?:int|size_t)\s+(smx_\w+)\s*\(", f.read(), re.M)
     assert sorted(names) == sorted(n for n, _, _ in _lib.BLOCK_SIGNATURES)
     assert all(hasattr(L, n) for n in names)
+
+
+def test_binding_beside_the_library():
+    """Loaded first, the binding leaves one HIP runtime and one copy of the library in the process."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import sys; sys.path.insert(0, %r); from ae_amd import _lib; b = _lib.blocks(); import ae_amd.layers; "
+            "maps = {l.split()[-1] for l in open('/proc/self/maps').read().splitlines()}; "
+            "print(b.__file__, *(len([m for m in maps if n in m]) for n in ('libamdhip64', 'libspecmoe_mi355x')))" % root)
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    assert out.stdout.split() == [BINDING_PATH, "1", "1"], out.stdout
 
 
 def _norm(**kw):
