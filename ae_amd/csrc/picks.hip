@@ -13,10 +13,10 @@
 // Bound by the instructions of the choice, not by the logits' bytes (8191 tokens over 256 experts in fp32: 8.4 MB, 2 us): 4
 // tokens a wave, about 490 vector instructions a token with groups and a bias. Measured, in bf16 unless said:
 //   1 token, 64 experts, 6 picks                                         4.8 us, one launch
-//   8191 tokens, 256 experts in 8 groups, bias, 8 picks, fp32            picks 14.9, places 7.3 us (at first 33, and 12 in two)
+//   8191 tokens, 256 experts in 8 groups, bias, 8 picks, fp32            picks 15, places 7.1 us (at first 33, and 12 in two)
 //   65536 tokens, the same                                               68 us with the order, 50 without
 //   65536 tokens, 256 experts, 8 picks, no groups, no bias               42 and 24 us
-//   16384 tokens, 64 experts, 6 picks                                    picks 8.2, places 6.6, gradient 5.5 us
+//   16384 tokens, 64 experts, 6 picks                                    picks 8.2, places 5.6, gradient 5.5 us
 #include <algorithm>
 
 #include "blocks.h"
@@ -31,7 +31,7 @@ constexpr int kMaxE = 1024;
 constexpr int kMaxGroups = 64;
 constexpr int kEntry = kMaxK + 2;     // slots of a token's picks: two more, whose distances are looked at
 constexpr int kBlockPicks = 1024;     // picks whose ranks a workgroup holds
-constexpr int kPlaceThreads = kBlockPicks;
+constexpr int kPlaceThreads = 512;
 constexpr int kScanCols = 16;         // experts of a workgroup that scans
 constexpr int kOneBlock = 512;        // picks that one workgroup sorts by itself
 
@@ -610,8 +610,14 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
   __shared__ int32_t waves[kPlaceThreads / kWave];
   const int n = a.E + 1, tid = static_cast<int>(threadIdx.x);
   const int64_t block = blockIdx.x, picks = a.T * a.k, pick = block * block_picks + tid;  // (block_picks <= kBlockPicks)
-  const bool some = tid < block_picks && pick < picks;
-  const int id = some ? a.ids[pick] : 0, rank = some ? a.places[pick] : 0, who = id < 0 ? a.E : id;
+  constexpr int kEach = kBlockPicks / kPlaceThreads;
+  int id[kEach], rank[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const bool some = tid + i * kPlaceThreads < block_picks && pick + i * kPlaceThreads < picks;
+    id[i] = some ? a.ids[pick + i * kPlaceThreads] : 0;
+    rank[i] = some ? a.places[pick + i * kPlaceThreads] : -1;
+  }
   if (a.scanned) {
     for (int e = tid; e < n; e += kPlaceThreads) {
       starts[e] = a.totals[e];
@@ -621,7 +627,7 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
     for (int e = tid; e < a.pitch; e += kPlaceThreads) starts[e] = base[e] = 0;
     __syncthreads();
     typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-    constexpr int kBatch = 18;  // loads on their way at once
+    constexpr int kBatch = 20;  // loads on their way at once
     const int quads = a.pitch / 4, shares = kPlaceThreads / quads, share = tid / quads, quad = tid - share * quads;
     if (share < shares) {
       i32x4 all = {0, 0, 0, 0}, before = {0, 0, 0, 0};
@@ -649,10 +655,13 @@ __global__ __launch_bounds__(kPlaceThreads) void pick_place_kernel(PickArgs a, i
   block_scan(starts, n, waves);
   if (block == 0)
     for (int e = tid; e < n; e += kPlaceThreads) a.offsets[e] = starts[e];
-  if (some) {
-    const int place = starts[who] + base[who] + rank;
-    a.places[pick] = id < 0 ? ~place : place;
-    a.order[place] = static_cast<int32_t>(id < 0 ? ~pick : pick);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (rank[i] < 0) continue;
+    const int who = id[i] < 0 ? a.E : id[i], place = starts[who] + base[who] + rank[i];
+    const int64_t mine = pick + i * kPlaceThreads;
+    a.places[mine] = id[i] < 0 ? ~place : place;
+    a.order[place] = static_cast<int32_t>(id[i] < 0 ? ~mine : mine);
   }
 }
 
@@ -765,7 +774,7 @@ struct PickPlan {
 };
 
 // Workgroups that add up the counts by themselves: (workgroups) x (experts) up to this. With 256 x 260 the placing kernel takes
-// 7.3 us that way, and 4.1 behind a scan of 4.8 and another launch; with 512 x 260 the scan is ahead.
+// 7.1 us that way, and 4.1 behind a scan of 4.8 and another launch; with 512 x 260 the scan is ahead.
 constexpr int64_t kOwnCounts = 1 << 17;
 
 PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {

@@ -9,6 +9,9 @@ counterpart.
     r = route_experts(logits, k)
     h = grouped_linear(dispatch_rows(x, r.places), w1, r.offsets, activation="swiglu")
     y = combine_rows(grouped_linear(h, w2, r.offsets), r.places, r.weights, residual=residual)
+
+Calls run on the current stream of their tensors' device, without host synchronisation, and can be captured into a graph; a
+captured backward pass as fused_linear has it (no autograd graph of the same leaves from outside the capture alive).
 """
 from __future__ import annotations
 

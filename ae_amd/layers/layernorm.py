@@ -10,6 +10,9 @@ RMSNorm and add_rmsnorm_gate serve: they take no part in differentiation. ``laye
 are the norms of a model that is trained (the reference has none). They write nothing in place, and
 normalise the sum as it is kept, rounded to its type, so that their gradients are those of the values the
 backward pass reads again.
+
+Calls run on the current stream of their tensors' device, without host synchronisation, and can be captured into a graph; a
+captured backward pass as fused_linear has it (no autograd graph of the same leaves from outside the capture alive).
 """
 from __future__ import annotations
 

@@ -4,6 +4,9 @@
 choices of scores, groups and bias, with the gradient of the logits and with what ``grouped_linear``,
 ``dispatch_rows`` and ``combine_rows`` need. It serves as well, from one token on. The reference has no
 counterpart.
+
+Calls run on the current stream of their tensors' device, without host synchronisation, and can be captured into a graph; a
+captured backward pass as fused_linear has it (no autograd graph of the same leaves from outside the capture alive).
 """
 from __future__ import annotations
 

@@ -1,6 +1,9 @@
 """dispatch_rows and combine_rows against the 64-bit reference, and a whole block of the operators together."""
+import threading
+
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from ae_amd._lib import SmxError
 from ae_amd.layers import (combine_rows, dispatch_rows, fused_linear, grouped_linear, layer_norm, rms_norm, route_experts,
@@ -350,6 +353,63 @@ def test_captured_block(tokens):
         torch.cuda.synchronize()
         got = [t.clone() for t in outs]
         assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+
+
+def test_block_checkpointed_and_accumulated():
+    """Recomputed in the backward pass, and twice into the same gradients: what one pass gives, twice."""
+    H, I, E, k, tokens = 64, 32, 4, 2, 33
+    g = _gen(15)
+    w = {"norm": _randn(g, H, scale=0.2) + 1, "gate": _randn(g, E, H, scale=0.2), "up": _randn(g, E, 2 * I, H, scale=0.1),
+         "down": _randn(g, E, H, I, scale=0.1)}
+    x, r, dy = (_randn(g, tokens, H) for _ in range(3))
+    leaves = [t.requires_grad_() for t in (x, r, *w.values())]
+
+    def block(x, r):
+        return _block("rms", x, r, w, k, "softmax", None)[0]
+
+    want = torch.autograd.grad(block(x, r), leaves, dy)
+    for _ in range(2):
+        torch.utils.checkpoint.checkpoint(block, x, r, use_reentrant=False).backward(dy)
+    for t, v in zip(leaves, want):
+        assert torch.equal(t.grad, 2 * v)
+
+
+def test_threads_at_once():
+    """Blocks of several Python threads, each on a stream of its own."""
+    H, E, k = 128, 16, 4
+    up, down = _randn(_gen(1), E, 64, H, scale=0.1), _randn(_gen(2), E, H, 32, scale=0.1)
+    inputs = [(_randn(_gen(10 + i), 200 + i, H), _randn(_gen(20 + i), 200 + i, E), _randn(_gen(30 + i), 200 + i, H)) for i in range(4)]
+
+    def step(i):
+        x, logits, dy = (t.detach().requires_grad_(j < 2) for j, t in enumerate(inputs[i]))
+        y, s = layer_norm(x, residual=x)
+        p = route_experts(logits, k)
+        h = grouped_linear(dispatch_rows(y, p.places), up, p.offsets, activation="swiglu")
+        out = combine_rows(grouped_linear(h, down, p.offsets), p.places, p.weights, residual=s)
+        return [out.detach(), *torch.autograd.grad(out, [x, logits], dy)]
+
+    want = [step(i) for i in range(4)]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[i] = step(i)
+            stream.synchronize()
+        except Exception as e:  # (shown in the main thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_padded_batch():
