@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_amd import _lib
 from ae_amd._lib import SmxError
 from ae_amd.layers import RMSNorm, layer_norm, rms_norm
 from tests.block_ref import F64, norm
@@ -277,6 +278,32 @@ def test_captured_training_step(rows):
         torch.cuda.synchronize()
         got = [t.clone() for t in outs]
         assert all(torch.equal(p, q) for p, q in zip(got, step())), i
+
+
+def test_margins_are_left_alone():
+    """The C calls write their results and nothing around them, and the workspace within its bytes."""
+    lib, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for rows, cols, dtype in ((37, 1001, F32), (130, 264, BF16), (5, 16384, BF16), (2000, 64, F16)):
+        code = {F32: 0, F16: 1, BF16: 2}[dtype]
+        x, r, w, b, dy, ds = _inputs(rows, cols, dtype, residual=True)
+        want = _check(False, x, r, w, b, dy, ds)
+        room = [torch.full((rows * cols + 256,), 5.0, dtype=dtype, device=DEV) for _ in range(3)]
+        y, s, dx = (t[128:128 + rows * cols] for t in room)
+        vectors = torch.full((3, cols + 256), 5.0, dtype=dtype, device=DEV)
+        dw, db = vectors[0, 128:128 + cols], vectors[1, 128:128 + cols]
+        stats = torch.full((2 * rows + 64,), 5.0, device=DEV)
+        need = lib.smx_norm_grad_workspace_size(0, rows, cols, code)
+        ws = torch.full((need + 512,), 77, dtype=torch.uint8, device=DEV)
+        assert lib.smx_norm(0, x.data_ptr(), cols, r.data_ptr(), cols, code, rows, cols, w.data_ptr(), b.data_ptr(), code, EPS,
+                            y.data_ptr(), s.data_ptr(), stats.data_ptr(), stream) == 0
+        assert lib.smx_norm_grad(0, dy.data_ptr(), cols, ds.data_ptr(), cols, s.data_ptr(), cols, code, rows, cols, w.data_ptr(),
+                                 code, stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need, stream) == 0
+        torch.cuda.synchronize()
+        for t, v in zip((y, dx, dx, dw, db), want):
+            assert torch.equal(t, v.flatten())
+        assert all((t[:128] == 5).all() and (t[-128:] == 5).all() for t in room)
+        assert (vectors[:2, :128] == 5).all() and (vectors[:2, 128 + cols:] == 5).all() and (vectors[2] == 5).all()
+        assert (stats[2 * rows:] == 5).all() and (ws[need:] == 77).all()
 
 
 def test_gradients_against_differences():

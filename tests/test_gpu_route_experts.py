@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from ae_amd import _lib
 from ae_amd._lib import SmxError
 from ae_amd.layers import route_experts, select_experts
 from tests.block_ref import F64, INF, choose, order_of, route
@@ -329,6 +330,45 @@ def test_gradients_against_differences(scoring, renormalize):
         want = float((d.to(F64) * way.to(F64)).sum())
         # 150 weights below 1, off by 2^-21 each: 150 * 4 * 2^-21 / (2 h) = 0.01; h^2 / 6 of third derivatives of some units
         assert abs(slope - want) < 0.01 + 150 * 4 * h * h / 6, (slope, want)
+
+
+def test_two_graphs_in_one_pool():
+    """Captured calls whose workspaces share memory, replayed in turn."""
+    sets = [(_logits(t, e), k) for t, e, k in ((3000, 64, 6), (9000, 256, 8))]
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x, k in sets:
+            route_experts(x, k)
+    torch.cuda.current_stream().wait_stream(side)
+    for x, k in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(route_experts(x, k))
+        graphs.append(graph)
+    for i in range(3):
+        for j, (x, k) in enumerate(sets):
+            x.copy_(_logits(*x.shape, seed=200 + i))
+        for j, (x, k) in enumerate(sets):
+            graphs[j].replay()
+        torch.cuda.synchronize()
+        for j, (x, k) in enumerate(sets):
+            assert all(torch.equal(p, q) for p, q in zip(outs[j], route_experts(x, k))), (i, j)
+
+
+@pytest.mark.parametrize("tokens", [1, 700])
+def test_picks_without_an_order(tokens):
+    """The C call without places, order and offsets: weights and ids alone."""
+    x = _logits(tokens, 64, BF16)
+    want = route_experts(x, 6, "sigmoid")
+    w, ids = torch.empty_like(want.weights), torch.empty_like(want.ids)
+    lib = _lib.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.smx_route(x.data_ptr(), 64, 2, tokens, 64, 6, 1, None, 1, 1, 1, 1.0, w.data_ptr(), ids.data_ptr(), None, None,
+                         None, None, 0, stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(w, want.weights) and torch.equal(ids, want.ids)
 
 
 def test_differentiable_once_and_moved_tensors():
