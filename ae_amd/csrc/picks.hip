@@ -33,7 +33,6 @@ constexpr int kEntry = kMaxK + 2;     // slots of a token's picks: two more, who
 constexpr int kBlockPicks = 1024;     // picks whose ranks a workgroup holds
 constexpr int kPlaceThreads = 512;
 constexpr int kScanCols = 16;         // experts of a workgroup that scans
-constexpr int kOneBlock = 512;        // picks that one workgroup sorts by itself
 
 struct PickArgs {
   const char* logits;
@@ -327,7 +326,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       uint64_t kept = 0u;
       float low = __builtin_inff(), high = -__builtin_inff();
       const int share = a.gs / PL;  // lanes of a group
-      if (L == 16 && share * PL == a.gs && (share & (share - 1)) == 0) {
+      if (share * PL == a.gs && (share & (share - 1)) == 0 && share <= 16) {
         // whole lanes a group: the two best of each lane's, joined over the group's lanes, and ranked over the token's
         uint32_t best = key[0], next = 0u;
 #pragma unroll
@@ -348,19 +347,31 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         if (share >= 2) join(integral_constant<int, kDppXor1>{});
         if (share >= 4) join(integral_constant<int, kDppXor2>{});
         if (share >= 8) join(integral_constant<int, kDppHalfMirror>{});
+        if (share >= 16) join(integral_constant<int, kDppMirror>{});
         if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
-        int before = 0;  // lanes whose group comes first (of groups that tie neither does)
-        auto turn = [&](auto steps) {
-          constexpr int kRor = 0x120 + decltype(steps)::value;  // row_ror: lane i has lane i - steps'
-          before += static_cast<uint32_t>(dpp<kRor>(static_cast<int>(best))) > best;
-        };
-        turn(integral_constant<int, 1>{}); turn(integral_constant<int, 2>{}); turn(integral_constant<int, 3>{});
-        turn(integral_constant<int, 4>{}); turn(integral_constant<int, 5>{}); turn(integral_constant<int, 6>{});
-        turn(integral_constant<int, 7>{}); turn(integral_constant<int, 8>{}); turn(integral_constant<int, 9>{});
-        turn(integral_constant<int, 10>{}); turn(integral_constant<int, 11>{}); turn(integral_constant<int, 12>{});
-        turn(integral_constant<int, 13>{}); turn(integral_constant<int, 14>{}); turn(integral_constant<int, 15>{});
-        const bool real = l * PL < E, keep = (before >> __builtin_ctz(share)) < a.tg;
-        if (!kExact && share * a.tg < __builtin_popcountll(of_token(real && keep && best != 0u))) close = true;
+        const bool real = l * PL < E;
+        bool keep;
+        if constexpr (L == kWave) {
+          int before = 0;
+          for (int g = 0; g < a.ng; ++g) {
+            const uint32_t other = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(best), g * share));
+            before += other > best || (other == best && g * share < (l & -share));
+          }
+          keep = before < a.tg;
+        } else {
+          int before = 0;  // lanes whose group comes first (of groups that tie neither does)
+          auto turn = [&](auto steps) {
+            constexpr int kRor = 0x120 + decltype(steps)::value;  // row_ror: lane i has lane i - steps'
+            before += static_cast<uint32_t>(dpp<kRor>(static_cast<int>(best))) > best;
+          };
+          turn(integral_constant<int, 1>{}); turn(integral_constant<int, 2>{}); turn(integral_constant<int, 3>{});
+          turn(integral_constant<int, 4>{}); turn(integral_constant<int, 5>{}); turn(integral_constant<int, 6>{});
+          turn(integral_constant<int, 7>{}); turn(integral_constant<int, 8>{}); turn(integral_constant<int, 9>{});
+          turn(integral_constant<int, 10>{}); turn(integral_constant<int, 11>{}); turn(integral_constant<int, 12>{});
+          turn(integral_constant<int, 13>{}); turn(integral_constant<int, 14>{}); turn(integral_constant<int, 15>{});
+          keep = (before >> __builtin_ctz(share)) < a.tg;
+          if (!kExact && share * a.tg < __builtin_popcountll(of_token(real && keep && best != 0u))) close = true;
+        }
         if (real && keep) low = value_of(best);
         if (real && !keep) high = value_of(best);
         if (!keep) {
@@ -758,7 +769,13 @@ __global__ __launch_bounds__(kGradThreads) void pick_grad_kernel(PickArgs a, boo
 
 struct PickShape { int lanes, each; };
 
-PickShape pick_shape(int64_t E) {
+// A wave a token where there are few and each takes long: its chain of instructions is shorter, though there are more in all
+// (256 experts in 8 groups with a bias, fp32: 1 token 11.1 -> 9.3 us, 1024 17.4 -> 15.5, 2048 20.6 and 20.0, 4096 23.3 -> 26.9).
+constexpr int64_t kFewTokens = 1024;
+
+PickShape pick_shape(int64_t T, int64_t E) {
+  if (T <= kFewTokens && E > 64 && E <= 128) return {64, 2};
+  if (T <= kFewTokens && E > 128 && E <= 256) return {64, 4};
   if (E <= 16) return {16, 1};
   if (E <= 64) return {16, 4};
   if (E <= 128) return {16, 8};
@@ -778,7 +795,8 @@ struct PickPlan {
 constexpr int64_t kOwnCounts = 1 << 17;
 
 PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
-  const int tokens = kWave / pick_shape(E).lanes;
+  const PickShape f = pick_shape(T, E);
+  const int tokens = kWave / f.lanes;
   PickPlan p{};
   p.waves = E <= 256 ? kPickThreads / kWave : kPickThreads / kWave / 2;  // (64 KB of LDS)
   p.waves = static_cast<int>(std::min<int64_t>(p.waves, std::max<int64_t>(1, (T + tokens - 1) / tokens)));
@@ -786,7 +804,10 @@ PickPlan pick_plan(int64_t T, int64_t E, int64_t k) {
   const int64_t most = std::max<int64_t>(1, kBlockPicks / (step * k));  // such steps whose ranks a workgroup can hold
   const int64_t spread = 256 * (E <= 256 ? 1 : 2);                      // workgroups for many tokens
   int64_t steps = std::max<int64_t>(1, (T + spread * step - 1) / (spread * step));
-  if (T * k <= kOneBlock) steps = (T + step - 1) / step;                // one workgroup
+  // one workgroup, while its steps take less than another kernel: of 64 experts two (42 tokens 7.5 us for 8.8, 85 9.4 for 9.0), of
+  // 16 four (128 tokens 7.5 for 8.0, 256 11.6 for 8.2), of more one (64 tokens over 256 experts in two 19.8 us for 16.0)
+  const int64_t alone = E <= 16 ? 4 : E <= 64 ? 2 : 1;
+  if (T <= alone * step) steps = (T + step - 1) / step;
   steps = std::max<int64_t>(1, std::min(steps, most));
   p.wave_tokens = static_cast<int>(steps * tokens);
   p.blocks = (T + steps * step - 1) / (steps * step);
@@ -823,7 +844,7 @@ hipError_t launch_pick_grad(const PickArgs& a, bool whole, hipStream_t s) {
 
 template <bool kGrad, int DT>
 hipError_t launch_typed(const PickArgs& a, const PickPlan& p, bool whole, hipStream_t s) {
-  const PickShape f = pick_shape(a.E);
+  const PickShape f = pick_shape(kGrad ? kFewTokens + 1 : a.T, a.E);
   auto go = [&](auto lanes, auto each) {
     constexpr int L = decltype(lanes)::value, PL = decltype(each)::value;
     if constexpr (kGrad) return launch_pick_grad<DT, L, PL>(a, whole, s);
@@ -837,6 +858,10 @@ hipError_t launch_typed(const PickArgs& a, const PickPlan& p, bool whole, hipStr
       case 8: return go(integral_constant<int, 16>{}, integral_constant<int, 8>{});
       default: return go(integral_constant<int, 16>{}, integral_constant<int, 16>{});
     }
+  }
+  if constexpr (!kGrad) {
+    if (f.each == 2) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (f.each == 4) return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
   }
   return f.each == 8 ? go(integral_constant<int, 64>{}, integral_constant<int, 8>{}) : go(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
@@ -921,7 +946,7 @@ int smx_route(const void* logits, int64_t logits_stride, int dtype, int64_t T, i
   a.weights = weights;
   a.wave_tokens = p.wave_tokens;
   while ((E >> a.bits) != 0) ++a.bits;
-  hipError_t err = launch_picks<false>(dtype, a, p, whole_runs(logits, logits_stride, E, es, pick_shape(E).each), s);
+  hipError_t err = launch_picks<false>(dtype, a, p, whole_runs(logits, logits_stride, E, es, pick_shape(T, E).each), s);
   if (err != hipSuccess || !ordered || p.blocks == 1) return static_cast<int>(err);
   if (p.scan) {
     pick_scan_kernel<<<static_cast<unsigned>((E + kScanCols) / kScanCols), kScanCols * kWave, 0, s>>>(a);
@@ -955,7 +980,7 @@ int smx_route_grad(const float* grad_weights, const void* logits, int64_t logits
   a.ids = const_cast<int32_t*>(ids);
   a.grad_w = grad_weights;
   a.grad = static_cast<char*>(grad_logits);
-  const int each = pick_shape(E).each;
+  const int each = pick_shape(kFewTokens + 1, E).each;
   const bool whole = whole_runs(logits, logits_stride, E, es, each) && whole_runs(grad_logits, E, E, es, each);
   return static_cast<int>(launch_picks<true>(dtype, a, PickPlan{}, whole, static_cast<hipStream_t>(stream)));
 }

@@ -61,6 +61,36 @@ def test_tokens(tokens):
     _check(_logits(tokens, 300, BF16), 9)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("experts,k,groups,top_groups", [(65, 5, 1, 1), (65, 5, 13, 3), (100, 16, 1, 1), (128, 8, 8, 3), (130, 1, 1, 1),
+                                                         (160, 6, 8, 3), (255, 16, 17, 4), (256, 8, 1, 1), (256, 8, 8, 4),
+                                                         (256, 16, 64, 9), (256, 2, 2, 1)])
+def test_experts_of_many_tokens(experts, k, groups, top_groups, dtype):
+    """Several tokens a wave, where few tokens have one each."""
+    logits = _logits(1100, experts, dtype)
+    logits[200] = 0.0
+    logits[300:310] = -INF
+    bias = torch.randn(experts, generator=_gen(experts), device=DEV) * 0.2
+    for scoring in ("softmax", "sigmoid"):
+        for b in (None, bias, torch.zeros(experts, device=DEV)):
+            _check(logits, k, scoring, b, groups, top_groups, renormalize=b is not None, scale=1.5)
+
+
+@pytest.mark.parametrize("experts", [100, 256])
+@pytest.mark.parametrize("k", [1, 7, 16])
+def test_near_choices_of_many_tokens(experts, k):
+    g = _gen(experts + k)
+    logits = _logits(1, experts)
+    step = torch.randint(0, experts // 3 + 1, (experts,), generator=g, device=DEV).double() / 8
+    bias = (step - torch.sigmoid(logits[0].double())).float()
+    other = (step - torch.softmax(logits[0].double(), 0)).float()
+    logits = logits + torch.randn((1100, experts), generator=g, device=DEV) * 1e-7
+    for groups, top_groups in ((1, 1), (4, 2)):
+        _check(logits, k, "sigmoid", bias, groups, top_groups)
+        _check(logits, k, "softmax", other, groups, top_groups)
+    _check((logits * 2 ** 20).round() / 2 ** 20, k)  # and plain ones that lie close or tie
+
+
 def test_many_tokens():
     """More workgroups than hold all tokens' ranks at one step each."""
     _check(_logits(140001, 20, BF16), 16)
@@ -97,6 +127,7 @@ def test_ties(experts):
         for b in (None, torch.zeros(experts, device=DEV), bias):
             _check(logits, 8, scoring, b)
             _check(logits, 8, scoring, b, 8, 4)
+            _check(logits.repeat(4, 1), 8, scoring, b, 8, 4)
     _check(torch.zeros(20, experts, device=DEV), 8, "sigmoid", torch.zeros(experts, device=DEV), 4, 2)
 
 
