@@ -7,8 +7,9 @@
 
 namespace smx {
 
-// Elements of one 16-byte load. Where rows are not whole chunks, a chunk's elements lie apart instead and are loaded
-// one by one (kVec false below).
+// Elements of one 16-byte load. kVec below: rows are whole chunks, 16-byte aligned. Otherwise a chunk is only aligned as its
+// elements are (global loads and stores take any alignment), and the last one of a row ends with the row: its first elements
+// are the one's before it too, which counts them; both write the same there. (Rows shorter than a chunk: element by element.)
 template <int DT> struct Chunk {
   using S = typename Elem<DT>::S;
   static constexpr int kN = 16 / sizeof(S);
@@ -16,46 +17,65 @@ template <int DT> struct Chunk {
   __device__ __forceinline__ float get(int j) const { return Elem<DT>::to_f32(e[j]); }
 };
 
+// 16 bytes at an element's alignment.
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int DT> struct Loose { using V = u32x4_at2; };
+template <> struct Loose<kF32> { using V = u32x4_at4; };
+
 // Round to nearest even (v_cvt_pk_bf16_f32); NaN stays NaN.
 template <int DT> __device__ __forceinline__ typename Elem<DT>::S round_to(float f) { return Elem<DT>::from_f32(f); }
 template <> __device__ __forceinline__ uint16_t round_to<kBF16>(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f));
 }
 
-// Chunk c of the TPR threads' walk over a row of H elements: elements (c TPR + tid) N .. + N - 1, or one by one
-// (c N + j) TPR + tid, so that neighbouring threads touch neighbouring elements either way.
+// Elements at p, of which only the first `rest` are there.
+template <int DT> __device__ __forceinline__ Chunk<DT> load_short(const typename Elem<DT>::S* p, int rest) {
+  Chunk<DT> r{};
+#pragma unroll
+  for (int j = 0; j < Chunk<DT>::kN; ++j)
+    if (j < rest) r.e[j] = p[j];
+  return r;
+}
+template <int DT> __device__ __forceinline__ void store_short(typename Elem<DT>::S* p, int rest, const Chunk<DT>& r) {
+#pragma unroll
+  for (int j = 0; j < Chunk<DT>::kN; ++j)
+    if (j < rest) p[j] = r.e[j];
+}
+
+// Chunk c of the TPR threads' walk over a row of H elements: elements (c TPR + tid) N .. + N - 1.
 template <int DT, int TPR, bool kVec> struct RowWalk {
   static constexpr int kN = Chunk<DT>::kN;
   using S = typename Elem<DT>::S;
   int H, tid;
 
-  __device__ __forceinline__ int col(int c, int j) const {
-    return kVec ? (c * TPR + tid) * kN + j : (c * kN + j) * TPR + tid;
+  __device__ __forceinline__ int first(int c) const { return (c * TPR + tid) * kN; }
+  __device__ __forceinline__ int at(int c) const { return kVec || H < kN ? first(c) : min(first(c), H - kN); }
+  __device__ __forceinline__ bool any(int c) const { return first(c) < H; }
+  __device__ __forceinline__ int col(int c, int j) const { return at(c) + j; }
+  // Whether the element is in the row, and this chunk's.
+  __device__ __forceinline__ bool in(int c, int j) const {
+    return kVec ? any(c) : any(c) && col(c, j) >= first(c) && col(c, j) < H;
   }
-  __device__ __forceinline__ bool in(int c, int j) const { return col(c, kVec ? 0 : j) < H; }
 
-  // Elements behind the row's end are zeros.
+  // Chunks behind the row's end are zeros.
   __device__ __forceinline__ Chunk<DT> load(const S* row, int c) const {
-    Chunk<DT> r;
+    Chunk<DT> r{};
     if constexpr (kVec) {
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (in(c, 0)) v = *reinterpret_cast<const u32x4*>(row + col(c, 0));
-      r = __builtin_bit_cast(Chunk<DT>, v);
+      if (any(c)) r = __builtin_bit_cast(Chunk<DT>, *reinterpret_cast<const u32x4*>(row + at(c)));
+    } else if (H < kN) {
+      if (any(c)) r = load_short<DT>(row + at(c), H - at(c));
     } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) r.e[j] = in(c, j) ? row[col(c, j)] : S{};
+      if (any(c)) r = __builtin_bit_cast(Chunk<DT>, static_cast<u32x4>(*reinterpret_cast<const typename Loose<DT>::V*>(row + at(c))));
     }
     return r;
   }
 
   __device__ __forceinline__ void store(S* row, int c, const Chunk<DT>& r) const {
-    if constexpr (kVec) {
-      if (in(c, 0)) *reinterpret_cast<u32x4*>(row + col(c, 0)) = __builtin_bit_cast(u32x4, r);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (in(c, j)) row[col(c, j)] = r.e[j];
-    }
+    if (!any(c)) return;
+    if constexpr (kVec) *reinterpret_cast<u32x4*>(row + at(c)) = __builtin_bit_cast(u32x4, r);
+    else if (H < kN) store_short<DT>(row + at(c), H - at(c), r);
+    else *reinterpret_cast<typename Loose<DT>::V*>(row + at(c)) = __builtin_bit_cast(u32x4, r);
   }
 
   // A vector of parameters of the row's type or fp32, `rest` where there is none.
@@ -69,13 +89,13 @@ template <int DT, int TPR, bool kVec> struct RowWalk {
 #pragma unroll
         for (int j = 0; j < kN; j += 4) {
           f32x4 v = {0.f, 0.f, 0.f, 0.f};
-          if (in(c, 0)) v = *reinterpret_cast<const f32x4*>(q + col(c, j));
+          if (any(c)) v = *reinterpret_cast<const f32x4*>(q + at(c) + j);
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[j + i] = v[i];
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) w[j] = in(c, j) ? q[col(c, j)] : 0.0f;
+        for (int j = 0; j < kN; ++j) w[j] = any(c) && col(c, j) < H ? q[col(c, j)] : 0.0f;
       }
     } else {
       const Chunk<DT> r = load(static_cast<const S*>(p), c);

@@ -9,7 +9,8 @@
 // The picks' rows are read past the caches: nothing reads them again soon, and what the call writes then stays there for the
 // next (combine 55 -> 45 us at 8191 tokens). Results are not stored past them: a dispatch alone would gain (39 -> 30 us), but
 // its reader loses that and more (dispatch and combine of what it wrote, 6 picks of 2048 columns: 8192 tokens 74 -> 82 us,
-// 4096 38 -> 42).
+// 4096 38 -> 42). Rows that are no whole chunks go by chunks at any alignment: 10000 tokens, 4 picks, 1001 columns in bf16 combine
+// 40 -> 25 us, its gradient 48 -> 42-47, in fp32 36 -> 38 and 76 -> 62, against elements one by one.
 #include <algorithm>
 
 #include "blocks.h"
@@ -35,49 +36,43 @@ struct MoveArgs {
   float* grad_weights;
 };
 
-// One thread's elements of a row: a 16-byte chunk, or as many elements a row of threads apart.
+// One thread's chunk of a row, from element `first` on; it lies at `col` (see Chunk).
 template <int DT, bool kVec> struct Part {
   static constexpr int kN = Chunk<DT>::kN;
   using S = typename Elem<DT>::S;
-  int col, step, H;
+  int first, col, H;
 
-  __device__ __forceinline__ bool in(int j) const { return col + j * step < H; }
-  // kOnce: nothing else reads it soon, so it takes no room in the caches (measured at combine_kernel).
+  __device__ __forceinline__ Part(int first, int H) : first(first), col(kVec || H < kN ? first : min(first, H - kN)), H(H) {}
+  __device__ __forceinline__ bool any() const { return first < H; }
+  __device__ __forceinline__ bool in(int j) const { return kVec || (col + j >= first && col + j < H); }
+
+  // kOnce: nothing else reads it soon, so it takes no room in the caches (measured above).
   template <bool kOnce = false> __device__ __forceinline__ Chunk<DT> load(const char* base, int64_t row, int64_t ld) const {
     const S* p = reinterpret_cast<const S*>(base) + row * ld + col;
-    Chunk<DT> r;
     if constexpr (kVec) {
       const u32x4* q = reinterpret_cast<const u32x4*>(p);
-      r = __builtin_bit_cast(Chunk<DT>, kOnce ? __builtin_nontemporal_load(q) : *q);
+      return __builtin_bit_cast(Chunk<DT>, kOnce ? __builtin_nontemporal_load(q) : *q);
     } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) r.e[j] = in(j) ? p[j * step] : S{};
+      if (H < kN) return load_short<DT>(p, H - col);
+      const auto* q = reinterpret_cast<const typename Loose<DT>::V*>(p);
+      return __builtin_bit_cast(Chunk<DT>, static_cast<u32x4>(kOnce ? __builtin_nontemporal_load(q) : *q));
     }
-    return r;
   }
   __device__ __forceinline__ void store(char* base, int64_t row, const Chunk<DT>& r) const {
     S* p = reinterpret_cast<S*>(base) + row * H + col;
-    if constexpr (kVec) {
-      *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, r);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (in(j)) p[j * step] = r.e[j];
-    }
+    if constexpr (kVec) *reinterpret_cast<u32x4*>(p) = __builtin_bit_cast(u32x4, r);
+    else if (H < kN) store_short<DT>(p, H - col, r);
+    else *reinterpret_cast<typename Loose<DT>::V*>(p) = __builtin_bit_cast(u32x4, r);
   }
 };
 
-// The token and the columns of a thread; false behind the end of either.
-template <int DT, bool kVec>
-__device__ __forceinline__ bool part_of(const MoveArgs& a, int64_t& t, Part<DT, kVec>& p) {
-  constexpr int kN = Chunk<DT>::kN;
+// The token of a thread, and its chunk of the columns.
+__device__ __forceinline__ int64_t token_of(const MoveArgs& a) {
+  return static_cast<int64_t>(blockIdx.x) * (kThreads >> a.shift) + (threadIdx.x >> a.shift);
+}
+template <int DT, bool kVec> __device__ __forceinline__ Part<DT, kVec> part_of(const MoveArgs& a) {
   const int width = 1 << a.shift, lane = static_cast<int>(threadIdx.x) & (width - 1);
-  t = static_cast<int64_t>(blockIdx.x) * (kThreads >> a.shift) + (threadIdx.x >> a.shift);
-  const int first = static_cast<int>(blockIdx.y) * width * kN;
-  p.H = a.H;
-  p.col = kVec ? first + lane * kN : first + lane;
-  p.step = kVec ? 1 : width;
-  return t < a.T && p.col < a.H;
+  return Part<DT, kVec>((static_cast<int>(blockIdx.y) * width + lane) * Chunk<DT>::kN, a.H);
 }
 
 // y[t] = residual[t] + sum_j weights[t, j] rows[places[t, j]]. The loads of four picks are on their way at once (of eight: 61
@@ -85,9 +80,9 @@ __device__ __forceinline__ bool part_of(const MoveArgs& a, int64_t& t, Part<DT, 
 template <int DT, bool kVec>
 __global__ __launch_bounds__(kThreads) void combine_kernel(MoveArgs a) {
   constexpr int kN = Chunk<DT>::kN, kBatch = 4;
-  int64_t t;
-  Part<DT, kVec> part;
-  if (!part_of(a, t, part)) return;
+  const int64_t t = token_of(a);
+  const Part<DT, kVec> part = part_of<DT, kVec>(a);
+  if (t >= a.T || !part.any()) return;
   float sum[kN] = {};
   const int32_t* at = a.places + t * a.k;
   for (int j0 = 0; j0 < a.k; j0 += kBatch) {
@@ -126,9 +121,9 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(MoveArgs a) {
 template <int DT, bool kVec>
 __global__ __launch_bounds__(kThreads) void spread_kernel(MoveArgs a) {
   constexpr int kN = Chunk<DT>::kN;
-  int64_t t;
-  Part<DT, kVec> part;
-  if (!part_of(a, t, part)) return;
+  const int64_t t = token_of(a);
+  const Part<DT, kVec> part = part_of<DT, kVec>(a);
+  if (t >= a.T || !part.any()) return;
   const Chunk<DT> x = part.load(a.x, t, a.x_ld);
   const int32_t* at = a.places + t * a.k;
   for (int j = 0; j < a.k; ++j) {
@@ -174,8 +169,8 @@ __global__ __launch_bounds__(grad_threads<TPR>()) void combine_grad_kernel(MoveA
   }
   const int picks = static_cast<int>(a.picks);
   for (int first = 0; first < a.H; first += TPR * kN) {
-    const Part<DT, kVec> part{kVec ? first + tid * kN : first + tid, kVec ? 1 : TPR, a.H};
-    if (part.col >= a.H) break;
+    const Part<DT, kVec> part(first + tid * kN, a.H);
+    if (!part.any()) break;
     const Chunk<DT> x = part.load(a.x, t, a.x_ld);
     Chunk<DT> r[K];
 #pragma unroll
@@ -191,7 +186,7 @@ __global__ __launch_bounds__(grad_threads<TPR>()) void combine_grad_kernel(MoveA
       if (p[j] >= 0) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-          dot[j] += r[j].get(i) * x.get(i);
+          dot[j] += part.in(i) ? r[j].get(i) * x.get(i) : 0.0f;
           o.e[i] = round_to<DT>(w[j] * x.get(i));
         }
       }

@@ -383,3 +383,20 @@ def test_the_serving_norm_beside_it():
     want, bound = norm(s, w, None, EPS, True, F32)["y"]
     check(y, want, bound)
     check(a, want, bound)
+
+
+@pytest.mark.parametrize("cols", [2, 4, 32])
+def test_a_large_mean_over_fewer_columns_than_threads(cols):
+    # Columns are a power of two, so the mean of equal values is exact and n is 0; mean * rstd = 2^113 1e6 passes fp32's range,
+    # and nothing behind the row's end may take part with it. dx = rstd (dy - mean of dy), dw = 0.
+    dy = torch.randint(-8, 9, (5, cols), generator=torch.Generator().manual_seed(cols)).float().cuda()
+    x = torch.full((5, cols), 2.0 ** 113, device="cuda").requires_grad_()
+    w = torch.ones(cols, device="cuda").requires_grad_()
+    b = torch.full((cols,), 0.5, device="cuda").requires_grad_()
+    y = layer_norm(x, w, b, 1e-12)
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    assert torch.equal(y, torch.full_like(y, 0.5)) and torch.equal(dw, torch.zeros_like(dw)) and torch.equal(db, dy.sum(0))
+    want = (dy.double() - dy.double().mean(1, keepdim=True)) * 1e6
+    # Sums of small integers are exact; roundings: eps to fp32 (half of it in its root), rsqrt (1 ulp, two half steps),
+    # and the product: 3.5 half steps.
+    assert ((dx.double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
