@@ -434,6 +434,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       for (int i = 0; i < PL; ++i) key[i] = key[i] == 0u ? 0u : (key[i] & ~kCode) | static_cast<uint32_t>(PL - 1 - i);
     }
     uint32_t pick = 0u;  // lane j: the key of pick j
+    const int listing = k < L ? k + 1 : L;  // entries that have a lane; one more is listed
     if constexpr (kExact) {
       for (int j = 0; j < k; ++j) {
         uint32_t top = key[0];
@@ -446,7 +447,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
       }
       if (l < k) entry[l] = pick != 0u ? static_cast<int>(kMaxE - 1 - (pick & kCode)) : E;
     } else {
-      for (int j = 0; j < k + 2; ++j) {
+      for (int j = 0; j <= listing; ++j) {
         uint32_t top = key[0];
 #pragma unroll
         for (int i = 1; i < PL; ++i) top = key[i] > top ? key[i] : top;
@@ -463,45 +464,72 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
     using S = typename Elem<DT>::S;
     const S* row = reinterpret_cast<const S*>(a.logits) + at;
     if constexpr (!kExact) {
-      // Which neighbours in the list the keys cannot tell apart: lane j looks at entries j and j + 1.
-      const int listing = k < L ? k + 1 : L;  // entries that have a lane
+      auto choice_of = [&](float x, float p) {  // as the keys have it, before it was cut
+        if constexpr (!kBiased) return x;
+        else return (a.sigmoid ? quick_sigmoid(x) : quick_exp(x - m) * rz) + p;
+      };
+      // How far two choices are off together, or one of them and any that the list does not hold. A sigmoid: exp, two
+      // roundings (2^-22 of it, and of small ones less than that). A softmax, of the largest: exp of an argument rounded
+      // twice, two products, and the sum, 22 roundings and its terms' (2^-18). The key: a rounding, and the bits that it
+      // lacks (2^-19).
+      auto reach = [&](float c, float d) {
+        if constexpr (!kBiased) return 0x1p-19f * (fabsf(c) + fabsf(d)) + 1e-37f;
+        else return (a.sigmoid ? 0x1p-20f : 0x1p-17f * rz) + 0x1.2p-19f * (fabsf(c) + fabsf(d)) + 1e-37f;
+      };
+      // Which neighbours in the list the keys cannot tell apart: lane j looks at entries j and j + 1. They are linked, equal or
+      // not: what lies behind a tie may still be larger than it.
       const int e = l < listing ? entry[l] : E, n = l < listing ? entry[l + 1] : E;
-      bool near = false;
+      bool linked = false, equal = false;
+      float x = 0.0f, p = 0.0f, c = 0.0f;  // logit, bias and choice of entry j
       if (e < E && n < E) {
-        const float x = Elem<DT>::to_f32(row[e]), y = Elem<DT>::to_f32(row[n]);
+        x = Elem<DT>::to_f32(row[e]);
+        const float y = Elem<DT>::to_f32(row[n]);
+        float q = 0.0f;
         if constexpr (kBiased) {
-          const float p = a.bias[e], q = a.bias[n];
-          const float s = a.sigmoid ? quick_sigmoid(x) : quick_exp(x - m) * rz, r = a.sigmoid ? quick_sigmoid(y) : quick_exp(y - m) * rz;
-          // How far the two are off together, or one of them and any that the list does not hold. A sigmoid: exp, two
-          // roundings (2^-22 of it, and of small ones less than that). A softmax, of the largest: exp of an argument rounded
-          // twice, two products, and the sum, 22 roundings and its terms' (2^-18). The key: a rounding, and the bits that it
-          // lacks (2^-19).
-          const float off = (a.sigmoid ? 0x1p-20f : 0x1p-17f * rz) + 0x1.2p-19f * (fabsf(s + p) + fabsf(r + q)) + 1e-37f;
-          near = (s + p) - (r + q) <= off && !(x == y && p == q);
-        } else {
-          near = x - y <= 0x1p-19f * (fabsf(x) + fabsf(y)) + 1e-37f && x != y;
+          p = a.bias[e];
+          q = a.bias[n];
         }
+        c = choice_of(x, p);
+        const float d = choice_of(y, q);
+        linked = c - d <= reach(c, d);
+        equal = x == y && p == q;
       }
-      const uint64_t pairs = of_token(near && live);
-      const bool inside = pairs & ((uint64_t{1} << k) - 1);  // among the picks and the one behind them
-      const bool edge = (pairs >> (k - 1)) & 1u, open = edge && (k == L || ((pairs >> k) & 1u));
+      const uint64_t links = of_token(linked && live), apart = of_token(linked && !equal && live);
+      const bool inside = apart & ((uint64_t{1} << k) - 1);  // among the picks and the one behind them
+      bool open = ((links >> (k - 1)) & 1u) && (k == L || ((links >> k) & 1u));  // from the last pick past what the list closes
+      if (ballot(open) != 0u) {
+        // Where all that the last pick cannot be told from are its equals, the list holds the first of them, in their order, and
+        // all that are larger: nothing is open. (A router of zeros is such a case, and 16-bit logits that tie.) What is not
+        // listed is not larger; the tenth more is for roundings.
+        const int at_last = seg * L + k - 1;
+        const float xk = __shfl(x, at_last, kWave), pk = __shfl(p, at_last, kWave), ck = __shfl(c, at_last, kWave);
+        const uint32_t below = key_of(ck - 1.1f * reach(ck, ck)) & ~kCode, least = below != 0u ? below : 1u;
+        bool other = apart & ((uint64_t{2} << k) - 1);
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+          bool same = v[i] == xk;
+          if constexpr (kBiased) same = same && b[i] == pk;
+          other |= key[i] >= least && !same;
+        }
+        open = open && of_token(other) != 0u;
+      }
       // Whole tokens again in 64 bits: where groups are near, or the set of the picks is open past what the list holds.
       // (A softmax's sum takes the whole token anyway.)
       uint64_t again = ballot(live && (close || open || (kBiased && !a.sigmoid && inside)));
       if (ballot(inside) & ~again) {
         // otherwise the list itself in 64 bits, the one behind the last pick among it, and each to its rank
         const bool listed = e < E;
-        uint64_t c = 0u;
+        uint64_t exact = 0u;
         if (listed) {
-          const double x = Elem<DT>::to_f32(row[e]);
-          c = key_of(kBiased ? 1.0 / (1.0 + exp(-x)) + static_cast<double>(a.bias[e]) : x);
+          const double w = Elem<DT>::to_f32(row[e]);
+          exact = key_of(kBiased ? 1.0 / (1.0 + exp(-w)) + static_cast<double>(a.bias[e]) : w);
         }
-        if (l < listing) lds.fine[seg * kEntry + l] = c;
+        if (l < listing) lds.fine[seg * kEntry + l] = exact;
         wave_sync();
         int rank = 0;
         for (int j = 0; j < listing; ++j) {
           const uint64_t o = lds.fine[seg * kEntry + j];
-          rank += o > c || (o == c && o != 0u && entry[j] < e);
+          rank += o > exact || (o == exact && o != 0u && entry[j] < e);
         }
         wave_sync();
         if (listed && live && inside) entry[rank] = e;

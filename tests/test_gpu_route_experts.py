@@ -1,11 +1,13 @@
 """route_experts against the 64-bit reference: choices and order exactly, weights and gradients within bounds."""
+import itertools
+
 import pytest
 import torch
 
 from ae_amd import _lib
 from ae_amd._lib import SmxError
 from ae_amd.layers import route_experts, select_experts
-from tests.block_ref import F64, INF, choose, order_of, route
+from tests.block_ref import F64, INF, choose, order_of, route, scores
 from tests.product_ref import check
 
 pytestmark = pytest.mark.gpu
@@ -442,3 +444,93 @@ def test_the_serving_router_beside_it(renormalize):
     value, bound = route(logits, r.ids, "softmax", renormalize, 1.0)["weights"]
     check(r.weights, value, bound)
     check(w, value, 4 * bound)
+
+
+def _few_above(tokens, experts, base, step, most, seed, dtype=F32):
+    """Rows of `base`, with up to `most` experts of a row one to eight steps above it."""
+    g = _gen(seed + experts)
+    at = torch.rand((tokens, experts), generator=g, device=DEV).argsort(1) < torch.randint(0, most + 1, (tokens, 1), generator=g, device=DEV)
+    up = torch.randint(1, 9, (tokens, experts), generator=g, device=DEV)
+    return (base + torch.where(at, up, 0).double() * step).to(dtype)
+
+
+def _check_near_groups(logits, k, scoring, bias, what):
+    """Two of four groups, whose sums 64 bits may not tell apart.
+
+    A score in 64 bits is off by 2^-52 of itself in exp and 2^-53 in each of the sum 1 + exp and the quotient (a softmax's
+    sum is off too, but for all experts of a token alike), the sum of two by 2^-53 more: 5 * 2^-53 in all. Sums of two groups
+    that differ by less than twice that, 2^-49 of them to be safe, may come out in either order, here as there (two experts 8
+    and 2 steps of 1e-8 above zero, and two 6 and 4 above it, differ by 6e-16). Such tokens may take either group, and are
+    few: none of the tokens whose groups lie further apart is let off."""
+    ids = route_experts(logits, k, scoring, bias, 4, 2).ids.long()
+    want = choose(logits, k, scoring, bias, 4, 2)
+    two = torch.topk(scores(logits.to(F64), scoring).view(len(logits), 4, -1), 2, dim=2).values.sum(2)
+    size = logits.shape[1] // 4
+    for t in (ids != want).any(1).nonzero().flatten().tolist():
+        cut = two[t].sort(descending=True).values[1]
+        sure, able = two[t] > cut * (1 + 2.0 ** -49), two[t] >= cut * (1 - 2.0 ** -49)
+        assert int(able.sum()) > 2, (what, scoring, t)
+        ways = []
+        for kept in itertools.combinations(range(4), 2):
+            if all(bool(able[g]) for g in kept) and all(g in kept for g in range(4) if bool(sure[g])):
+                x = logits[t:t + 1].clone()
+                x.view(4, size)[[g for g in range(4) if g not in kept]] = -INF
+                ways.append(choose(x, k, scoring, bias, 1, 1)[0].tolist())
+        assert ids[t].tolist() in ways, (what, scoring, t)
+
+
+@pytest.mark.parametrize("tokens", [150, 1100])
+@pytest.mark.parametrize("k", [1, 4, 8, 16])
+@pytest.mark.parametrize("experts", [16, 64, 256, 512])
+def test_ties_beside_near_choices(experts, k, tokens):
+    """Choices that tie across the end of the picks, and a few that are larger by less than the keys hold."""
+    bias = torch.zeros(experts, device=DEV)
+    for most in (1, 5, experts):
+        ones = _few_above(tokens, experts, 1.0, 2.0 ** -23, most, k)
+        zeros = _few_above(tokens, experts, 0.0, 1e-7 / 8, most, k + 1)
+        what = f"up to {most}"
+        _check(ones, k, what=what, train=False)
+        for scoring in ("softmax", "sigmoid"):
+            for x in (ones, zeros, zeros.to(BF16)):
+                _check(x, k, scoring, bias, what=f"{what} {scoring}", train=False)
+            if k <= experts // 2:
+                _check(zeros, k, scoring, None, 4, 2, what=f"{what} {scoring}", train=False)
+                _check_near_groups(zeros, k, scoring, bias, what)
+
+
+@pytest.mark.parametrize("tokens", [500, 1500])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_routers_of_very_small_weights(dtype, tokens):
+    """A balance bias as it is initialised: scores that differ by little or nothing decide."""
+    for experts, k in ((256, 8), (64, 6), (512, 8), (128, 4)):
+        bias = torch.zeros(experts, device=DEV)
+        for spread in (1e-6, 3e-5, 1e-4, 1e-2):
+            x = _logits(tokens, experts, dtype, spread)
+            for scoring in ("softmax", "sigmoid"):
+                _check(x, k, scoring, bias, what=f"{experts} {spread} {scoring}", train=False)
+                _check(x, k, scoring, bias + 0.25, 4, 2, what=f"{experts} {spread} {scoring}", train=False)
+
+
+@pytest.mark.parametrize("tokens", [1, 1100])
+def test_the_one_larger_choice_behind_a_tie(tokens):
+    """One expert that the list of the nearest does not hold, or holds last."""
+    up = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0)).item()
+    for experts, at in ((64, 63), (64, 2), (256, 255), (512, 300), (16, 15)):
+        x = torch.ones((tokens, experts), device=DEV)
+        x[:, at] = up
+        for k in (1, 2, 6):
+            assert (_check(x, k, what=f"{experts} {at} {k}", train=False)[1][:, 0] == at).all()
+    zero = torch.zeros(256, device=DEV)
+    x = torch.full((tokens, 256), -2.0, device=DEV, dtype=BF16)
+    x[:, :9], x[:, 9] = 13.0, 13.0625  # sigmoids that saturate
+    assert (_check(x, 8, "sigmoid", zero, train=False)[1][:, 0] == 9).all()
+    x = torch.zeros((tokens, 64), device=DEV)
+    x[:, 40] = 1e-7
+    assert _check(x, 6, "sigmoid", zero[:64], train=False)[1][0].tolist() == [40, 0, 1, 2, 3, 4]
+    x[:, 40] = -1e-7  # a smaller one among the ties, in front of most of them
+    x[:, 2] = -1e-7
+    assert _check(x, 6, "sigmoid", zero[:64], train=False)[1][0].tolist() == [0, 1, 3, 4, 5, 6]
+    x[:, 2] = -INF
+    assert _check(x, 6, "sigmoid", zero[:64], train=False)[1][0].tolist() == [0, 1, 3, 4, 5, 6]
+    x[0, 30] = NAN
+    assert route_experts(x, 6, "sigmoid", zero[:64]).ids[0].tolist() == [30, 0, 1, 3, 4, 5]
