@@ -21,6 +21,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPicks = 16;
 constexpr int64_t kMaxCols = int64_t{1} << 24;
+constexpr int64_t kGridX = int64_t{1} << 22;  // workgroups along x (HIP takes less than 2^32 threads there); the rest goes along z
 
 struct MoveArgs {
   const char* x;         // one row a token: x, or the gradient of the sum
@@ -66,9 +67,11 @@ template <int DT, bool kVec> struct Part {
   }
 };
 
+__device__ __forceinline__ int64_t block_of() { return static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x; }
+
 // The token of a thread, and its chunk of the columns.
 __device__ __forceinline__ int64_t token_of(const MoveArgs& a) {
-  return static_cast<int64_t>(blockIdx.x) * (kThreads >> a.shift) + (threadIdx.x >> a.shift);
+  return block_of() * (kThreads >> a.shift) + (threadIdx.x >> a.shift);
 }
 template <int DT, bool kVec> __device__ __forceinline__ Part<DT, kVec> part_of(const MoveArgs& a) {
   const int width = 1 << a.shift, lane = static_cast<int>(threadIdx.x) & (width - 1);
@@ -154,7 +157,7 @@ __global__ __launch_bounds__(grad_threads<TPR>()) void combine_grad_kernel(MoveA
   using Sum = RowSum<TPR, K>;
   __shared__ typename Sum::Lds lds;
   int turn = 0;
-  const int64_t t = TPR == kWave ? static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + wave_id() : blockIdx.x;
+  const int64_t t = TPR == kWave ? block_of() * (kThreads / kWave) + wave_id() : block_of();
   const int tid = static_cast<int>(threadIdx.x) % TPR;
   if (t >= a.T) return;  // (whole waves; with TPR > kWave there is a workgroup a token)
   int p[K];
@@ -219,14 +222,18 @@ MoveArgs move_args(int64_t T, int64_t H, int64_t k, const int32_t* places) {
   return a;
 }
 
+// `blocks` workgroups of a part of the columns.
+dim3 grid_of(int64_t blocks, int64_t parts) {
+  return dim3(static_cast<unsigned>(std::min(blocks, kGridX)), static_cast<unsigned>(parts), static_cast<unsigned>((blocks + kGridX - 1) / kGridX));
+}
+
 template <typename Kernel>
 hipError_t launch_parts(Kernel kernel, MoveArgs& a, int64_t es, hipStream_t s) {
   const int64_t chunks = (a.H * es + 15) / 16;
   a.shift = 0;
   while (a.shift < 8 && (int64_t{1} << a.shift) < chunks) ++a.shift;
   const int64_t tokens = kThreads >> a.shift, width = int64_t{1} << a.shift;
-  const dim3 grid(static_cast<unsigned>((a.T + tokens - 1) / tokens), static_cast<unsigned>((chunks + width - 1) / width));
-  kernel<<<grid, kThreads, 0, s>>>(a);
+  kernel<<<grid_of((a.T + tokens - 1) / tokens, (chunks + width - 1) / width), kThreads, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -249,7 +256,7 @@ hipError_t launch_spread(int dtype, bool vec, MoveArgs& a, hipStream_t s) {
 template <int DT, bool kVec, int TPR>
 hipError_t launch_grad_picks(const MoveArgs& a, hipStream_t s) {
   constexpr int threads = grad_threads<TPR>(), tokens = threads / TPR;
-  const unsigned n = static_cast<unsigned>((a.T + tokens - 1) / tokens);
+  const dim3 n = grid_of((a.T + tokens - 1) / tokens, 1);
   if (a.k <= 2) combine_grad_kernel<DT, kVec, TPR, 2><<<n, threads, 0, s>>>(a);
   else if (a.k <= 4) combine_grad_kernel<DT, kVec, TPR, 4><<<n, threads, 0, s>>>(a);
   else if (a.k <= 8) combine_grad_kernel<DT, kVec, TPR, 8><<<n, threads, 0, s>>>(a);

@@ -441,3 +441,50 @@ def test_padded_batch():
     for t, v in pairs:
         assert float((t - v).abs().max()) <= 2 * 3 * 74 * 2.0 ** -24 * float(v.abs().max())
     assert not got[0][tokens - pad:].any() and not got[1][tokens - pad:].any()
+
+
+def _need(gib):
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < gib << 30:
+        pytest.skip(f"needs {gib} GiB of GPU memory")
+
+
+def test_tokens_beyond_a_grid_s_threads():
+    """A wave a token in the weights' gradient: 2^32 threads and more. Small whole numbers, so all results are exact."""
+    _need(40)
+    tokens = (1 << 26) + 5
+    at = torch.arange(tokens - 1, -1, -1, device=DEV)
+    rows = ((at[:, None] * torch.arange(1, 9, device=DEV)) % 7 - 3).to(BF16).requires_grad_()
+    w = ((at % 3) + 1).float()[:, None].requires_grad_()
+    y = combine_rows(rows, at.int()[:, None], w)
+    dy = ((at[:, None] + torch.arange(8, device=DEV)) % 5 - 2).to(BF16)
+    drows, dw = torch.autograd.grad([y], [rows, w], [dy])
+    with torch.no_grad():
+        assert torch.equal(y, rows.flip(0) * w.to(BF16))
+        assert torch.equal(drows, (dy * w.to(BF16)).flip(0))
+        assert torch.equal(dw[:, 0], (rows.flip(0).float() * dy.float()).sum(1))
+    (only,) = torch.autograd.grad([combine_rows(rows, at.int()[:, None], w.detach())], [rows], [dy])
+    assert torch.equal(only, drows)
+
+
+def test_wide_rows_beyond_a_grid_s_threads():
+    """A workgroup a token where rows are wide."""
+    _need(120)
+    tokens, cols = (1 << 24) + 3, 1032
+    at = torch.arange(tokens - 1, -1, -1, device=DEV)
+    tag = (at % 251).to(BF16)[:, None]
+    x = torch.empty((tokens, cols), dtype=BF16, device=DEV)
+    x.copy_(tag)
+    x[:, -1] = 1.0
+    rows = dispatch_rows(x, at.int()[:, None])
+    want = tag.flip(0).expand(tokens, cols - 1)
+    assert all(torch.equal(rows[i:i + (1 << 20), :-1], want[i:i + (1 << 20)]) for i in range(0, tokens, 1 << 20))
+    assert bool((rows[:, -1] == 1.0).all())
+    x.zero_()
+    del x
+    y = combine_rows(rows, at.int()[:, None])
+    want = tag.expand(tokens, cols - 1)
+    assert all(torch.equal(y[i:i + (1 << 20), :-1], want[i:i + (1 << 20)]) for i in range(0, tokens, 1 << 20))
+    assert bool((y[:, -1] == 1.0).all())
+    del rows, y, want
+    torch.cuda.empty_cache()
