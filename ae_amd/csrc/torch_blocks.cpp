@@ -4,11 +4,13 @@
 // pass for 46: a node of Python runs in the engine's thread, and waits for the interpreter there.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -128,10 +130,27 @@ bool records(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
-// Refuses forward-mode duals, whose tangents the kernels would drop.
-void no_tangents(const char* name, at::TensorList tensors) {
-  for (const Tensor& t : tensors)
-    if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error(text(name, " has no forward-mode derivative"));
+// Whether a trace is recorded: it would hold the allocation of a result and not the kernel that fills it.
+bool traced() {
+  using c10::impl::TorchDispatchModeKey, c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing()) return true;
+  if (!TorchDispatchModeTLS::any_modes_set()) return false;
+  for (const auto key : {TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FAKE, TorchDispatchModeKey::FUNCTIONAL})
+    if (TorchDispatchModeTLS::get_mode(key).has_value()) return true;
+  return false;
+}
+
+// Refuses what the kernels would not see: traces, tensors that stand for others under a transform, and the tangents of
+// forward-mode duals.
+void check_plain(const char* name, at::TensorList tensors) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrapped({DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper, DispatchKey::Batched, DispatchKey::Functionalize});
+  if (traced()) throw std::runtime_error(text(name, " cannot be traced"));
+  for (const Tensor& t : tensors) {
+    if (!t.defined()) continue;
+    if (t.key_set().has_any(wrapped)) throw std::runtime_error(text(name, " does not run under vmap or another transform of torch.func"));
+    if (t._fw_grad(0).defined()) throw std::runtime_error(text(name, " has no forward-mode derivative"));
+  }
 }
 
 // Where a graph of the gradients themselves is recorded, they depend on deps in a way that it cannot differentiate, and says so
@@ -147,7 +166,7 @@ struct Once : torch::autograd::Function<Once> {
 };
 
 template <typename Make> variable_list once(const char* name, variable_list deps, Make make) {
-  no_tangents(name, deps);
+  check_plain(name, deps);
   if (!c10::GradMode::is_enabled()) return failing(make);
   variable_list grads, some;
   {
@@ -270,7 +289,7 @@ struct Norm : torch::autograd::Function<Norm> {
 
 py::object norm(int kind, const Tensor& x, const Maybe& weight, const Maybe& bias, double eps, const Maybe& residual) {
   const Tensor w = defined(weight), b = defined(bias), r = defined(residual);
-  no_tangents(kNorm, {x, w, b, r});
+  check_plain(kNorm, {x, w, b, r});
   check_norm(x, w, b, eps, r);
   const bool train = records({&x, &w, &b, &r});
   const variable_list out = raising([&] {
@@ -370,7 +389,7 @@ struct Route : torch::autograd::Function<Route> {
 
 py::tuple route_experts(const Tensor& logits, int64_t top_k, const std::string& scoring, const Maybe& bias, int64_t num_groups,
                         std::optional<int64_t> top_groups, bool renormalize, double scale) {
-  no_tangents(kRoute, {logits});
+  check_plain(kRoute, {logits});
   const RouteOptions o{top_k, scoring == "softmax" ? SMX_SCORE_SOFTMAX : scoring == "sigmoid" ? SMX_SCORE_SIGMOID : -1, num_groups,
                        top_groups.value_or(num_groups), renormalize, scale};
   check_route(logits, scoring, defined(bias), o);
@@ -471,7 +490,7 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 Tensor dispatch_rows(const Tensor& x, const Tensor& places) {
-  no_tangents(kDispatch, {x});
+  check_plain(kDispatch, {x});
   check_matrix("x", x);
   check_places(places, x);
   if (places.size(0) != x.size(0))
@@ -482,7 +501,7 @@ Tensor dispatch_rows(const Tensor& x, const Tensor& places) {
 
 Tensor combine_rows(const Tensor& rows, const Tensor& places, const Maybe& weights, const Maybe& residual) {
   const Tensor w = defined(weights), r = defined(residual);
-  no_tangents(kCombine, {rows, w, r});
+  check_plain(kCombine, {rows, w, r});
   check_matrix("rows", rows);
   check_places(places, rows);
   const int64_t tokens = places.size(0), picks = tokens * places.size(1);

@@ -13,6 +13,7 @@ backward pass reads again.
 
 Calls run on the current stream of their tensors' device, without host synchronisation, and can be captured into a graph; a
 captured backward pass as fused_linear has it (no autograd graph of the same leaves from outside the capture alive).
+Traces (torch.jit.trace, make_fx, torch.export) and torch.func's transforms, which would not see the kernels, are refused.
 """
 from __future__ import annotations
 

@@ -7,7 +7,10 @@ import sys
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from ae_amd import _lib
 from ae_amd.build import BINDING_PATH
@@ -351,3 +354,41 @@ def test_forward_mode_refused():
                      lambda: dispatch_rows(d, p), lambda: combine_rows(torch.zeros(8, 8), p, residual=d)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+def _calls(x, p):
+    w, rows = torch.ones(8), torch.zeros(8, 8)
+    return {"rms_norm": lambda t: rms_norm(t, w), "layer_norm": lambda t: layer_norm(x, residual=t),
+            "route": lambda t: route_experts(t, 2).weights, "dispatch": lambda t: dispatch_rows(t, p),
+            "combine": lambda t: combine_rows(rows, p, residual=t)}
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "layer_norm", "route", "dispatch", "combine"])
+def test_traces_and_transforms_refused(name):
+    """A trace would hold an empty result without its kernel, and a transform's tensors stand for others."""
+    x, p = torch.zeros(4, 8), torch.zeros(4, 2, dtype=torch.int32)
+    call = _calls(x, p)[name]
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(call)(x)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(call, tracing_mode="fake")(x)
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="traced"):
+        call(torch.empty(4, 8))
+    for transform in (lambda f: torch.vmap(f)(x[None]), lambda f: torch.func.grad(lambda t: f(t).sum())(x),
+                      lambda f: torch.func.functionalize(f)(x), lambda f: torch.func.jacrev(f)(x)):
+        with pytest.raises(RuntimeError, match="torch.func"):
+            transform(call)
+    with pytest.raises(ValueError, match="GPU"):  # and again as before
+        call(x)
+
+
+def test_other_modes_stay():
+    """A mode that only looks on (of a checkpoint's, a counter of operations) is no trace."""
+    class Looks(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Looks(), pytest.raises(ValueError, match="GPU"):
+        rms_norm(torch.zeros(4, 8))

@@ -400,3 +400,19 @@ def test_a_large_mean_over_fewer_columns_than_threads(cols):
     # Sums of small integers are exact; roundings: eps to fp32 (half of it in its root), rsqrt (1 ulp, two half steps),
     # and the product: 3.5 half steps.
     assert ((dx.double() - want).abs() <= 4 * 2.0 ** -24 * want.abs()).all()
+
+
+def test_batched_gradients_refused():
+    """torch.autograd.grad over a batch of gradients runs the backward pass on tensors that stand for others."""
+    x = torch.randn(3, 8, device=DEV, requires_grad=True)
+    y = rms_norm(x)
+    with pytest.raises(RuntimeError, match="vmap"):
+        torch.autograd.grad(y, x, torch.ones(2, 3, 8, device=DEV), is_grads_batched=True)
+
+
+def test_compiled_around():
+    """torch.compile leaves the call as it is, between what it compiles."""
+    x, w = torch.randn(30, 64, device=DEV), torch.randn(64, device=DEV)
+    call = torch.compile(lambda t: 2.0 * rms_norm(t + 1.0, w), backend="eager")
+    assert torch.equal(call(x), 2.0 * rms_norm(x + 1.0, w))
+    assert torch.equal(call(x + 1.0), 2.0 * rms_norm((x + 1.0) + 1.0, w))  # (rounded in the same steps)
