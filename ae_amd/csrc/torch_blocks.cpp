@@ -96,7 +96,8 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 void* address(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 template <typename T> T* address(const Tensor& t) { return static_cast<T*>(address(t)); }
 
-Tensor dense(const Tensor& t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+// Elements side by side, with their sign (z.conj().imag keeps it in a flag of the tensor).
+Tensor dense(const Tensor& t) { return !t.defined() || (t.is_contiguous() && !t.is_neg()) ? t : t.resolve_neg().contiguous(); }
 Tensor defined(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 
 Tensor empty(c10::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
@@ -115,6 +116,7 @@ struct Rows {
     if (!t.defined()) return;
     const int64_t n = t.size(-1);
     stride = n;
+    if (t.is_neg()) t = t.resolve_neg();
     if (t.is_contiguous()) return;
     if (t.dim() != 2) t = t.reshape({-1, n});
     if ((t.stride(1) != 1 && n != 1) || (t.stride(0) < n && t.size(0) > 1)) t = t.contiguous();
@@ -407,7 +409,7 @@ void check_matrix(const char* name, const Tensor& t) {
 }
 
 void check_places(const Tensor& places, const Tensor& rows) {
-  if (places.scalar_type() != at::kInt || places.dim() != 2 || !places.is_contiguous())
+  if (places.scalar_type() != at::kInt || places.dim() != 2 || !places.is_contiguous() || places.is_neg())
     throw py::type_error("places must be a contiguous int32 matrix [T, k]");
   if (places.device() != rows.device())
     throw py::value_error(text("expected a GPU tensor, places is on ", places.device().str(), ", the rows on ", rows.device().str()));

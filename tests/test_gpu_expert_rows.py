@@ -488,3 +488,33 @@ def test_wide_rows_beyond_a_grid_s_threads():
     assert bool((y[:, -1] == 1.0).all())
     del rows, y, want
     torch.cuda.empty_cache()
+
+
+def test_signs_kept_in_a_flag():
+    """The imaginary part of a conjugate is the memory's numbers with the other sign."""
+    g = _gen(3)
+    z = torch.complex(_randn(g, 12, 1), _randn(g, 12, 1))
+    column = z.conj().imag
+    assert column.is_neg()
+    places, order = _places(12, 2)
+    assert torch.equal(dispatch_rows(column, places), dispatch_rows(-z.imag, places))
+
+    x, r, w, b, dy, rows, dr = (_randn(g, *s) for s in ((12, 64), (12, 64), (64,), (64,), (12, 64), (24, 64), (24, 64)))
+    share = torch.rand((12, 2), generator=g, device=DEV)
+
+    def grads(call, leaves, given):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        outs = call(*leaves)
+        outs = outs if isinstance(outs, tuple) else (outs,)
+        return [*outs, *torch.autograd.grad(outs, leaves, given)]
+
+    for call, leaves, given in ((lambda x, r, w: rms_norm(x, w, residual=r), (x, r, w), (dy, x)),
+                                (lambda x, w, b: layer_norm(x, w, b), (x, w, b), (dy,)),
+                                (lambda x: route_experts(x, 2, "sigmoid", torch._neg_view(-w)).weights, (x,), (share,)),
+                                (lambda x: dispatch_rows(x, places), (x,), (dr,)),
+                                (lambda x, s, r: combine_rows(x, places, s, r), (rows, share, r), (dy,))):
+        want = grads(call, leaves, given)
+        got = grads(call, [torch._neg_view(-t) for t in leaves], [torch._neg_view(-t) for t in given])
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with pytest.raises(TypeError, match="places"):
+        dispatch_rows(x, torch._neg_view(-places))
