@@ -10,7 +10,8 @@ reference has no counterpart: it leaves such products to torch.
 Contract: everything runs on the current stream of x's device, without host synchronisation, so
 the calls can be captured into a graph. A backward pass can be captured too, but not while an
 autograd graph of the same leaves built outside the capture is still alive (torch's gradient
-accumulation would join the capture from another stream): drop its outputs first.
+accumulation would join the capture from another stream): drop its outputs first. Traces (torch.jit.trace, make_fx,
+torch.export), which would not see the kernels, are refused.
 """
 from __future__ import annotations
 
@@ -27,6 +28,8 @@ from ._torch import dtype_code, workspace
 _ACTIVATIONS = _lib.ACTIVATIONS
 _SWIGLU = _ACTIVATIONS["swiglu"]
 _raw_stream = torch._C._cuda_getCurrentRawStream  # of a device index: the hipStream_t itself
+_jit_trace, _modes, _mode = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
+_TRACES = tuple(torch._C._TorchDispatchModeKey.__members__.values())  # (of make_fx, fake and functional tensors)
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -230,7 +233,7 @@ class _Once(torch.autograd.Function):
 
 
 def _gradients(ctx, dy):
-    _no_tangents(dy)
+    _check_plain(dy)
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     grads = (None, None, None)
     if need_x or need_w or need_b:
@@ -238,15 +241,18 @@ def _gradients(ctx, dy):
     return (*grads, dy if need_r else None, None, None, None, None)
 
 
-def _no_tangents(*tensors) -> None:
-    """Refuses forward-mode duals, whose tangents the kernels would drop."""
+def _check_plain(*tensors) -> None:
+    """Refuses traces, which would hold an empty result without its kernel, and forward-mode duals, whose tangents the
+    kernels would drop."""
+    if _jit_trace() is not None or (_modes() and any(_mode(key) is not None for key in _TRACES)):
+        raise RuntimeError("fused_linear and grouped_linear cannot be traced")
     if forward_ad._current_level >= 0 and any(
             t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("fused_linear and grouped_linear have no forward-mode derivative")
 
 
 def _run(x, weight, bias, activation, residual, offsets, slots, out):
-    _no_tangents(x, weight, bias, residual, out)
+    _check_plain(x, weight, bias, residual, out)
     sizes, strides = _check(x, weight, bias, activation, residual, offsets, slots, out)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad) or

@@ -7,6 +7,7 @@ import re
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from ae_amd import _lib
 from ae_amd.layers import fused_linear, grouped_linear
@@ -211,3 +212,16 @@ def test_forward_mode_refused(which):
                 call(**args)
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda v: fused_linear(**{**t, which: v}), (t[which],), (t[which],))
+
+
+@pytest.mark.parametrize("which", ["fused", "grouped"])
+def test_traces_refused(which):
+    """A trace would hold an empty result without its kernel."""
+    x, w, off = torch.zeros(4, 8), torch.zeros(2, 8, 8), torch.tensor([0, 2, 4])
+    call = (lambda t: fused_linear(t, w[0])) if which == "fused" else (lambda t: grouped_linear(t, w, off))
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(call, (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(call)(x)
+    with pytest.raises(ValueError, match="GPU"):  # and again as before
+        call(x)
