@@ -416,3 +416,27 @@ def test_compiled_around():
     call = torch.compile(lambda t: 2.0 * rms_norm(t + 1.0, w), backend="eager")
     assert torch.equal(call(x), 2.0 * rms_norm(x + 1.0, w))
     assert torch.equal(call(x + 1.0), 2.0 * rms_norm((x + 1.0) + 1.0, w))  # (rounded in the same steps)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,cols,offset", [(70001, 128, 0), (70001, 128, 1), (131077, 64, 0), (40003, 256, 0), (20011, 512, 3),
+                                              (30001, 1024, 0), (20011, 2048, 0), (9001, 4096, 0), (5003, 16384, 0)])
+def test_no_row_is_left_out_of_the_column_sums(rows, cols, offset, dtype):
+    """Rows of +-1 whose mean is 0 and whose variance is 1, small whole gradients: every sum is a whole number below
+    2^24, so the parameters' gradients in 32 bits are exact, and a row too few or too many shows."""
+    g = _gen(rows + cols)
+    sign = torch.where(torch.randperm(cols, generator=g, device=DEV) < cols // 2, 1.0, -1.0)
+    flip = torch.where(torch.rand((rows, 1), generator=g, device=DEV) < 0.5, 1.0, -1.0)
+    wide = torch.empty((rows, cols + 8), dtype=dtype, device=DEV)
+    x = wide[:, offset:offset + cols] if offset else torch.empty((rows, cols), dtype=dtype, device=DEV)
+    x.copy_(flip * sign)
+    dy = torch.randint(-2, 3, (rows, cols), generator=g, device=DEV).to(dtype)
+    w = torch.ones(cols, device=DEV, requires_grad=True)
+    b = torch.zeros(cols, device=DEV, requires_grad=True)
+    sums = (dy.float() * x.float()).sum(0, dtype=F64), dy.sum(0, dtype=F64)
+    y = rms_norm(x, w, 0.0)
+    assert torch.equal(y.detach(), x)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0].double(), sums[0])
+    y = layer_norm(x, w, b, 0.0)
+    assert torch.equal(y.detach(), x)
+    assert all(torch.equal(p.double(), q) for p, q in zip(torch.autograd.grad(y, [w, b], dy), sums))
