@@ -87,6 +87,15 @@ __device__ __forceinline__ uint64_t key_of(double v) {
   return (u >> 63) ? ~u : (u | (uint64_t{1} << 63));
 }
 
+// The sum of a group's two best choices (next 0: there is one). Sums behind the largest finite number are that: they lie as near
+// as can be, and 64 bits tell them apart.
+__device__ __forceinline__ uint32_t key_of_two(uint32_t best, uint32_t next) {
+  if (best == 0u) return 0u;
+  constexpr float kMost = 0x1.fffffep+127f;
+  const float s = value_of(best) + (next != 0u ? value_of(next) : 0.0f);
+  return s != s ? 0xffffffffu : key_of(fminf(fmaxf(s, -kMost), kMost));
+}
+
 template <int L> __device__ __forceinline__ float sum_over(float v) {
   return group_reduce<L>(v, [](float a, float b) { return a + b; });
 }
@@ -348,7 +357,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         if (share >= 4) join(integral_constant<int, kDppXor2>{});
         if (share >= 8) join(integral_constant<int, kDppHalfMirror>{});
         if (share >= 16) join(integral_constant<int, kDppMirror>{});
-        if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
+        if constexpr (kBiased) best = key_of_two(best, next);
         const bool real = l * PL < E;
         bool keep;
         if constexpr (L == kWave) {
@@ -390,7 +399,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
             next = next > less ? next : less;
             best = best > c ? best : c;
           }
-          if (kBiased && next != 0u) best = key_of(value_of(best) + value_of(next));
+          if constexpr (kBiased) best = key_of_two(best, next);
           lds.group[seg][g] = best;
         }
         wave_sync();

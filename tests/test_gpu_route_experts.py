@@ -534,3 +534,19 @@ def test_the_one_larger_choice_behind_a_tie(tokens):
     assert _check(x, 6, "sigmoid", zero[:64], train=False)[1][0].tolist() == [0, 1, 3, 4, 5, 6]
     x[0, 30] = NAN
     assert route_experts(x, 6, "sigmoid", zero[:64]).ids[0].tolist() == [30, 0, 1, 3, 4, 5]
+
+
+@pytest.mark.parametrize("tokens", [3, 1100])
+@pytest.mark.parametrize("experts,groups", [(64, 8), (60, 5), (128, 4), (256, 8), (256, 64), (512, 8)])
+def test_groups_whose_sums_leave_32_bits(experts, groups, tokens):
+    """Finite biases whose sum of two is behind the largest number of 32 bits: larger groups are still larger."""
+    size = experts // groups
+    bias = torch.zeros(experts, device=DEV).view(groups, size)
+    bias[:, :2] = torch.linspace(2e38, 3e38, groups, device=DEV)[:, None]
+    one = bias.clone()
+    one[groups - 1, 0] = INF  # (a sum of infinity is larger still)
+    low = torch.where(bias == 0, -3.2e38, -bias)
+    for order in (bias, bias.flip(0), bias[torch.randperm(groups, generator=_gen(groups), device=DEV)], low, low.flip(0), one):
+        for scoring in ("softmax", "sigmoid"):
+            _check(_logits(tokens, experts), 2, scoring, order.flatten(), groups, 1, train=False)
+            _check(_logits(tokens, experts), 3, scoring, order.flatten(), groups, 2, train=False)
