@@ -261,6 +261,11 @@ __device__ __forceinline__ void block_scan(int32_t* v, int n, int32_t* waves) {
   __syncthreads();
 }
 
+// Waves of a SIMD at least. Four tokens a wave, 16 experts and their biases a lane take just over 128 registers, which leaves a CU
+// one workgroup of 8 waves instead of two (65536 tokens over 256 experts in groups 90 us for 67, 8191 the same); the others
+// take less, or nothing from it.
+template <int L, int PL, bool kBiased> constexpr int pick_waves() { return L == 16 && PL == 16 && kBiased ? 4 : 1; }
+
 // The keys that the rounds compare are the choices' with the expert's number in their low bits, so that one comparison finds
 // an expert, takes it out and settles ties:
 //   plain logits of 16 bits  all ten bits of it (1023 - e): their fp32 images have 13 low bits that say nothing. The keys of a
@@ -268,7 +273,7 @@ __device__ __forceinline__ void block_scan(int32_t* v, int n, int32_t* waves) {
 //   otherwise                the number within the lane (PL - 1 - i, up to four bits). Lanes that tie in the rest of the key
 //                            are settled by their order. What these bits and fp32 itself leave open is looked at afterwards.
 template <int DT, int L, int PL, bool kBiased>
-__global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool whole) {
+__global__ __launch_bounds__(kPickThreads, (pick_waves<L, PL, kBiased>())) void pick_kernel(PickArgs a, bool whole) {
   constexpr int kTokens = kWave / L;
   constexpr bool kExact = DT != kF32 && !kBiased;
   constexpr uint32_t kCode = kExact ? kMaxE - 1 : PL - 1;
@@ -514,6 +519,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(PickArgs a, bool who
         const float xk = __shfl(x, at_last, kWave), pk = __shfl(p, at_last, kWave), ck = __shfl(c, at_last, kWave);
         const uint32_t below = key_of(ck - 1.1f * reach(ck, ck)) & ~kCode, least = below != 0u ? below : 1u;
         bool other = apart & ((uint64_t{2} << k) - 1);
+        if constexpr (PL == 16) load_run<DT, PL>(a.logits, at, opaque(l * PL), E, whole, v);  // (kept, they take 16 registers of every token)
 #pragma unroll
         for (int i = 0; i < PL; ++i) {
           bool same = v[i] == xk;
