@@ -2,10 +2,10 @@
 //
 //   norm_kernel        s = x + residual, y = (s - mean) rstd w + b: a row stays in the registers of its threads, so that the mean,
 //                      the mean square of the differences from it, and the result are three passes over registers and one over
-//                      memory. Bound by memory: 16384 rows of 4096 in bf16 with a residual 87-100 us (537 MB, 5.4-6.2 TB/s; a
-//                      copy of 2 GiB runs at 4.9), 131072 rows of 128 11 us (6 TB/s), one row of 2048 2.2 us.
+//                      memory. Bound by memory: 16384 rows of 4096 in bf16 with a residual 86-87 us (537 MB, 6.2 TB/s; a
+//                      copy of 2 GiB runs at 4.9), 131072 rows of 128 12 us (5.4 TB/s), one row of 2048 2.1 us.
 //   norm_grad_kernel   dx, and the workgroup's partial sums of dw and db over the rows that it walks over. Bound by memory: the
-//                      same rows 102-111 us (537 MB and 8 MB of partial sums, 4.8-5.3 TB/s); 131072 rows of 128 19 us (5.3).
+//                      same rows 109-111 us (537 MB and 8 MB of partial sums, 4.9-5.0 TB/s); 131072 rows of 128 19 us (5.3).
 //   norm_fold_kernel   the partial sums added up, in a fixed order: 4-5 us, of which two are the launch.
 //
 // Threads of a row: 16 to 1024, so that a thread has one 16-byte chunk of most widths; a workgroup of 256 holds several short

@@ -11,12 +11,14 @@
 // Everything is counted in integers and in the order of the picks, so the order is the stable one on every run.
 //
 // Bound by the instructions of the choice, not by the logits' bytes (8191 tokens over 256 experts in fp32: 8.4 MB, 2 us): 4
-// tokens a wave, about 490 vector instructions a token with groups and a bias. Measured, in bf16 unless said:
-//   1 token, 64 experts, 6 picks                                         4.8 us, one launch
-//   8191 tokens, 256 experts in 8 groups, bias, 8 picks, fp32            picks 15, places 7.1 us (at first 33, and 12 in two)
+// tokens a wave, about 490 vector instructions a token with groups and a bias, 200 without. The gradient is bound by the
+// comparison of each of a lane's experts with each pick (153 instructions a token over 256 experts with 8 picks, 272 in the
+// dense form; issued at four cycles each they take 16 and 29 us of 65536 tokens). Measured, in bf16 unless said:
+//   1 token, 64 experts, 6 picks                                         4.4 us, one launch
+//   8191 tokens, 256 experts in 8 groups, bias, 8 picks, fp32            picks 15, places 7.0 us (at first 33, and 12 in two)
 //   65536 tokens, the same                                               68 us with the order, 50 without
-//   65536 tokens, 256 experts, 8 picks, no groups, no bias               42 and 24 us
-//   16384 tokens, 64 experts, 6 picks                                    picks 8.2, places 5.6, gradient 5.5 us
+//   65536 tokens, 256 experts, 8 picks, no groups, no bias               41 and 24 us, gradient 19 (of all scores: 29)
+//   16384 tokens, 64 experts, 6 picks                                    picks 8.0, places 5.4, gradient 5.4 us
 #include <algorithm>
 
 #include "blocks.h"
@@ -241,7 +243,7 @@ __device__ __forceinline__ void pick_exactly(const PickArgs& a, int64_t t, uint6
   }
 }
 
-// Exclusive prefix sums over n <= 4 * 1025 counts in LDS, by the whole workgroup (of at least one wave).
+// Exclusive prefix sums over n <= 1025 counts in LDS, by the whole workgroup (of at least one wave).
 __device__ __forceinline__ void block_scan(int32_t* v, int n, int32_t* waves) {
   const int threads = static_cast<int>(blockDim.x), per = (n + threads - 1) / threads;
   const int first = static_cast<int>(threadIdx.x) * per;
@@ -626,7 +628,7 @@ __global__ __launch_bounds__(kPickThreads, (pick_waves<L, PL, kBiased>())) void 
   }
 }
 
-// counts [blocks][E + 1] -> exclusive prefix sums over the workgroups, and the totals. A workgroup takes kScanCols experts;
+// counts [blocks][pitch] -> exclusive prefix sums over the workgroups, and the totals. A workgroup takes kScanCols experts;
 // 64 threads an expert take a share of the workgroups each.
 __global__ __launch_bounds__(kScanCols * kWave) void pick_scan_kernel(PickArgs a) {
   __shared__ int32_t sums[kWave][kScanCols + 1];

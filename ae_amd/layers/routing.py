@@ -33,7 +33,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     top_k <= 16).
 
     Scores are the logits' softmax or sigmoid. A token's experts are those of the largest score + ``bias``
-    (``[E]``, the bias that balances the experts' loads; it moves the choice only), in that order, ties to the
+    (``[E]``, read in fp32, the bias that balances the experts' loads; it moves the choice only), in that order, ties to the
     lower expert, compared as exact scores would be. With ``num_groups`` > 1 only the ``top_groups`` best groups of
     consecutive experts are selectable (default: all): by their best expert, or with a bias by their two
     best. Weights are the scores, divided by their sum over the token's picks (``renormalize``), times
